@@ -341,6 +341,96 @@ int pkv_paged_attention_multi_dev(pkv_backend *b, int64_t layer, const void *q, 
 int pkv_paged_attention_plan_dev(pkv_backend *b, const int32_t *context_lens, int64_t num_seqs,
                                  int64_t max_context_len, void *stream);
 
+/* ---- one layer of a model's step over ragged new tokens -----------------------
+ * rope_and_cache, then attention of the same tokens: over their own rows for
+ * whole prompts (prompt_attention), over the cache for later chunks and for
+ * decoded tokens (paged_attention_chunk), which read the cu_seqlens that
+ * rope_and_cache wrote. No counterparts in the reference. */
+
+/* Appends the new tokens' keys and values to layer `layer` of the pool, the
+ * queries and keys rotated by their positions on the way (one launch).
+ * Sequence s has ctx_lens[s] cached tokens and new_lens[s] new ones; its token
+ * i sits at position p = ctx_lens[s] + i and takes the slot that
+ * pkv_resolve_and_cache_dev would give it. q is [num_tokens][num_q_heads]
+ * [head_dim] (row pitch q_token_stride elements; num_q_heads 0: no queries), k
+ * and v are [num_tokens][kv heads held here][head_dim] (row pitch
+ * kv_token_stride); a pitch <= 0 is dense, so rows may be columns of a fused
+ * projection's output. For pair j of a head, with c = cos_sin[p][j] and n =
+ * cos_sin[p][rotary_dim / 2 + j]:
+ *   a' = a * c - b * n,  b' = b * c + a * n
+ * in f32, where the pair is elements (j, j + rotary_dim / 2), or (2j, 2j + 1)
+ * with `interleaved` set; elements from rotary_dim on pass through. cos_sin is
+ * f32 [max_position][rotary_dim] in device memory, the cosines of a position
+ * first; rotary_dim is even, 2 <= rotary_dim <= head_dim.
+ * q_out receives the rotated queries (NULL: written over q), k_out, if given,
+ * the rotated keys as rows (it may be k), each rounded once to src_dtype; the
+ * cache takes them rounded once from f32 (quantised as pkv_set_kv_scales says
+ * for an fp8 pool). src_dtype is f32, bf16 or f16 and equals the pool type, or
+ * the pool is fp8. Other overlaps of outputs with inputs are not allowed.
+ * Writes cu_seqlens[0..num_seqs] and, if given, slot_mapping. The sum of
+ * new_lens may be less than num_tokens (a padded batch): rows past it are left
+ * as they were. More, or a negative length, is recorded as ShapeMismatch and
+ * nothing but cu_seqlens is written. A token whose position is not in cos_sin
+ * is recorded (ShapeMismatch) and skipped, slot -1; one past its table
+ * (SlotOutOfRange) or with a bad block id (InvalidBlock) is rotated but not
+ * cached, slot -1. Two tokens must not share a slot. */
+int pkv_rope_and_cache_dev(pkv_backend *b, const int32_t *block_tables, int64_t table_stride,
+                           const int32_t *ctx_lens, const int32_t *new_lens, int64_t num_seqs,
+                           int64_t num_tokens, int32_t *cu_seqlens, int64_t *slot_mapping,
+                           int64_t layer, const void *q, int64_t q_token_stride,
+                           int64_t num_q_heads, void *q_out, int64_t q_out_stride, const void *k,
+                           const void *v, int64_t kv_token_stride, void *k_out,
+                           int64_t k_out_stride, int src_dtype, const float *cos_sin,
+                           int64_t max_position, int64_t rotary_dim, int interleaved,
+                           void *stream);
+/* Causal attention of a ragged chunk of new tokens over layer `layer` of the
+ * pool, their own keys and values already cached. Sequence s has the packed
+ * rows cu_seqlens[s] .. cu_seqlens[s + 1] (int32, device memory) of q and out;
+ * its row i sits at position ctx_lens[s] + i, where ctx_lens counts the tokens
+ * cached BEFORE the chunk (as for pkv_rope_and_cache_dev), and attends keys 0
+ * .. that position. Any mix of lengths, 0 and 1 (decoded tokens) among them.
+ * q is [num_tokens][num_q_heads][head_dim] in query_dtype (as
+ * pkv_paged_attention_typed_dev), row pitch q_token_stride elements (<= 0:
+ * dense; else a multiple of 8); out is dense; lse (optional, f32
+ * [num_tokens][num_q_heads]) receives log(sum exp(scale * q.k)). head_dim 64,
+ * 128 or 256, block_size a multiple of 16, at most 128 query heads per kv head.
+ * max_new_len bounds every sequence's rows and max_context_len every ctx_lens
+ * + rows (it must fit the tables); a sequence beyond either, or with a
+ * negative ctx_lens, is recorded as ShapeMismatch and its rows are zeros (lse
+ * -inf). Rows of cu_seqlens outside [0, num_tokens] or out of order are
+ * recorded and not touched, nor are rows of no sequence. Keys in blocks
+ * outside the pool are recorded (InvalidBlock) and skipped; a row left with no
+ * key gives zeros and -inf. Positions that a row does not attend may hold
+ * anything, NaN and infinities included.
+ *
+ * Uses the handle's prefill workspace (a fixed size, see
+ * pkv_attention_reserve). */
+int pkv_paged_attention_chunk_dev(pkv_backend *b, int64_t layer, const void *q, int query_dtype,
+                                  int64_t q_token_stride, int64_t num_q_heads,
+                                  const int32_t *cu_seqlens, int64_t num_seqs, int64_t num_tokens,
+                                  int64_t max_new_len, const int32_t *block_tables,
+                                  int64_t table_stride, const int32_t *ctx_lens,
+                                  int64_t max_context_len, float softmax_scale, void *out,
+                                  float *lse, void *stream);
+/* Causal attention over whole packed prompts, from their rows (nothing is read
+ * from the pool, whatever its type; the backend gives the kv heads held here,
+ * head_dim and the workspace). k and v are [num_tokens][kv heads][head_dim] of
+ * the queries' type (bf16 or f16), row pitch kv_token_stride elements (<= 0:
+ * dense; else a multiple of 8), 16-byte aligned. Sequence s is the rows
+ * cu_seqlens[s] .. cu_seqlens[s + 1]; its row i attends its rows 0 .. i.
+ * max_len bounds every sequence. Otherwise as pkv_paged_attention_chunk_dev. */
+int pkv_prompt_attention_dev(pkv_backend *b, const void *q, const void *k, const void *v, int dtype,
+                             int64_t q_token_stride, int64_t kv_token_stride, int64_t num_q_heads,
+                             const int32_t *cu_seqlens, int64_t num_seqs, int64_t num_tokens,
+                             int64_t max_len, float softmax_scale, void *out, float *lse,
+                             void *stream);
+/* Allocates the prefill workspace that the two calls above share (its size is
+ * fixed by head_dim; about 40 MB at 128). Without it the first of them
+ * allocates, which a stream capture does not allow: reserve once before
+ * capturing. Calls on one handle that run concurrently on different streams
+ * share the workspace and must be ordered. */
+int pkv_attention_reserve(pkv_backend *b);
+
 /* Order-independent 64-bit digests of this backend's K and V planes (the
  * element's global index in the full plane and its f32-widened bits, summed;
  * zeros contribute nothing). Digests of the shards of one pool add up

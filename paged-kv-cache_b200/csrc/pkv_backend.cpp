@@ -1124,6 +1124,255 @@ Status B200Backend::paged_attention_plan_dev(const int32_t *ctx, int64_t num_seq
     return Status::Ok();
 }
 
+// The kv heads held here, for calls that work on whole heads.
+Status B200Backend::whole_heads(const char *what, int64_t *kv_heads) const {
+    const uint64_t hd = cfg_.head_dim;
+    if (hd == 0 || shard_entry_ == 0 || elem_offset() % hd != 0 || shard_entry_ % hd != 0)
+        return error(PKV_ERR_DEVICE, 0, 0, std::string(what) + " needs whole kv heads in this shard");
+    *kv_heads = (int64_t)(shard_entry_ / hd);
+    return Status::Ok();
+}
+
+Status B200Backend::rope_and_cache_dev(const int32_t *tables, int64_t table_stride,
+                                       const int32_t *ctx, const int32_t *new_lens,
+                                       int64_t num_seqs, int64_t num_tokens, int32_t *cu,
+                                       int64_t *slots_out, int64_t layer, const void *q,
+                                       int64_t q_stride, int64_t num_q_heads, void *q_out,
+                                       int64_t q_out_stride, const void *k, const void *v,
+                                       int64_t kv_stride, void *k_out, int64_t k_out_stride,
+                                       DType src, const float *cos_sin, int64_t max_position,
+                                       int64_t rotary_dim, int interleaved, cudaStream_t st) {
+    if (layer < 0 || (uint64_t)layer >= cfg_.num_layers)
+        return error(PKV_ERR_INVALID_LAYER, layer, (int64_t)cfg_.num_layers,
+                     msg_layer((uint64_t)layer, cfg_.num_layers));
+    if (num_seqs < 0 || num_tokens < 0 || table_stride < 0)
+        return error(PKV_ERR_SHAPE_MISMATCH, 0, std::min({num_seqs, num_tokens, table_stride}),
+                     "negative size");
+    if (num_seqs > kMaxResolveSeqs)
+        return error(PKV_ERR_DEVICE, 0, 0,
+                     "slot resolution handles at most " + std::to_string(kMaxResolveSeqs) +
+                         " sequences per call");
+    if (num_tokens > std::numeric_limits<int32_t>::max())
+        return error(PKV_ERR_SHAPE_MISMATCH, std::numeric_limits<int32_t>::max(), num_tokens,
+                     "too many tokens for int32 cu_seqlens");
+    if (src != DType::F32 && src != DType::BF16 && src != DType::F16)
+        return error(PKV_ERR_DEVICE, 0, 0, "rope_and_cache rotates f32, bf16 or f16 rows");
+    if (dtype_ != DType::FP8_E4M3 && src != dtype_)
+        return error(PKV_ERR_DEVICE, 0, 0,
+                     "rope_and_cache rows have the pool's type, or go to an fp8 pool");
+    int64_t kv = 0;
+    Status held = whole_heads("rope_and_cache", &kv);
+    if (!held.ok()) return held;
+    const int64_t hd = (int64_t)cfg_.head_dim;
+    const int64_t most = std::numeric_limits<int32_t>::max() / 4;  // heads and elements in 32 bits
+    if (num_q_heads < 0 || num_q_heads > most / hd || kv > most / hd)
+        return error(PKV_ERR_SHAPE_MISMATCH, 0, num_q_heads, "query head count out of range");
+    if (rotary_dim < 2 || rotary_dim > hd || rotary_dim % 2 != 0)
+        return error(PKV_ERR_SHAPE_MISMATCH, hd, rotary_dim,
+                     "rotary_dim must be even, at least 2 and at most head_dim");
+    if (max_position <= 0)
+        return error(PKV_ERR_SHAPE_MISMATCH, 1, max_position, "the angle table has no positions");
+    if (!cu || (num_seqs > 0 && (!ctx || !new_lens)) ||
+        (num_tokens > 0 && (!tables || !k || !v || !cos_sin || (num_q_heads > 0 && !q))))
+        return error(PKV_ERR_DEVICE, 0, 0, "null device pointer");
+    if (num_q_heads > 0 && !q_out) {  // in place
+        q_out = const_cast<void *>(q);
+        q_out_stride = q_stride;
+    }
+    const struct {
+        int64_t *stride, least;
+        bool used;
+        const char *what;
+    } rows[] = {{&q_stride, num_q_heads * hd, num_q_heads > 0, "query row pitch shorter than its heads"},
+                {&q_out_stride, num_q_heads * hd, num_q_heads > 0, "rotated query row pitch shorter than its heads"},
+                {&kv_stride, kv * hd, true, "key and value row pitch shorter than an entry"},
+                {&k_out_stride, kv * hd, k_out != nullptr, "rotated key row pitch shorter than an entry"}};
+    for (const auto &r : rows) {
+        if (*r.stride <= 0) *r.stride = r.least;
+        if (r.used && *r.stride < r.least) return error(PKV_ERR_SHAPE_MISMATCH, r.least, *r.stride, r.what);
+    }
+    DeviceGuard g(device_);
+    const size_t layer_bytes = (size_t)layer * slots_per_layer() * entry_bytes();
+    RopeCacheLaunch a{};
+    a.tables = tables;
+    a.table_stride = table_stride;
+    a.ctx_lens = ctx;
+    a.new_lens = new_lens;
+    a.num_seqs = num_seqs;
+    a.num_tokens = num_tokens;
+    a.block_size = (long long)cfg_.block_size;
+    a.num_blocks = (long long)cfg_.num_blocks;
+    a.cu_seqlens = cu;
+    a.slots_out = reinterpret_cast<long long *>(slots_out);
+    a.q = q;
+    a.q_stride = q_stride;
+    a.q_out = q_out;
+    a.q_out_stride = q_out_stride;
+    a.k = k;
+    a.v = v;
+    a.kv_stride = kv_stride;
+    a.k_out = k_out;
+    a.k_out_stride = k_out_stride;
+    a.k_layer = static_cast<char *>(k_plane_) + layer_bytes;
+    a.v_layer = static_cast<char *>(v_plane_) + layer_bytes;
+    a.num_q_heads = (int)num_q_heads;
+    a.kv_heads = (int)kv;
+    a.head_dim = (int)hd;
+    a.rotary_dim = (int)rotary_dim;
+    a.interleaved = interleaved != 0;
+    a.cos_sin = cos_sin;
+    a.max_position = max_position;
+    if (dtype_ == DType::FP8_E4M3) {
+        const long long at = layer * (long long)cfg_.num_kv_heads + (long long)(elem_offset() / hd);
+        a.k_inv = fp8_scales().k_inv + at;
+        a.v_inv = fp8_scales().v_inv + at;
+    }
+    a.err = d_err_;
+    return check("rope_and_cache", launch_rope_cache(a, src, dtype_, sms_, st));
+}
+
+// What the two prefill attentions ask of their rows and lengths alike.
+Status B200Backend::check_prefill(const char *what, const void *q, int64_t num_q_heads, int64_t kv_heads,
+                                  int64_t *q_stride, const int32_t *cu, int64_t num_seqs,
+                                  int64_t num_tokens, int64_t max_new, int64_t max_len,
+                                  float softmax_scale, const void *out) const {
+    const int64_t hd = (int64_t)cfg_.head_dim;
+    if (hd != 64 && hd != 128 && hd != 256)
+        return error(PKV_ERR_DEVICE, 0, 0, std::string(what) + " supports head_dim 64, 128 or 256");
+    if (num_q_heads <= 0 || num_q_heads % kv_heads != 0)
+        return error(PKV_ERR_SHAPE_MISMATCH, kv_heads, num_q_heads,
+                     "query heads must be a positive multiple of the kv heads held here");
+    if (num_q_heads / kv_heads > 128)
+        return error(PKV_ERR_DEVICE, 0, 0, std::string(what) + " supports at most 128 query heads per kv head");
+    if (num_seqs < 0 || num_tokens < 0 || max_new < 0 || max_len < 0)
+        return error(PKV_ERR_SHAPE_MISMATCH, 0, std::min({num_seqs, num_tokens, max_new, max_len}), "negative size");
+    if (num_seqs > 65535) return error(PKV_ERR_DEVICE, 0, 0, "at most 65535 sequences per call");
+    const int64_t most = std::numeric_limits<int32_t>::max() - 1024;
+    if (num_tokens > most || max_len > most)
+        return error(PKV_ERR_SHAPE_MISMATCH, most, std::max(num_tokens, max_len), "lengths beyond 32 bits");
+    if (*q_stride <= 0) *q_stride = num_q_heads * hd;
+    if (*q_stride < num_q_heads * hd || *q_stride % 8 != 0)
+        return error(PKV_ERR_SHAPE_MISMATCH, num_q_heads * hd, *q_stride,
+                     "query row pitch must cover the heads and be a multiple of 8 elements");
+    if (!std::isfinite(softmax_scale) || !(softmax_scale > 0.0f))
+        return error(PKV_ERR_DEVICE, 0, 0, "softmax scale must be finite and positive");
+    if (num_seqs == 0 || num_tokens == 0) return Status::Ok();
+    if (!q || !out || !cu) return error(PKV_ERR_DEVICE, 0, 0, "null device pointer");
+    if (reinterpret_cast<uintptr_t>(q) % 16 || reinterpret_cast<uintptr_t>(out) % 16)
+        return error(PKV_ERR_DEVICE, 0, 0, "query and output must be 16-byte aligned");
+    return Status::Ok();
+}
+
+Status B200Backend::attention_reserve() { return Status::Ok(); }
+
+Status B200Backend::attention_chunk_dev(int64_t layer, const void *q, DType query, int64_t q_stride,
+                                        int64_t num_q_heads, const int32_t *cu, int64_t num_seqs,
+                                        int64_t num_tokens, int64_t max_new, const int32_t *tables,
+                                        int64_t table_stride, const int32_t *ctx, int64_t max_len,
+                                        float softmax_scale, void *out, float *lse, cudaStream_t st) {
+    if (layer < 0 || (uint64_t)layer >= cfg_.num_layers)
+        return error(PKV_ERR_INVALID_LAYER, layer, (int64_t)cfg_.num_layers,
+                     msg_layer((uint64_t)layer, cfg_.num_layers));
+    if (dtype_ == DType::FP8_E4M3) {
+        if (query != DType::BF16 && query != DType::F16)
+            return error(PKV_ERR_DEVICE, 0, 0, "attention over an fp8 pool takes bf16 or f16 queries");
+    } else if (dtype_ != DType::BF16 && dtype_ != DType::F16) {
+        return error(PKV_ERR_DEVICE, 0, 0, "paged attention reads bf16, f16 or fp8 (E4M3) pools");
+    } else if (query != dtype_) {
+        return error(PKV_ERR_DEVICE, 0, 0, "queries must have the pool dtype (bf16 or f16)");
+    }
+    if (cfg_.block_size % 16 != 0)
+        return error(PKV_ERR_DEVICE, 0, 0, "chunk attention needs a block_size that is a multiple of 16");
+    int64_t kv = 0;
+    Status s = whole_heads("chunk attention", &kv);
+    if (!s.ok()) return s;
+    s = check_prefill("chunk attention", q, num_q_heads, kv, &q_stride, cu, num_seqs, num_tokens,
+                      max_new, max_len, softmax_scale, out);
+    if (!s.ok()) return s;
+    if (table_stride < 0 || max_len > table_stride * (int64_t)cfg_.block_size)
+        return error(PKV_ERR_SHAPE_MISMATCH, table_stride * (int64_t)cfg_.block_size, max_len,
+                     "max_context_len exceeds the block tables");
+    const long long rows = (long long)(cfg_.num_layers * cfg_.num_blocks * cfg_.block_size);
+    if (rows >= (1ll << 31)) return error(PKV_ERR_DEVICE, 0, 0, "pool too tall for paged attention");
+    if (num_seqs == 0 || num_tokens == 0) return Status::Ok();
+    if (!tables || !ctx) return error(PKV_ERR_DEVICE, 0, 0, "null device pointer");
+    DeviceGuard g(device_);
+    PrefillLaunch a{};
+    a.q = q;
+    a.q_stride = q_stride;
+    a.out = out;
+    a.lse = lse;
+    a.cu = cu;
+    a.ctx = ctx;
+    a.num_seqs = (int)num_seqs;
+    a.num_tokens = (int)num_tokens;
+    a.max_new = (int)std::min(max_new, num_tokens);
+    a.max_len = (int)max_len;
+    a.kv_heads = (int)kv;
+    a.group = (int)(num_q_heads / kv);
+    a.head_dim = (int)cfg_.head_dim;
+    a.scale_log2 = softmax_scale * 1.4426950408889634f;
+    a.k = k_plane_;
+    a.v = v_plane_;
+    a.tables = tables;
+    a.table_stride = table_stride;
+    a.num_blocks = (int)cfg_.num_blocks;
+    a.block_size = (int)cfg_.block_size;
+    a.layer_row0 = layer * (long long)slots_per_layer();
+    if (dtype_ == DType::FP8_E4M3) {
+        const long long stride = std::max<long long>((long long)(cfg_.num_layers * cfg_.num_kv_heads), 1);
+        const long long at = layer * (long long)cfg_.num_kv_heads + (long long)(elem_offset() / cfg_.head_dim);
+        a.k_scale = d_inv_ + 2 * stride + at;
+        a.v_scale = d_inv_ + 3 * stride + at;
+    }
+    a.err = d_err_;
+    return check("paged_attention_chunk", launch_prefill_attention(a, query, dtype_, sms_, st));
+}
+
+Status B200Backend::prompt_attention_dev(const void *q, const void *k, const void *v, DType dtype,
+                                         int64_t q_stride, int64_t kv_stride, int64_t num_q_heads,
+                                         const int32_t *cu, int64_t num_seqs, int64_t num_tokens,
+                                         int64_t max_len, float softmax_scale, void *out, float *lse,
+                                         cudaStream_t st) {
+    if (dtype != DType::BF16 && dtype != DType::F16)
+        return error(PKV_ERR_DEVICE, 0, 0, "prompt attention takes bf16 or f16 rows");
+    int64_t kv = 0;
+    Status s = whole_heads("prompt attention", &kv);
+    if (!s.ok()) return s;
+    s = check_prefill("prompt attention", q, num_q_heads, kv, &q_stride, cu, num_seqs, num_tokens,
+                      max_len, max_len, softmax_scale, out);
+    if (!s.ok()) return s;
+    const int64_t entry = (int64_t)shard_entry_;
+    if (kv_stride <= 0) kv_stride = entry;
+    if (kv_stride < entry || kv_stride % 8 != 0)
+        return error(PKV_ERR_SHAPE_MISMATCH, entry, kv_stride,
+                     "key and value row pitch must cover the heads and be a multiple of 8 elements");
+    if (num_seqs == 0 || num_tokens == 0) return Status::Ok();
+    if (!k || !v) return error(PKV_ERR_DEVICE, 0, 0, "null device pointer");
+    if (reinterpret_cast<uintptr_t>(k) % 16 || reinterpret_cast<uintptr_t>(v) % 16)
+        return error(PKV_ERR_DEVICE, 0, 0, "keys and values must be 16-byte aligned");
+    DeviceGuard g(device_);
+    PrefillLaunch a{};
+    a.q = q;
+    a.q_stride = q_stride;
+    a.out = out;
+    a.lse = lse;
+    a.cu = cu;
+    a.num_seqs = (int)num_seqs;
+    a.num_tokens = (int)num_tokens;
+    a.max_new = (int)std::min(max_len, num_tokens);
+    a.max_len = (int)max_len;
+    a.kv_heads = (int)kv;
+    a.group = (int)(num_q_heads / kv);
+    a.head_dim = (int)cfg_.head_dim;
+    a.scale_log2 = softmax_scale * 1.4426950408889634f;
+    a.k = k;
+    a.v = v;
+    a.kv_stride = kv_stride;
+    a.err = d_err_;
+    return check("prompt_attention", launch_prefill_attention(a, dtype, dtype, sms_, st));
+}
+
 Status B200Backend::digest(uint64_t *k, uint64_t *v, cudaStream_t st) {
     DeviceGuard g(device_);
     cudaStream_t s = st;

@@ -113,6 +113,28 @@ class B200Backend {
                                  const void *v, int64_t tok_stride, int64_t layer_stride,
                                  DType src, cudaStream_t s, const int64_t *direct_slots = nullptr,
                                  int64_t num_direct = 0);
+    // One layer's new tokens: queries and keys rotated by position, keys and
+    // values appended to the pool.
+    Status rope_and_cache_dev(const int32_t *tables, int64_t table_stride, const int32_t *ctx,
+                              const int32_t *new_lens, int64_t num_seqs, int64_t num_tokens,
+                              int32_t *cu, int64_t *slots_out, int64_t layer, const void *q,
+                              int64_t q_stride, int64_t num_q_heads, void *q_out,
+                              int64_t q_out_stride, const void *k, const void *v,
+                              int64_t kv_stride, void *k_out, int64_t k_out_stride, DType src,
+                              const float *cos_sin, int64_t max_position, int64_t rotary_dim,
+                              int interleaved, cudaStream_t s);
+    // Causal attention of ragged new tokens over the pool and over packed rows.
+    Status attention_chunk_dev(int64_t layer, const void *q, DType query, int64_t q_stride,
+                               int64_t num_q_heads, const int32_t *cu, int64_t num_seqs,
+                               int64_t num_tokens, int64_t max_new, const int32_t *tables,
+                               int64_t table_stride, const int32_t *ctx, int64_t max_len,
+                               float softmax_scale, void *out, float *lse, cudaStream_t s);
+    Status prompt_attention_dev(const void *q, const void *k, const void *v, DType dtype,
+                                int64_t q_stride, int64_t kv_stride, int64_t num_q_heads,
+                                const int32_t *cu, int64_t num_seqs, int64_t num_tokens,
+                                int64_t max_len, float softmax_scale, void *out, float *lse,
+                                cudaStream_t s);
+    Status attention_reserve();
     Status digest(uint64_t *k, uint64_t *v, cudaStream_t s);
     Status digest_rows(int64_t layer, const void *k, const void *v, int64_t tok_stride,
                        int64_t layer_stride, const int64_t *slots, int64_t num_tokens, DType src,
@@ -157,6 +179,11 @@ class B200Backend {
     Fp8Scales fp8_scales() const;
     Status fp8_source_error() const;
     Status upload_inv_scales();
+    Status whole_heads(const char *what, int64_t *kv_heads) const;
+    Status check_prefill(const char *what, const void *q, int64_t num_q_heads, int64_t kv_heads,
+                         int64_t *q_stride, const int32_t *cu, int64_t num_seqs,
+                         int64_t num_tokens, int64_t max_new, int64_t max_len,
+                         float softmax_scale, const void *out) const;
     Status check(const char *what, cudaError_t e) const;
 
     pkv_config cfg_{};

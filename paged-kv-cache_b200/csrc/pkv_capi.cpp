@@ -230,6 +230,65 @@ int pkv_paged_attention_plan_dev(pkv_backend *b, const int32_t *context_lens, in
     });
 }
 
+int pkv_rope_and_cache_dev(pkv_backend *b, const int32_t *block_tables, int64_t table_stride,
+                           const int32_t *ctx_lens, const int32_t *new_lens, int64_t num_seqs,
+                           int64_t num_tokens, int32_t *cu_seqlens, int64_t *slot_mapping,
+                           int64_t layer, const void *q, int64_t q_token_stride,
+                           int64_t num_q_heads, void *q_out, int64_t q_out_stride, const void *k,
+                           const void *v, int64_t kv_token_stride, void *k_out,
+                           int64_t k_out_stride, int src_dtype, const float *cos_sin,
+                           int64_t max_position, int64_t rotary_dim, int interleaved,
+                           void *stream) {
+    if (!b) return null_handle();
+    if (!valid_dtype(src_dtype)) return bad_dtype();
+    return guarded("pkv_rope_and_cache_dev", [&] {
+        return b->impl->rope_and_cache_dev(block_tables, table_stride, ctx_lens, new_lens, num_seqs,
+                                           num_tokens, cu_seqlens, slot_mapping, layer, q,
+                                           q_token_stride, num_q_heads, q_out, q_out_stride, k, v,
+                                           kv_token_stride, k_out, k_out_stride,
+                                           static_cast<pkv::DType>(src_dtype), cos_sin, max_position,
+                                           rotary_dim, interleaved, as_stream(stream));
+    });
+}
+
+int pkv_paged_attention_chunk_dev(pkv_backend *b, int64_t layer, const void *q, int query_dtype,
+                                  int64_t q_token_stride, int64_t num_q_heads,
+                                  const int32_t *cu_seqlens, int64_t num_seqs, int64_t num_tokens,
+                                  int64_t max_new_len, const int32_t *block_tables,
+                                  int64_t table_stride, const int32_t *ctx_lens,
+                                  int64_t max_context_len, float softmax_scale, void *out,
+                                  float *lse, void *stream) {
+    if (!b) return null_handle();
+    if (!valid_dtype(query_dtype)) return bad_dtype();
+    return guarded("pkv_paged_attention_chunk_dev", [&] {
+        return b->impl->attention_chunk_dev(layer, q, static_cast<pkv::DType>(query_dtype),
+                                            q_token_stride, num_q_heads, cu_seqlens, num_seqs,
+                                            num_tokens, max_new_len, block_tables, table_stride,
+                                            ctx_lens, max_context_len, softmax_scale, out, lse,
+                                            as_stream(stream));
+    });
+}
+
+int pkv_prompt_attention_dev(pkv_backend *b, const void *q, const void *k, const void *v, int dtype,
+                             int64_t q_token_stride, int64_t kv_token_stride, int64_t num_q_heads,
+                             const int32_t *cu_seqlens, int64_t num_seqs, int64_t num_tokens,
+                             int64_t max_len, float softmax_scale, void *out, float *lse,
+                             void *stream) {
+    if (!b) return null_handle();
+    if (!valid_dtype(dtype)) return bad_dtype();
+    return guarded("pkv_prompt_attention_dev", [&] {
+        return b->impl->prompt_attention_dev(q, k, v, static_cast<pkv::DType>(dtype), q_token_stride,
+                                             kv_token_stride, num_q_heads, cu_seqlens, num_seqs,
+                                             num_tokens, max_len, softmax_scale, out, lse,
+                                             as_stream(stream));
+    });
+}
+
+int pkv_attention_reserve(pkv_backend *b) {
+    if (!b) return null_handle();
+    return guarded("pkv_attention_reserve", [&] { return b->impl->attention_reserve(); });
+}
+
 int pkv_set_copy_engine(pkv_backend *b, int engine) {
     if (!b) return null_handle();
     return guarded("pkv_set_copy_engine", [&] { return b->impl->set_copy_engine(engine); });

@@ -221,6 +221,79 @@ struct AttnLaunch {
     DevError *err;
 };
 
+// rope_and_cache of one layer (pkv_rope.cu): the new tokens' queries and keys
+// rotated, keys and values appended to the pool. Strides are in elements of
+// the source type; heads are those held by this backend.
+struct RopeCacheLaunch {
+    const int *tables;
+    long long table_stride;
+    const int *ctx_lens;
+    const int *new_lens;
+    long long num_seqs;
+    long long num_tokens;   // packed rows; sum(new_lens) of them hold tokens
+    long long block_size;
+    long long num_blocks;
+    int *cu_seqlens;        // [num_seqs + 1], written
+    long long *slots_out;   // [num_tokens] or null
+    const void *q;          // [num_tokens][num_q_heads][head_dim]
+    long long q_stride;
+    void *q_out;            // may be q
+    long long q_out_stride;
+    const void *k;          // [num_tokens][kv_heads][head_dim], v alike
+    const void *v;
+    long long kv_stride;
+    void *k_out;            // rotated keys as rows, or null; may be k
+    long long k_out_stride;
+    void *k_layer;          // this layer of the pool planes
+    void *v_layer;
+    int num_q_heads;
+    int kv_heads;
+    int head_dim;
+    int rotary_dim;
+    int interleaved;
+    const float *cos_sin;   // [max_position][rotary_dim]: cosines, then sines
+    long long max_position;
+    const float *k_inv;     // fp8 pools: [kv_heads] inverse scales of this layer
+    const float *v_inv;
+    DevError *err;
+    // Set by the launcher: a token's heads are split over `head_splits`
+    // warps of up to `heads_per_split` heads.
+    int head_splits = 1;
+    int heads_per_split = 0;
+};
+
+// Causal attention of ragged new tokens over one layer (pkv_prefill.cu).
+// Sequence s has the packed rows cu[s] .. cu[s + 1]; its row i sits at
+// position ctx[s] + i and attends keys 0 .. that position.
+struct PrefillLaunch {
+    const void *q;           // [num_tokens][num_q_heads][head_dim], row pitch q_stride elements
+    long long q_stride;
+    void *out;               // [num_tokens][num_q_heads][head_dim], dense
+    float *lse;              // [num_tokens][num_q_heads] natural log, or null
+    const int *cu;           // [num_seqs + 1]
+    const int *ctx;          // [num_seqs] cached tokens before the rows; null: none (prompt rows)
+    int num_seqs;
+    int num_tokens;          // packed rows of q and out
+    int max_new;             // bounds every sequence's rows
+    int max_len;             // bounds every ctx[s] + rows
+    int kv_heads;
+    int group;               // query heads per kv head
+    int head_dim;
+    float scale_log2;        // softmax scale * log2(e)
+    // Keys and values in the pool (paged), or in packed rows beside q.
+    const void *k;           // the pool's K plane, or [num_tokens][kv_heads][head_dim]
+    const void *v;
+    long long kv_stride;     // packed rows: row pitch in elements
+    const int *tables = nullptr;
+    long long table_stride = 0;
+    int num_blocks = 0;
+    int block_size = 0;
+    long long layer_row0 = 0;  // first pool row of the layer
+    const float *k_scale = nullptr;  // fp8 pools: [kv_heads] scales of this layer
+    const float *v_scale = nullptr;
+    DevError *err;
+};
+
 int num_sms(int device);
 
 cudaError_t launch_reshape(const ReshapeLaunch &a, int sms, cudaStream_t s);
@@ -254,6 +327,14 @@ cudaError_t launch_attention_plan(const int *ctx, int num_seqs, int max_ctx, uns
 // bf16/f16 pools; bf16 or f16 over an fp8 pool).
 cudaError_t launch_paged_attention(const AttnLaunch &a, const void *tmaps, DType pool, DType query,
                                    int head_dim, cudaStream_t s);
+
+// src: type of q, k, v and their outputs; it equals the pool type, or the
+// pool is fp8.
+cudaError_t launch_rope_cache(const RopeCacheLaunch &a, DType src, DType pool, int sms, cudaStream_t s);
+
+// query: type of q and out (bf16 or f16); kv: type of the keys and values,
+// the query type or fp8 (paged only).
+cudaError_t launch_prefill_attention(const PrefillLaunch &a, DType query, DType kv, int sms, cudaStream_t s);
 
 // fp8 (E4M3) pools (pkv_fp8.cu): quantising scatter, fused slot resolution +
 // quantising scatter, and the digests of E4M3 planes and rows.

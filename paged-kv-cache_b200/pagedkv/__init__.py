@@ -11,11 +11,12 @@ the built library raises ImportError (there is no fallback).
 from .config import CacheConfig, PhysicalSlot
 from .errors import (BlockNotAllocated, CacheError, Device, InvalidBlock, InvalidLayer,
                      OutOfBlocks, RefCountOverflow, ShapeMismatch, SlotOutOfRange, UnknownSequence)
+from .rope import rope_table
 
 __all__ = [
     "B200Backend", "CacheConfig", "PhysicalSlot", "CacheError", "OutOfBlocks", "InvalidBlock",
     "BlockNotAllocated", "RefCountOverflow", "SlotOutOfRange", "ShapeMismatch", "InvalidLayer",
-    "UnknownSequence", "Device",
+    "UnknownSequence", "Device", "rope_table",
 ]
 
 

@@ -343,6 +343,83 @@ class B200Backend:
                                                      max_context_len, float(softmax_scale), _ptr(out),
                                                      _ptr(lse), _stream_ptr(stream)))
 
+    def rope_and_cache(self, block_tables, ctx_lens, new_lens, num_tokens: int, cu_out, q, k, v,
+                       cos_sin, layer: int, q_out=None, k_out=None, interleaved: bool = False,
+                       slots_out=None, stream=None) -> None:
+        """One layer's new tokens: q and k rotated by position, k and v
+        appended to the pool (pkv_rope_and_cache_dev). q [T][num_q_heads]
+        [head_dim] or None, k and v [T][kv heads][head_dim] with rows of any
+        pitch; cos_sin f32 [positions][rotary_dim] (see pagedkv.rope_table);
+        q_out None rotates q in place, k_out (rows like k) is optional."""
+        s = ctx_lens.shape[0]
+        stride = block_tables.shape[1] if block_tables.dim() == 2 else 0
+        tag = _torch_tag(k)
+        _same_layout(k, v)
+        rows = [x for x in (q, q_out, k, k_out) if x is not None]
+        for x in rows:
+            _head_rows(x)
+            if x.dtype != k.dtype:
+                raise ValueError("q, k, v and their outputs must share a dtype")
+            if x.shape[0] < num_tokens:
+                raise ValueError("num_tokens exceeds the rows")
+        if k.shape[1] * k.shape[2] != self.shard_entry_elems or k.shape[2] != self._cfg.head_dim:
+            raise ValueError("k and v must hold the kv heads of this backend")
+        if q_out is not None and (q is None or q_out.shape != q.shape):
+            raise ValueError("q_out must have the shape of q")
+        if k_out is not None and k_out.shape != k.shape:
+            raise ValueError("k_out must have the shape of k")
+        if q is not None and q.shape[2] != k.shape[2]:
+            raise ValueError("q and k must share head_dim")
+        if cos_sin.dim() != 2 or not cos_sin.is_contiguous() or cos_sin.dtype.itemsize != 4 or not cos_sin.is_floating_point():
+            raise ValueError("cos_sin must be a dense f32 [positions][rotary_dim] tensor")
+        _check(lib.pkv_rope_and_cache_dev(
+            self._h, _ptr(block_tables), stride, _ptr(ctx_lens), _ptr(new_lens), s, num_tokens,
+            _ptr(cu_out), _ptr(slots_out), layer, _ptr(q), 0 if q is None else q.stride(0),
+            0 if q is None else q.shape[1], _ptr(q_out), 0 if q_out is None else q_out.stride(0),
+            _ptr(k), _ptr(v), k.stride(0), _ptr(k_out), 0 if k_out is None else k_out.stride(0),
+            tag, _ptr(cos_sin), cos_sin.shape[0], cos_sin.shape[1], int(interleaved),
+            _stream_ptr(stream)))
+
+    def paged_attention_chunk(self, q, cu_seqlens, block_tables, ctx_lens, max_new_len: int,
+                              max_context_len: int, out, layer: int,
+                              softmax_scale: float | None = None, lse=None, stream=None) -> None:
+        """Causal attention of ragged new tokens over one layer of the cache
+        (pkv_paged_attention_chunk_dev): q and out [T][num_q_heads][head_dim],
+        sequence s at rows cu_seqlens[s] .. cu_seqlens[s + 1], ctx_lens the
+        tokens cached before them, lse optional f32 [T][num_q_heads]."""
+        t, hq, d = _head_rows(q)
+        _dense_out(q, out)
+        if softmax_scale is None:
+            softmax_scale = d ** -0.5
+        stride = block_tables.shape[1] if block_tables.dim() == 2 else 0
+        _check(lib.pkv_paged_attention_chunk_dev(
+            self._h, layer, _ptr(q), _torch_tag(q), q.stride(0), hq, _ptr(cu_seqlens),
+            ctx_lens.shape[0], t, max_new_len, _ptr(block_tables), stride, _ptr(ctx_lens),
+            max_context_len, float(softmax_scale), _ptr(out), _ptr(lse), _stream_ptr(stream)))
+
+    def prompt_attention(self, q, k, v, cu_seqlens, max_len: int, out,
+                         softmax_scale: float | None = None, lse=None, stream=None) -> None:
+        """Causal attention over whole packed prompts from their rows
+        (pkv_prompt_attention_dev): q and out [T][num_q_heads][head_dim], k and
+        v [T][kv heads][head_dim], sequence s at rows cu_seqlens[s] ..
+        cu_seqlens[s + 1], lse optional f32 [T][num_q_heads]."""
+        t, hq, d = _head_rows(q)
+        _dense_out(q, out)
+        _same_layout(k, v)
+        if _head_rows(k) != (t, self.shard_entry_elems // self._cfg.head_dim, d) or k.dtype != q.dtype:
+            raise ValueError("k and v must hold q's rows, the kv heads of this backend, q's dtype")
+        if softmax_scale is None:
+            softmax_scale = d ** -0.5
+        _check(lib.pkv_prompt_attention_dev(
+            self._h, _ptr(q), _ptr(k), _ptr(v), _torch_tag(q), q.stride(0), k.stride(0), hq,
+            _ptr(cu_seqlens), cu_seqlens.shape[0] - 1, t, max_len, float(softmax_scale), _ptr(out),
+            _ptr(lse), _stream_ptr(stream)))
+
+    def attention_reserve(self) -> None:
+        """Allocates the workspace of paged_attention_chunk and prompt_attention
+        ahead, so that their first call can be captured (pkv_attention_reserve)."""
+        _check(lib.pkv_attention_reserve(self._h))
+
     def digest(self, stream=None) -> tuple[int, int]:
         k, v = C.c_uint64(), C.c_uint64()
         _check(lib.pkv_digest(self._h, C.byref(k), C.byref(v), _stream_ptr(stream)))
@@ -413,3 +490,16 @@ def _same_layout(k, v) -> None:
         raise ValueError("k and v must share shape, strides and dtype")
     if k.stride(-1) != 1:
         raise ValueError("entries must be contiguous")
+
+
+def _head_rows(x) -> tuple[int, int, int]:
+    """(rows, heads, head_dim) of a [rows][heads][head_dim] tensor whose rows
+    are dense and may lie at any pitch."""
+    if x.dim() != 3 or x.stride(2) != 1 or (x.shape[1] > 1 and x.stride(1) != x.shape[2]):
+        raise ValueError("rows must be contiguous [heads][head_dim]")
+    return tuple(x.shape)
+
+
+def _dense_out(q, out) -> None:
+    if out.shape != q.shape or out.dtype != q.dtype or not out.is_contiguous():
+        raise ValueError("out must be dense, with the shape and dtype of q")
