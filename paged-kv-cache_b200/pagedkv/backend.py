@@ -75,9 +75,12 @@ def _stream_ptr(stream) -> int | None:
 
 
 class _DeviceArray:
-    """Minimal __cuda_array_interface__ so torch can view the pool planes."""
+    """Minimal __cuda_array_interface__ so torch can view the pool planes. A
+    tensor made of it keeps it, and with it `owner`: the pool lives as long as
+    its views (unless it is closed by hand)."""
 
-    def __init__(self, ptr: int, shape: tuple, typestr: str):
+    def __init__(self, ptr: int, shape: tuple, typestr: str, owner=None):
+        self.owner = owner
         self.__cuda_array_interface__ = {
             "shape": shape, "typestr": typestr, "data": (ptr, False), "version": 3, "strides": None}
 
@@ -461,7 +464,7 @@ class B200Backend:
         typestr = {F32: "<f4", BF16: "<i2", F16: "<f2", FP8_E4M3: "|u1"}[self._dtype]
         out = []
         for p in (k.value, v.value):
-            t = torch.as_tensor(_DeviceArray(p or 0, shape, typestr), device=f"cuda:{self.device}")
+            t = torch.as_tensor(_DeviceArray(p or 0, shape, typestr, self), device=f"cuda:{self.device}")
             if self._dtype == BF16:
                 t = t.view(torch.bfloat16)
             elif self._dtype == FP8_E4M3:
