@@ -242,6 +242,7 @@ B200Backend::~B200Backend() {
     if (d_err_) cudaFree(d_err_);
     if (d_inv_) cudaFree(d_inv_);
     if (d_attn_ws_) cudaFree(d_attn_ws_);
+    if (d_prefill_ws_) cudaFree(d_prefill_ws_);
     if (d_plan_) cudaFree(d_plan_);
     if (d_stage_) cudaFree(d_stage_);
     if (h_stage_) cudaFreeHost(h_stage_);
@@ -1263,7 +1264,19 @@ Status B200Backend::check_prefill(const char *what, const void *q, int64_t num_q
     return Status::Ok();
 }
 
-Status B200Backend::attention_reserve() { return Status::Ok(); }
+Status B200Backend::attention_reserve() {
+    const uint64_t hd = cfg_.head_dim;
+    if (hd != 64 && hd != 128 && hd != 256)
+        return error(PKV_ERR_DEVICE, 0, 0, "prefill attention supports head_dim 64, 128 or 256");
+    if (d_prefill_ws_) return Status::Ok();
+    DeviceGuard g(device_);
+    const cudaError_t e = cudaMalloc(&d_prefill_ws_, prefill_workspace_bytes((int)hd, sms_));
+    if (e != cudaSuccess) {
+        d_prefill_ws_ = nullptr;
+        return device_error("allocating the prefill workspace", e);
+    }
+    return Status::Ok();
+}
 
 Status B200Backend::attention_chunk_dev(int64_t layer, const void *q, DType query, int64_t q_stride,
                                         int64_t num_q_heads, const int32_t *cu, int64_t num_seqs,
@@ -1319,6 +1332,7 @@ Status B200Backend::attention_chunk_dev(int64_t layer, const void *q, DType quer
     a.num_blocks = (int)cfg_.num_blocks;
     a.block_size = (int)cfg_.block_size;
     a.layer_row0 = layer * (long long)slots_per_layer();
+    a.pool_rows = rows;
     if (dtype_ == DType::FP8_E4M3) {
         const long long stride = std::max<long long>((long long)(cfg_.num_layers * cfg_.num_kv_heads), 1);
         const long long at = layer * (long long)cfg_.num_kv_heads + (long long)(elem_offset() / cfg_.head_dim);
@@ -1326,7 +1340,10 @@ Status B200Backend::attention_chunk_dev(int64_t layer, const void *q, DType quer
         a.v_scale = d_inv_ + 3 * stride + at;
     }
     a.err = d_err_;
-    return check("paged_attention_chunk", launch_prefill_attention(a, query, dtype_, sms_, st));
+    s = attention_reserve();
+    if (!s.ok()) return s;
+    return check("paged_attention_chunk",
+                 launch_prefill_attention(a, query, dtype_, {d_prefill_ws_, sms_}, sms_, st));
 }
 
 Status B200Backend::prompt_attention_dev(const void *q, const void *k, const void *v, DType dtype,
@@ -1370,7 +1387,10 @@ Status B200Backend::prompt_attention_dev(const void *q, const void *k, const voi
     a.v = v;
     a.kv_stride = kv_stride;
     a.err = d_err_;
-    return check("prompt_attention", launch_prefill_attention(a, dtype, dtype, sms_, st));
+    s = attention_reserve();
+    if (!s.ok()) return s;
+    return check("prompt_attention",
+                 launch_prefill_attention(a, dtype, dtype, {d_prefill_ws_, sms_}, sms_, st));
 }
 
 Status B200Backend::digest(uint64_t *k, uint64_t *v, cudaStream_t st) {

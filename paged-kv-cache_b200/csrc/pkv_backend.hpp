@@ -233,6 +233,7 @@ class B200Backend {
     bool tmaps_ready_ = false;
     float *d_attn_ws_ = nullptr;
     size_t d_attn_ws_bytes_ = 0;
+    void *d_prefill_ws_ = nullptr;  // of the prefill attentions: one size, made on first use
     // The attention plan (sequence order, 65,535 entries) and the call shape
     // it was made for.
     unsigned *d_plan_ = nullptr;

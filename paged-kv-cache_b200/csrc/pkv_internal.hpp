@@ -289,6 +289,7 @@ struct PrefillLaunch {
     int num_blocks = 0;
     int block_size = 0;
     long long layer_row0 = 0;  // first pool row of the layer
+    long long pool_rows = 0;   // rows of a pool plane, all layers
     const float *k_scale = nullptr;  // fp8 pools: [kv_heads] scales of this layer
     const float *v_scale = nullptr;
     DevError *err;
@@ -334,7 +335,15 @@ cudaError_t launch_rope_cache(const RopeCacheLaunch &a, DType src, DType pool, i
 
 // query: type of q and out (bf16 or f16); kv: type of the keys and values,
 // the query type or fp8 (paged only).
-cudaError_t launch_prefill_attention(const PrefillLaunch &a, DType query, DType kv, int sms, cudaStream_t s);
+// Partials of split items: two slots per CTA, so a size that no call's lengths
+// change.
+struct PrefillWorkspace {
+    void *base;
+    int ctas;
+};
+size_t prefill_workspace_bytes(int head_dim, int ctas);
+cudaError_t launch_prefill_attention(const PrefillLaunch &a, DType query, DType kv, const PrefillWorkspace &ws, int sms,
+                                     cudaStream_t s);
 
 // fp8 (E4M3) pools (pkv_fp8.cu): quantising scatter, fused slot resolution +
 // quantising scatter, and the digests of E4M3 planes and rows.

@@ -6,142 +6,1232 @@
 // p = ctx[s] + i:
 //   out = sum_{j <= p} softmax_j(scale * q . k_j) v_j
 //
-// One warp per (row, query head): 32 keys at a time, a lane to a key for the
-// scores, a lane to a run of head_dim / 32 elements for the output; the
-// running maximum and sum of the softmax in f32.
+// Mapping. An item is up to 2 x 128 query rows of one sequence and kv head
+// (a row is a token and a head of the group, so the group shares every K and V
+// tile) and walks the key tiles from 0 to its causal end. Both products run on
+// the tensor core with f32 accumulators in tensor memory: S = Q K^T from
+// shared memory, O += P V with the weights P (rounded to the query type)
+// written back over S in tensor memory. The work is the 4 D operations a
+// (query, key) pair that the products cost, and one exponential.
+// - Row items: two 128-row tiles share each K/V tile; while a warpgroup takes
+//   the softmax of one, the tensor core works on the other.
+// - Key items (at most 128 rows): both warpgroups hold the same rows and take
+//   every other key tile, each with its own O and statistics, merged at the
+//   end: few rows are bound by the K/V stream, and this halves the chain of
+//   softmaxes that the stream waits for.
+// - head_dim 256: O alone takes half of tensor memory, so one row tile, two S
+//   buffers, one warpgroup: a tile's products take twice its softmax.
+// Schedule. One CTA per SM. The items' costs (keys, plus a constant) are
+// summed in order of sequence, head and row; CTA b takes the b-th equal share,
+// so lengths need no sorting and few rows over a long context are split along
+// the keys. A share that begins or ends inside an item leaves a partial
+// (O, max, sum) in a workspace of fixed size, two slots a CTA, and a second
+// kernel joins an item's partials in order. Everything is derived from the
+// lengths on the device; nothing depends on which CTA finishes first.
+// Roles (16 warps): 8 warps softmax and epilogue, one issues the products, one
+// brings K and V by TMA, one plans items and brings Q, four fill the V tiles
+// that a mask crosses (and, over an fp8 pool, convert every tile).
+//
+// Masked keys may hold anything. A masked score is replaced before it is used.
+// A masked value still meets a weight of 0 in the product, and 0 * NaN is NaN,
+// so V tiles that some row masks are not brought by TMA: rows past the
+// sequence and blocks outside the pool become zeros, and elements that are not
+// finite become zero and are noted; at the end they are added to the rows
+// that do attend them (a weight times an infinity or NaN is that infinity or
+// NaN whatever the weight).
 
+#include <cuda.h>
+#include <cudaTypedefs.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 
 #include <algorithm>
+#include <cfloat>
 #include <cstdint>
 #include <type_traits>
 
 #include "pkv_device.cuh"
 #include "pkv_internal.hpp"
+#include "pkv_tcgen05.cuh"
 
 namespace pkv {
 namespace {
 
-__device__ __forceinline__ float wide(__nv_bfloat16 x) { return __bfloat162float(x); }
-__device__ __forceinline__ float wide(__half x) { return __half2float(x); }
-__device__ __forceinline__ float wide(uint8_t code) {
-    unsigned y;
-    asm("{\n\t.reg .b16 a;\n\tcvt.u16.u32 a, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, a;\n\t}" : "=r"(y) : "r"((unsigned)code));
-    return __half2float(__ushort_as_half((unsigned short)(y & 0xffffu)));
-}
-template <typename T>
-__device__ __forceinline__ T tight(float x);
-template <>
-__device__ __forceinline__ __nv_bfloat16 tight<__nv_bfloat16>(float x) { return __float2bfloat16_rn(x); }
-template <>
-__device__ __forceinline__ __half tight<__half>(float x) { return __float2half_rn(x); }
+using namespace tc;
 
-// A sequence's rows and keys as the kernel uses them. Lengths that the call
-// does not allow are recorded; the rows of one whose lengths alone are wrong
-// are written as empty, rows outside the packed ones are not touched.
+constexpr int kDeviceCode = 9;                            // PKV_ERR_DEVICE
+constexpr long long kWaitCycles = 4000000000ll;           // about 2 s
+constexpr int kPrefillThreads = 512;
+constexpr int kItemRing = 4;
+constexpr int kMaskRing = 32;
+constexpr int kFlagWords = 12;                            // 3 key tiles of 128 bits
+// Registers a thread after the split of the launch's 128 x 512: softmax
+// threads hold a row of 128 scores, the others a few addresses.
+constexpr int kSoftmaxRegs = 192, kOtherRegs = 64;
+static_assert(2 * (kSoftmaxRegs + kOtherRegs) * 128 <= 128 * kPrefillThreads, "register split");
+// The reference point of a row's weights moves when a score passes it by more
+// than this (base 2): weights stay below 2^8, sums and products keep their
+// relative precision, and most tiles skip the rescale of O.
+constexpr float kLazy = 8.0f;
+
+enum Source { kPaged = 0, kPagedFp8 = 1, kRows = 2 };
+
+// Tile geometry. Operand tiles are slabs of 64 elements: [D / 64][rows][128 B],
+// 128-byte swizzled (16-byte chunk c of row r at c ^ (r % 8)).
+template <int D, Source SRC>
+struct Geom {
+    static constexpr int kRowTiles = D == 256 ? 1 : 2;          // 128-row tiles per item
+    static constexpr int kKeys = D == 256 ? 64 : 128;           // keys per tile
+    static constexpr int kSlabs = D / 64;
+    static constexpr int kQTile = 128 * D * 2;
+    static constexpr int kTile = kKeys * D * 2;                 // one K or V tile
+    static constexpr int kSlab = kKeys * 128;
+    static constexpr bool kFp8 = SRC == kPagedFp8;
+    static constexpr int kStages = kFp8 ? (D == 64 ? 6 : 3) : (D == 64 ? 10 : 5);
+    static constexpr int kRawTile = kKeys * D;                  // fp8: the tile's codes
+    static constexpr int kRawStages = kFp8 ? (D == 64 ? 6 : 3) : 0;
+    static constexpr int kGranules = kKeys / 16;
+    static constexpr int kSCols = kKeys;                        // tensor-memory columns of an S buffer
+    static constexpr int kOCol = 2 * kSCols;
+    static constexpr int kStatBytes = 2 * 128 * 8;
+    static constexpr int kSmem = kRowTiles * kQTile + kStages * kTile + kRawStages * kRawTile + kStatBytes;
+    static constexpr int kSlotRows = kRowTiles * 128;           // rows of a partial
+    static_assert(kOCol + kRowTiles * D <= 512, "tensor memory");
+};
+
+// Costs, in key-tile units of 1/128: a tile costs its keys times the row
+// tiles, an item kItemCost more (queries in, outputs out).
+constexpr int kItemCost = 256;
+// Shares do not begin or end closer than this many key tiles to an item's
+// ends: the join costs about as much.
+constexpr int kSnapRows = 3, kSnapKeys = 4;
+
+struct Header {          // of a partial slot
+    int valid, last;     // last: the piece reaches the item's last key
+    int row0, tokens;    // packed row of the item's first token; its tokens
+    int head, two;       // kv head; two row tiles
+    int pad[2];
+};
+
+struct Params {
+    PrefillLaunch a;
+    int tile_tokens;     // tokens per 128-row tile: 128 / group
+    float *part_o;       // [2 * ctas][slot rows][D]
+    float2 *part_ml;     // [2 * ctas][slot rows]: reference point (base 2), sum
+    Header *headers;     // [2 * ctas]
+};
+
+struct Item {
+    int seq, head;
+    int row0;            // packed row of the first token
+    int tokens;
+    int key0;            // keys before the first token's own: row i's limit is key0 + i + 1
+    int base;            // packed row of key 0 (packed rows only)
+    int t0, t1, tiles;   // this piece's key tiles; the item's
+    int two;             // row item
+    int slot;            // partial slot, or -1: the whole item
+    int end;             // no more items
+};
+
+// A sequence as every role sees it: rows < 0 are not touched; empty ones are
+// written as rows without keys.
 struct Seq {
-    int row0, rows, ctx;  // rows < 0: none
+    int row0, rows, ctx;
     bool empty;
 };
 __device__ __forceinline__ Seq sequence(const PrefillLaunch &a, int s, bool report) {
     const int lo = __ldg(a.cu + s), hi = __ldg(a.cu + s + 1);
     const int ctx = a.ctx ? __ldg(a.ctx + s) : 0;
-    Seq q{lo, hi - lo, ctx, false};
+    Seq q{lo, 0, ctx, false};
     if (lo < 0 || hi < lo || hi > a.num_tokens) {
         if (report) record_error(a.err, kShapeMismatch, s);
-        q.rows = -1;
-    } else if (q.rows > 0 && (ctx < 0 || q.rows > a.max_new || ctx > a.max_len - q.rows)) {
+        return q;
+    }
+    q.rows = hi - lo;
+    if (q.rows > 0 && (ctx < 0 || q.rows > a.max_new || ctx > a.max_len - q.rows)) {
         if (report) record_error(a.err, kShapeMismatch, s);
         q.empty = true;
+        q.ctx = 0;
     }
     return q;
 }
 
-template <typename T, typename KV, int D>
-__global__ void __launch_bounds__(256) prefill_attention_kernel(const PrefillLaunch a) {
+// The cost of the items of a sequence. Items 0 .. items - 2 are full; item i
+// ends at key ctx + min((i + 1) * per, rows).
+template <int ROW_TILES>
+struct Costs {
+    long long ctx, per, rows, items, last;
+    bool empty;
+    __device__ __forceinline__ Costs(const Seq &q, int tile_tokens) {
+        ctx = q.ctx;
+        per = (long long)ROW_TILES * tile_tokens;
+        rows = q.rows;
+        empty = q.empty;
+        items = (rows + per - 1) / per;
+        const bool two = ROW_TILES == 2 && rows - (items - 1) * per > tile_tokens;
+        last = empty ? kItemCost : (two ? 2 : 1) * (ctx + rows) + kItemCost;
+    }
+    // Cost of items 0 .. i - 1, i < items (all full).
+    __device__ __forceinline__ long long before(long long i) const {
+        if (empty) return i * kItemCost;
+        return i * (ROW_TILES * ctx + kItemCost) + ROW_TILES * per * (i * (i + 1) / 2);
+    }
+    __device__ __forceinline__ long long head() const { return items ? before(items - 1) + last : 0; }
+    __device__ __forceinline__ long long of(long long i) const { return i + 1 < items ? before(i + 1) - before(i) : last; }
+};
+
+struct Pos {
+    int s, h, i, t;  // key tile t of item i of kv head h of sequence s
+};
+
+// The place of cost x within sequence s. Rounded to a key tile; within kSnap
+// tiles of an item's ends, to that end.
+template <int ROW_TILES, int KEYS>
+__device__ __forceinline__ Pos locate(const Costs<ROW_TILES> &c, int s, long long x, int tile_tokens) {
+    const long long head = c.head();
+    const int h = (int)(x / head);
+    long long r = x - h * head;
+    long long lo = 0, hi = c.items - 1;
+    while (lo < hi) {
+        const long long mid = (lo + hi + 1) >> 1;
+        if (c.before(mid) <= r) lo = mid;
+        else hi = mid - 1;
+    }
+    r -= c.before(lo);
+    const long long end = c.ctx + min((lo + 1) * c.per, c.rows);
+    const int tiles = c.empty ? 0 : (int)((end + KEYS - 1) / KEYS);
+    const bool two = ROW_TILES == 2 && (lo + 1 < c.items || c.rows - lo * c.per > tile_tokens);
+    const int snap = two ? kSnapRows : kSnapKeys;
+    int t = (int)((double)r / (double)c.of(lo) * tiles + 0.5);
+    if (t < snap && t * 2 <= tiles) t = 0;
+    if (tiles - t < snap) t = tiles;
+    if (tiles < 2 * snap) t = 2 * t < tiles ? 0 : tiles;
+    Pos p{s, h, (int)lo, t};
+    if (t == tiles && (tiles > 0 || r > 0)) {  // the item's end is the next one's beginning
+        p.t = 0;
+        ++p.i;
+    }
+    return p;
+}
+
+template <typename T>
+__device__ __forceinline__ uint32_t nonfinite_mask(uint32_t w) {  // a bit 15 / 31 for an element that is not finite
+    if constexpr (std::is_same_v<T, __half>) return ((w & 0x7C007C00u) + 0x04000400u) & 0x80008000u;
+    else return ((w & 0x7F807F80u) + 0x00800080u) & 0x80008000u;
+}
+__device__ __forceinline__ float wide(__nv_bfloat16 x) { return __bfloat162float(x); }
+__device__ __forceinline__ float wide(__half x) { return __half2float(x); }
+
+// Two E4M3 codes as a pair of T, exactly.
+template <typename T>
+__device__ __forceinline__ uint32_t codes_to(uint32_t two) {
+    uint32_t h;
+    asm("{\n\t.reg .b16 a, b;\n\tmov.b32 {a, b}, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, a;\n\t}" : "=r"(h) : "r"(two));
+    if constexpr (std::is_same_v<T, __half>) return h;
+    const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&h));
+    return pack2<__nv_bfloat16>(f.x, f.y);
+}
+
+template <typename T, int D, Source SRC>
+__global__ void __launch_bounds__(kPrefillThreads, 1)
+prefill_attention_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CUtensorMap tk,
+                         const __grid_constant__ CUtensorMap tv, const __grid_constant__ Params p) {
+    using G = Geom<D, SRC>;
+    constexpr int NT = G::kRowTiles, KEYS = G::kKeys, ST = G::kStages, RS = G::kRawStages ? G::kRawStages : 1;
+    extern __shared__ __align__(1024) unsigned char smem[];
+    __shared__ __align__(8) uint64_t kv_full[ST], kv_empty[ST], raw_full[RS], raw_empty[RS], by_hand_go[ST];
+    __shared__ __align__(8) uint64_t s_full[2], p_full[2], o_full[2], o_free[2], pv_done, pair_bar, q_full, q_empty, drain;
+    __shared__ __align__(8) uint64_t item_full[kItemRing], item_empty[kItemRing];
+    __shared__ Item s_item[kItemRing];
+    __shared__ unsigned s_flag[kItemRing][kFlagWords + 1];
+    __shared__ unsigned char s_mask[kMaskRing];
+    __shared__ long long s_scan[kPrefillThreads / 32];
+    __shared__ Pos s_range[2];
+    __shared__ uint32_t s_tmem;
+    __shared__ volatile int s_failed;
+
+    const PrefillLaunch &a = p.a;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    unsigned char *sq = smem, *skv = smem + NT * G::kQTile, *sraw = skv + ST * G::kTile;
+    float2 *stat = reinterpret_cast<float2 *>(sraw + G::kRawStages * G::kRawTile);
+
+    if (smem_u32(smem) & 1023u) {  // the swizzle's atoms would not line up
+        if (tid == 0) record_error(a.err, kDeviceCode, blockIdx.x);
+        return;
+    }
+    if (warp == 0) tmem_alloc(&s_tmem, 512);
+    if (tid == 32) {
+        for (int i = 0; i < ST; ++i) mbar_init(&kv_full[i], 1), mbar_init(&kv_empty[i], 1), mbar_init(&by_hand_go[i], 1);
+        for (int i = 0; i < RS; ++i) mbar_init(&raw_full[i], 1), mbar_init(&raw_empty[i], 1);
+        for (int i = 0; i < 2; ++i)
+            mbar_init(&s_full[i], 1), mbar_init(&p_full[i], 128), mbar_init(&o_full[i], 1), mbar_init(&o_free[i], 128);
+        mbar_init(&pv_done, 1), mbar_init(&pair_bar, 256), mbar_init(&q_full, 1), mbar_init(&q_empty, 1), mbar_init(&drain, 1);
+        for (int i = 0; i < kItemRing; ++i) mbar_init(&item_full[i], 1), mbar_init(&item_empty[i], 6 + 4 * NT);
+        fence_barrier_init();
+        s_failed = 0;
+    }
+    if (tid == 64) prefetch_map(&tq), prefetch_map(&tk), prefetch_map(&tv);
     pdl_wait();
-    const int s = blockIdx.x, lane = threadIdx.x & 31;
-    const int warp = blockIdx.y * 8 + (threadIdx.x >> 5), warps = gridDim.y * 8;
-    const Seq sq = sequence(a, s, warp == 0 && lane == 0);
-    const int heads = a.kv_heads * a.group;
-    constexpr int E = D / 32;
-    for (long long u = warp; u < (long long)max(sq.rows, 0) * heads; u += warps) {
-        const int i = (int)(u / heads), qh = (int)(u - (long long)i * heads), h = qh / a.group;
-        const T *q = static_cast<const T *>(a.q) + (long long)(sq.row0 + i) * a.q_stride + (long long)qh * D;
-        const int keys = sq.empty ? 0 : sq.ctx + i + 1;
-        float m = -INFINITY, last = 0.f, l = 0.f, o[E];
+    // The join may be scheduled from here on; it waits for this grid's end.
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+
+    // ---- this CTA's share ----
+    {
+        if (tid < 2) p.headers[2 * blockIdx.x + tid].valid = 0;
+        if (tid == 0) s_range[0] = s_range[1] = Pos{a.num_seqs, 0, 0, 0};
+        const int seg = (a.num_seqs + kPrefillThreads - 1) / kPrefillThreads;
+        const int b0 = min(a.num_seqs, tid * seg), b1 = min(a.num_seqs, b0 + seg);
+        long long local = 0;
+        for (int s = b0; s < b1; ++s) {
+            const Costs<NT> c(sequence(a, s, blockIdx.x == 0), p.tile_tokens);
+            local += c.head() * a.kv_heads;
+        }
+        long long incl = local;
 #pragma unroll
-        for (int e = 0; e < E; ++e) o[e] = 0.f;
-        float ks = 1.f, vs = 1.f;
-        if (std::is_same_v<KV, uint8_t>) ks = __ldg(a.k_scale + h), vs = __ldg(a.v_scale + h);
-        for (int j0 = 0; j0 < keys; j0 += 32) {
-            const int j = j0 + lane;
-            long long row = -1;
-            if (j < keys) {
-                if (a.tables) {
-                    const int blk = __ldg(a.tables + (long long)s * a.table_stride + j / a.block_size);
-                    if (blk < 0 || blk >= a.num_blocks) record_error(a.err, kInvalidBlock, s);
-                    else row = (a.layer_row0 + (long long)blk * a.block_size + j % a.block_size) * a.kv_heads * D;
-                } else {
-                    row = (long long)(sq.row0 + j) * a.kv_stride;
+        for (int o = 1; o < 32; o <<= 1) {
+            const long long y = __shfl_up_sync(0xffffffffu, incl, o);
+            if (lane >= o) incl += y;
+        }
+        if (lane == 31) s_scan[warp] = incl;
+        __syncthreads();
+        long long add = 0, total = 0;
+#pragma unroll
+        for (int w = 0; w < kPrefillThreads / 32; ++w) {
+            if (w < warp) add += s_scan[w];
+            total += s_scan[w];
+        }
+        const long long first = add + incl - local, n = gridDim.x;
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+            const long long b = blockIdx.x + e;
+            const long long x = total / n * b + total % n * b / n;
+            if (b < n && x >= first && x < first + local) {
+                long long at = first;
+                for (int s = b0; s < b1; ++s) {
+                    const Costs<NT> c(sequence(a, s, false), p.tile_tokens);
+                    const long long w = c.head() * a.kv_heads;
+                    if (x < at + w) {
+                        s_range[e] = locate<NT, KEYS>(c, s, x - at, p.tile_tokens);
+                        break;
+                    }
+                    at += w;
                 }
             }
-            float sc = -INFINITY;
-            if (row >= 0) {
-                const KV *k = static_cast<const KV *>(a.k) + row + (long long)h * D;
-                sc = 0.f;
-                for (int d = 0; d < D; ++d) sc = fmaf(wide(q[d]), wide(k[d]), sc);
-                sc *= a.scale_log2 * ks;
-            }
-            float mx = sc;
-#pragma unroll
-            for (int off = 16; off > 0; off >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, off));
-            m = fmaxf(m, mx);
-            const float ref = m == -INFINITY ? 0.f : m;  // nothing but -inf so far: weights 0
-            const float corr = exp2f(last - ref), p = exp2f(sc - ref);
-            last = ref;
-            l = l * corr + p;
-#pragma unroll
-            for (int e = 0; e < E; ++e) o[e] *= corr;
-            for (int t = 0; t < 32; ++t) {
-                const float w = __shfl_sync(0xffffffffu, p, t);
-                const long long r = __shfl_sync(0xffffffffu, row, t);
-                if (r < 0) continue;
-                const KV *v = static_cast<const KV *>(a.v) + r + (long long)h * D + lane * E;
-#pragma unroll
-                for (int e = 0; e < E; ++e) o[e] = fmaf(w, wide(v[e]), o[e]);
+        }
+        if (blockIdx.x == 0 && tid == 0) s_range[0] = Pos{0, 0, 0, 0};
+    }
+    if (tid == 0) {
+        for (int i = 0; i < kItemRing; ++i) s_flag[i][kFlagWords] = 0;
+    }
+    fence_before();
+    __syncthreads();
+    fence_after();
+    const uint32_t tmem = s_tmem;
+
+    // Waits are bounded: after about 2 s, or once another role has given up,
+    // the wait fails, its role leaves, and the CTA drains and ends.
+    auto wait = [&](uint64_t *bar, uint32_t parity) -> bool {
+        if (mbar_try_wait(bar, parity)) return true;
+        const long long t0 = clock64();
+        while (!mbar_try_wait(bar, parity)) {
+            if (s_failed) return false;
+            if (clock64() - t0 > kWaitCycles) {
+                s_failed = 1;
+                record_error(a.err, kDeviceCode, blockIdx.x);
+                return false;
             }
         }
+        return true;
+    };
+    // Key tiles that some row masks: from the one that holds the first row's limit.
+    auto first_careful = [&](const Item &it) { return (it.key0 + 1) / KEYS; };
+    // Places in the K/V ring, relative to the item's first: K runs `ahead`
+    // tiles before V.
+    auto k_at = [](int i, int ahead) { return i < ahead ? i : 2 * i - ahead + 1; };
+    auto v_at = [](int j, int n, int ahead) { return j + min(n, j + ahead); };
+    const int ahead_rows = 1, ahead_keys = 2;
+    unsigned item_n = 0;  // items taken by this role
+
+    if (warp >= 8 && warp < 12) {
+        reg_dealloc<kOtherRegs>();
+    } else if (warp >= 12) {
+        reg_dealloc<kOtherRegs>();
+    } else {
+        reg_alloc<kSoftmaxRegs>();
+    }
+
+    if (warp < 4 * NT) {
+        // ================= softmax and epilogue =================
+        const int w = warp >> 2, row = tid & 127;
+        const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
+        const int group = a.group, tau = row / group, hq = row - tau * group;
+        unsigned s_ph[2] = {0, 0}, of_ph[2] = {0, 0}, pv_n = 0, pair_n = 0;
+        unsigned kt = 0;  // key tiles of earlier items
+        bool ok = true;
+        for (; ok; ++item_n) {
+            const unsigned ring = item_n % kItemRing;
+            ok = wait(&item_full[ring], (item_n / kItemRing) & 1);
+            if (!__all_sync(0xffffffffu, ok)) break;
+            const Item it = s_item[ring];
+            if (it.end) break;
+            const int n = it.t1 - it.t0;
+            const bool two = NT == 2 && it.two, keys = NT == 2 && !it.two;
+            const int my_token = tau + (two && w ? p.tile_tokens : 0);
+            const bool live = tau < p.tile_tokens && my_token < it.tokens;
+            const int limit = live ? it.key0 + my_token + 1 : 0;
+            // Tiles of this warpgroup: a first row tile may end a tile early.
+            int mine = n;
+            if (two && !w)
+                mine = max(0, min(it.t1, (it.key0 + min(p.tile_tokens, it.tokens) + KEYS - 1) / KEYS) - it.t0);
+            // The other warpgroup's: its o_full turns too.
+            int others = two && w ? max(0, min(it.t1, (it.key0 + min(p.tile_tokens, it.tokens) + KEYS - 1) / KEYS) - it.t0) : n;
+            if (keys) mine = (n - w + 1) / 2, others = (n - (w ^ 1) + 1) / 2;
+            float scale = a.scale_log2, v_scale = 1.f;
+            if constexpr (SRC == kPagedFp8) scale *= __ldg(a.k_scale + it.head), v_scale = __ldg(a.v_scale + it.head);
+            float m = -INFINITY, l = 0.f;
+            const bool warp_live = __any_sync(0xffffffffu, live);
+            const int careful = first_careful(it);
+            for (int j = 0; j < mine; ++j) {
+                const int t = it.t0 + (keys ? 2 * j + w : j);
+                const int buf = NT == 1 ? j & 1 : w;
+                const uint32_t s_addr = tmem + lanes + buf * G::kSCols;
+                ok = wait(&s_full[buf], s_ph[buf] & 1);
+                if (!__all_sync(0xffffffffu, ok)) break;
+                ++s_ph[buf];
+                fence_after();
+                if (warp_live) {
+                    uint32_t sr[KEYS];
 #pragma unroll
-        for (int off = 16; off > 0; off >>= 1) l += __shfl_xor_sync(0xffffffffu, l, off);
-        const long long at = (long long)(sq.row0 + i) * heads + qh;
+                    for (int c = 0; c < KEYS / 32; ++c) tmem_ld32(s_addr + c * 32, sr + c * 32);
+                    wait_ld();
+                    float *s = reinterpret_cast<float *>(sr);
+                    const unsigned blocks = SRC == kRows ? 0xffu : s_mask[(kt + t - it.t0) % kMaskRing];
+                    constexpr unsigned kAll = (1u << G::kGranules) - 1;
+                    if (t >= careful || (SRC != kRows && (blocks & kAll) != kAll)) {
+                        const int lim = limit - t * KEYS;
 #pragma unroll
-        for (int e = 0; e < E; ++e)
-            static_cast<T *>(a.out)[at * D + lane * E + e] = tight<T>(l > 0.f ? o[e] / l * vs : l == 0.f ? 0.f : l);
-        if (lane == 0 && a.lse) a.lse[at] = l > 0.f ? (m + log2f(l)) * 0.69314718055994531f : l == 0.f ? -INFINITY : l;
+                        for (int i = 0; i < KEYS; ++i)
+                            if (i >= lim || !((blocks >> (i / 16)) & 1u)) s[i] = -INFINITY;
+                    }
+                    float mx[4] = {s[0], s[1], s[2], s[3]};
+#pragma unroll
+                    for (int i = 4; i < KEYS; i += 4)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) mx[e] = fmaxf(mx[e], s[i + e]);
+                    const float mt = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * scale;
+                    const bool grew = mt > m + kLazy || (m == -INFINITY && mt > m);
+                    if (__any_sync(0xffffffffu, grew)) {
+                        const float mn = fmaxf(m, mt);
+                        const float corr = m == -INFINITY ? 0.f : ex2(m - mn);
+                        l *= corr;
+                        m = mn;
+                        if (j > 0) {
+                            // O holds the tiles before this one: S of this tile was
+                            // issued after their product (head_dim 256: two S buffers,
+                            // so wait for the last product).
+                            if constexpr (NT == 1) {
+                                ok = wait(&pv_done, (pv_n + j - 1) & 1);
+                                if (!__all_sync(0xffffffffu, ok)) break;
+                                fence_after();
+                            }
+                            const uint32_t o_addr = tmem + lanes + G::kOCol + (NT == 2 ? w * D : 0);
+#pragma unroll
+                            for (int c = 0; c < D / 32; ++c) {
+                                uint32_t o[32];
+                                tmem_ld32(o_addr + c * 32, o);
+                                wait_ld();
+#pragma unroll
+                                for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * corr);
+                                tmem_st32(o_addr + c * 32, o);
+                            }
+                        }
+                    }
+                    const float ref = m == -INFINITY ? 0.f : m;  // nothing yet: weights 2^-inf = 0
+                    const uint64_t sc2 = pair(scale, scale), mr2 = pair(-ref, -ref);
+                    uint64_t sum[2] = {pair(l, 0.f), pair(0.f, 0.f)};
+#pragma unroll
+                    for (int c = 0; c < KEYS / 64; ++c) {
+                        uint32_t pk[32];
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) {
+                            float x, y;
+                            unpair(fma2(pair(s[c * 64 + 2 * i], s[c * 64 + 2 * i + 1]), sc2, mr2), x, y);
+                            x = ex2(x);
+                            y = ex2(y);
+                            sum[i & 1] = add2(sum[i & 1], pair(x, y));
+                            pk[i] = pack2<T>(x, y);
+                        }
+                        tmem_st32(s_addr + c * 32, pk);
+                    }
+                    float u, v;
+                    unpair(add2(sum[0], sum[1]), u, v);
+                    l = u + v;
+                    wait_st();
+                }
+                fence_before();
+                mbar_arrive(&p_full[buf]);
+            }
+            if (!__all_sync(0xffffffffu, ok)) break;
+            if (NT == 1) pv_n += n;
+            kt += n;
+
+            // ---- epilogue: this row's O (key items: the two halves merged) ----
+            const long long out_row = (long long)(it.row0 + my_token) * (a.kv_heads * group) + (long long)it.head * group + hq;
+            const bool wait_mine = mine > 0;
+            if (wait_mine) {
+                const int ob = NT == 1 ? 0 : w;
+                ok = wait(&o_full[ob], of_ph[ob] & 1);
+                if (!__all_sync(0xffffffffu, ok)) break;
+                ++of_ph[ob];
+            }
+            int c0 = 0, c1 = D;
+            float f[2] = {1.f, 0.f};
+            bool use[2] = {true, false};
+            if constexpr (NT == 2) {
+                use[0] = w == 0 ? mine > 0 : false;
+                use[1] = w == 1 ? mine > 0 : false;
+                f[w] = 1.f;
+                f[w ^ 1] = 0.f;
+                if (keys) {
+                    stat[w * 128 + row] = make_float2(m, l);
+                    mbar_arrive(&pair_bar);
+                    ok = wait(&pair_bar, pair_n++ & 1);
+                    if (!__all_sync(0xffffffffu, ok)) break;
+                    const float2 other = stat[(w ^ 1) * 128 + row];
+                    const float mm = fmaxf(m, other.x);
+                    const float mine_f = m == -INFINITY ? 0.f : ex2(m - mm);
+                    const float other_f = other.x == -INFINITY ? 0.f : ex2(other.x - mm);
+                    // A NaN sum stays: 0 * NaN.
+                    l = l * mine_f + other.y * other_f;
+                    m = mm;
+                    f[w] = mine_f;
+                    f[w ^ 1] = other_f;
+                    use[0] = n > 0;
+                    use[1] = n > 1;
+                    c0 = w * (D / 2);
+                    c1 = c0 + D / 2;
+                    // The wait above covers this warpgroup's half alone.
+                    if (others > 0) {
+                        ok = wait(&o_full[w ^ 1], of_ph[w ^ 1] & 1);
+                        if (!__all_sync(0xffffffffu, ok)) break;
+                    }
+                }
+                of_ph[w ^ 1] += others > 0;
+            } else {
+                use[0] = n > 0;
+            }
+            fence_after();
+            const unsigned flagged = s_flag[ring][kFlagWords];
+            const float inv = l == 0.f ? 0.f : v_scale / l;
+#pragma unroll 1
+            for (int c = c0; c < c1; c += 32) {
+                float o[32];
+#pragma unroll
+                for (int i = 0; i < 32; ++i) o[i] = 0.f;
+                __syncwarp();
+                if (warp_live) {
+#pragma unroll
+                    for (int h = 0; h < NT; ++h) {
+                        if (!use[h]) continue;
+                        uint32_t r[32];
+                        tmem_ld32(tmem + lanes + G::kOCol + h * D + c, r);
+                        wait_ld();
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) o[i] = fmaf(__uint_as_float(r[i]), f[h], o[i]);
+                    }
+                }
+                if (live && flagged) {
+                    // Elements of V that were not finite, for the rows that attend them.
+                    for (int b = 0; b < kFlagWords * 32; ++b) {
+                        if (!((s_flag[ring][b >> 5] >> (b & 31)) & 1u)) continue;
+                        const int key = careful * KEYS + b;
+                        if (key >= limit) continue;
+                        if constexpr (SRC == kPagedFp8) {
+                            const int blk = __ldg(a.tables + (long long)it.seq * a.table_stride + key / a.block_size);
+                            const uint8_t *v = static_cast<const uint8_t *>(a.v) +
+                                               (a.layer_row0 + (long long)blk * a.block_size + key % a.block_size) * a.kv_heads * D +
+                                               (long long)it.head * D + c;
+                            for (int i = 0; i < 32; ++i)
+                                if ((__ldg(v + i) & 0x7fu) == 0x7fu) o[i] = NAN;
+                        } else {
+                            const T *v = static_cast<const T *>(a.v);
+                            if constexpr (SRC == kPaged) {
+                                const int blk = __ldg(a.tables + (long long)it.seq * a.table_stride + key / a.block_size);
+                                v += (a.layer_row0 + (long long)blk * a.block_size + key % a.block_size) * a.kv_heads * D;
+                            } else {
+                                v += (long long)(it.base + key) * a.kv_stride;
+                            }
+                            v += (long long)it.head * D + c;
+#pragma unroll
+                            for (int i = 0; i < 32; ++i) {
+                                const float x = wide(v[i]);
+                                if (!isfinite(x)) o[i] += x;
+                            }
+                        }
+                    }
+                }
+                if (!live) {
+                } else if (it.slot < 0) {
+                    T *out = static_cast<T *>(a.out) + out_row * D + c;
+#pragma unroll
+                    for (int i = 0; i < 32; i += 8) {
+                        uint4 x;
+                        x.x = pack2<T>(o[i] * inv, o[i + 1] * inv);
+                        x.y = pack2<T>(o[i + 2] * inv, o[i + 3] * inv);
+                        x.z = pack2<T>(o[i + 4] * inv, o[i + 5] * inv);
+                        x.w = pack2<T>(o[i + 6] * inv, o[i + 7] * inv);
+                        *reinterpret_cast<uint4 *>(out + i) = x;
+                    }
+                } else {
+                    float *part = p.part_o + ((long long)it.slot * G::kSlotRows + (two ? w * 128 : 0) + row) * D + c;
+#pragma unroll
+                    for (int i = 0; i < 32; i += 4)
+                        *reinterpret_cast<float4 *>(part + i) = make_float4(o[i], o[i + 1], o[i + 2], o[i + 3]);
+                }
+            }
+            __syncwarp();
+            if (live && (!keys || w == 0)) {
+                if (it.slot < 0) {
+                    if (a.lse) a.lse[out_row] = l == 0.f ? -INFINITY : (m + log2f(l)) * 0.69314718055994531f;
+                } else {
+                    p.part_ml[(long long)it.slot * G::kSlotRows + (two ? w * 128 : 0) + row] = make_float2(m, l);
+                }
+            }
+            if (it.slot >= 0 && tid == 0) {
+                Header h{1, it.t1 == it.tiles, it.row0, it.tokens, it.head, two, {0, 0}};
+                p.headers[it.slot] = h;
+            }
+            fence_before();
+            if (keys) {  // both halves have read both accumulators, and the statistics
+                mbar_arrive(&pair_bar);
+                ok = wait(&pair_bar, pair_n++ & 1);
+                if (!__all_sync(0xffffffffu, ok)) break;
+            }
+            if (mine > 0) mbar_arrive(&o_free[NT == 1 ? 0 : w]);
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&item_empty[ring]);
+        }
+    } else if (warp == 8) {
+        // ================= the products =================
+        if (lane == 0) {
+            constexpr uint32_t id_s = instr_desc<T>(128, KEYS, false), id_o = instr_desc<T>(128, D, true);
+            const uint32_t q0 = smem_u32(sq), kv0 = smem_u32(skv);
+            unsigned pos = 0, p_ph[2] = {0, 0}, ou[2] = {0, 0}, qn = 0;
+            bool ok = true;
+            auto stage = [&](unsigned at) { return at % ST; };
+            auto full = [&](unsigned at) { return wait(&kv_full[at % ST], (at / ST) & 1); };
+            auto scores = [&](int qt, int buf, unsigned at) {
+                const uint32_t kb = kv0 + stage(at) * G::kTile, qb = q0 + qt * G::kQTile;
+#pragma unroll
+                for (int k = 0; k < D / 16; ++k)
+                    mma_ss(tmem + buf * G::kSCols, smem_desc(qb + (k / 4) * (128 * 128) + (k % 4) * 32, 16, 1024),
+                           smem_desc(kb + (k / 4) * G::kSlab + (k % 4) * 32, 16, 1024), id_s, k > 0);
+            };
+            auto values = [&](int buf, int ob, unsigned at, bool accumulate) {
+                const uint32_t vb = kv0 + stage(at) * G::kTile;
+#pragma unroll
+                for (int k = 0; k < KEYS / 16; ++k)
+                    mma_ts(tmem + G::kOCol + ob * D, tmem + buf * G::kSCols + k * 8,
+                           smem_desc(vb + k * 2048, G::kSlab, 1024), id_o, accumulate || k > 0);
+            };
+            auto o_ready = [&](int ob) { return ou[ob] == 0 || wait(&o_free[ob], (ou[ob] - 1) & 1); };
+            for (; ok; ++item_n) {
+                const unsigned ring = item_n % kItemRing;
+                if (!wait(&item_full[ring], (item_n / kItemRing) & 1)) break;
+                const Item it = s_item[ring];
+                mbar_arrive(&item_empty[ring]);
+                if (it.end) break;
+                const int n = it.t1 - it.t0;
+                if (n == 0) continue;
+                if (!(ok = wait(&q_full, qn & 1))) break;
+                ++qn;
+                fence_after();
+                if (NT == 2 && it.two) {
+                    const int n0 = max(0, min(it.t1, (it.key0 + min(p.tile_tokens, it.tokens) + KEYS - 1) / KEYS) - it.t0);
+                    if (!(ok = full(pos))) break;
+                    fence_after();
+                    if (n0 > 0) scores(0, 0, pos), commit(&s_full[0]);
+                    scores(1, 1, pos);
+                    commit(&s_full[1]);
+                    commit(&kv_empty[stage(pos)]);
+                    if (n == 1) commit(&q_empty);
+                    for (int j = 0; j < n; ++j) {
+                        const unsigned va = pos + v_at(j, n, ahead_rows), ka = pos + k_at(j + 1, ahead_rows);
+                        if (!(ok = full(va))) break;
+                        if (j < n0) {
+                            if (!(ok = wait(&p_full[0], p_ph[0]++ & 1))) break;
+                            if (j == 0 && !(ok = o_ready(0))) break;
+                            fence_after();
+                            values(0, 0, va, j > 0);
+                            if (j + 1 == n0) commit(&o_full[0]), ++ou[0];
+                        }
+                        if (j + 1 < n) {
+                            if (!(ok = full(ka))) break;
+                            fence_after();
+                            if (j + 1 < n0) scores(0, 0, ka), commit(&s_full[0]);
+                        }
+                        if (!(ok = wait(&p_full[1], p_ph[1]++ & 1))) break;
+                        if (j == 0 && !(ok = o_ready(1))) break;
+                        fence_after();
+                        values(1, 1, va, j > 0);
+                        commit(&kv_empty[stage(va)]);
+                        if (j + 1 < n) {
+                            scores(1, 1, ka);
+                            commit(&s_full[1]);
+                            commit(&kv_empty[stage(ka)]);
+                            if (j + 2 == n) commit(&q_empty);
+                        } else {
+                            commit(&o_full[1]);
+                            ++ou[1];
+                        }
+                    }
+                } else {
+                    for (int i = 0; i < min(2, n); ++i) {
+                        if (!(ok = full(pos + i))) break;
+                        fence_after();
+                        scores(0, i, pos + i);
+                        commit(&s_full[i]);
+                        commit(&kv_empty[stage(pos + i)]);
+                    }
+                    if (!ok) break;
+                    if (n <= 2) commit(&q_empty);
+                    for (int j = 0; j < n; ++j) {
+                        const int buf = j & 1, ob = NT == 2 ? buf : 0;
+                        const bool first = NT == 2 ? j < 2 : j == 0;
+                        const unsigned va = pos + v_at(j, n, ahead_keys), ka = pos + k_at(j + 2, ahead_keys);
+                        if (!(ok = full(va))) break;
+                        if (!(ok = wait(&p_full[buf], p_ph[buf]++ & 1))) break;
+                        if (first && !(ok = o_ready(ob))) break;
+                        fence_after();
+                        values(buf, ob, va, !first);
+                        commit(&kv_empty[stage(va)]);
+                        if (NT == 1) commit(&pv_done);
+                        if (j + 2 < n) {
+                            if (!(ok = full(ka))) break;
+                            fence_after();
+                            scores(0, buf, ka);
+                            commit(&s_full[buf]);
+                            commit(&kv_empty[stage(ka)]);
+                            if (j + 3 == n) commit(&q_empty);
+                        }
+                        if (NT == 2 ? j + 2 >= n : j + 1 == n) commit(&o_full[ob]), ++ou[ob];
+                    }
+                }
+                pos += 2 * n;
+            }
+            // Nothing may be in flight when tensor memory is freed.
+            commit(&drain);
+            const long long t0 = clock64();
+            while (!mbar_try_wait(&drain, 0) && clock64() - t0 < kWaitCycles) {}
+        }
+    } else if (warp == 9) {
+        // ================= K and V by TMA =================
+        unsigned pos = 0, kt = 0;
+        bool ok = true;
+        const uint32_t kv0 = smem_u32(skv), raw0 = smem_u32(sraw);
+        for (; ok; ++item_n) {
+            const unsigned ring = item_n % kItemRing;
+            ok = wait(&item_full[ring], (item_n / kItemRing) & 1);
+            if (!__all_sync(0xffffffffu, ok)) break;
+            const Item it = s_item[ring];
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&item_empty[ring]);
+            if (it.end) break;
+            const int n = it.t1 - it.t0, ahead = NT == 2 && it.two ? ahead_rows : ahead_keys;
+            const int careful = first_careful(it), len = it.key0 + it.tokens;
+            for (int f = 0; f < 2 * n; ++f) {
+                // Fill f of the item: K 0 .. ahead - 1, then V j and K j + ahead in turn.
+                bool is_k;
+                int j;
+                const int lead = min(ahead, n), both = n - lead;
+                if (f < lead) is_k = true, j = f;
+                else if (f - lead < 2 * both) is_k = (f - lead) & 1, j = ((f - lead) >> 1) + (is_k ? ahead : 0);
+                else is_k = false, j = both + (f - lead - 2 * both);
+                const int t = it.t0 + j;
+                const unsigned at = pos + f;
+                if constexpr (SRC == kRows) {
+                    if (lane == 0) {
+                        ok = wait(&kv_empty[at % ST], ((at / ST) & 1) ^ 1);
+                        if (ok && !is_k && t >= careful) {
+                            mbar_arrive(&by_hand_go[at % ST]);
+                        } else if (ok) {
+                            mbar_expect_tx(&kv_full[at % ST], G::kTile);
+#pragma unroll
+                            for (int c = 0; c < G::kSlabs; ++c)
+                                tma_load_2d(kv0 + (at % ST) * G::kTile + c * G::kSlab, is_k ? &tk : &tv,
+                                            it.head * D + c * 64, it.base + t * KEYS, &kv_full[at % ST]);
+                        }
+                    }
+                    ok = __shfl_sync(0xffffffffu, ok, 0);
+                    if (!ok) break;
+                } else {
+                    const bool by_hand = SRC == kPaged && !is_k && t >= careful;
+                    // Lane g brings the tile's 16-key granule g.
+                    const int key = t * KEYS + lane * 16;
+                    const bool have = lane < G::kGranules && key < len;
+                    int blk = -1;
+                    if (have && !by_hand) blk = __ldg(a.tables + (long long)it.seq * a.table_stride + key / a.block_size);
+                    const bool good = have && blk >= 0 && blk < a.num_blocks;
+                    if (have && !good && !by_hand) record_error(a.err, kInvalidBlock, it.seq);
+                    const unsigned bits = __ballot_sync(0xffffffffu, good || (lane < G::kGranules && !have));
+                    const unsigned loads = __ballot_sync(0xffffffffu, good);
+                    uint64_t *full = SRC == kPagedFp8 ? &raw_full[at % RS] : &kv_full[at % ST];
+                    uint64_t *empty = SRC == kPagedFp8 ? &raw_empty[at % RS] : &kv_empty[at % ST];
+                    const unsigned turn = SRC == kPagedFp8 ? at / RS : at / ST;
+                    ok = wait(empty, (turn & 1) ^ 1);
+                    ok = __all_sync(0xffffffffu, ok);
+                    if (!ok) break;
+                    if (by_hand) {
+                        if (lane == 0) mbar_arrive(&by_hand_go[at % ST]);
+                        continue;
+                    }
+                    if (is_k && lane == 0) s_mask[(kt + j) % kMaskRing] = (unsigned char)bits;
+                    const int y = (int)(a.layer_row0 + (long long)blk * a.block_size + key % a.block_size);
+                    if constexpr (SRC == kPagedFp8) {
+                        __syncwarp();
+                        if (lane == 0) mbar_expect_tx(full, __popc(loads) * 16 * D);
+                        __syncwarp();
+                        if (good)
+                            tma_load_2d(raw0 + (at % RS) * G::kRawTile + lane * 16 * D, is_k ? &tk : &tv, it.head * D, y, full);
+                    } else {
+                        unsigned char *dst = skv + (at % ST) * G::kTile;
+                        if (!is_k && loads != (1u << G::kGranules) - 1) {
+                            // A block outside the pool: its values are zeros.
+                            for (int g = 0; g < G::kGranules; ++g) {
+                                if ((loads >> g) & 1u) continue;
+                                for (int i = lane; i < G::kSlabs * 128; i += 32)
+                                    *reinterpret_cast<uint4 *>(dst + (i >> 7) * G::kSlab + g * 2048 + (i & 127) * 16) =
+                                        make_uint4(0, 0, 0, 0);
+                            }
+                            fence_async();
+                        }
+                        __syncwarp();
+                        if (lane == 0) mbar_expect_tx(full, __popc(loads) * 16 * D * 2);
+                        __syncwarp();
+                        if (good) {
+#pragma unroll
+                            for (int c = 0; c < G::kSlabs; ++c)
+                                tma_load_2d(smem_u32(dst) + c * G::kSlab + lane * 2048, is_k ? &tk : &tv,
+                                            it.head * D + c * 64, y, full);
+                        }
+                    }
+                }
+            }
+            pos += 2 * n;
+            kt += n;
+        }
+        if (!ok && lane == 0) {
+            // Copies in flight land before the CTA's memory is given up.
+            const long long t0 = clock64();
+            while (clock64() - t0 < 20000000ll) {}
+        }
+    } else if (warp == 10) {
+        // ================= items, and Q by TMA =================
+        Pos at = s_range[0];
+        const Pos end = s_range[1];
+        unsigned qn = 0;
+        bool ok = true;
+        auto publish = [&](const Item &it) -> bool {
+            const unsigned ring = item_n % kItemRing;
+            bool good = true;
+            if (lane == 0) {
+                if (item_n >= kItemRing) good = wait(&item_empty[ring], ((item_n / kItemRing) & 1) ^ 1);
+                if (good) {
+                    s_item[ring] = it;
+                    for (int i = 0; i <= kFlagWords; ++i) s_flag[ring][i] = 0;
+                    mbar_arrive(&item_full[ring]);
+                }
+            }
+            ++item_n;
+            return __shfl_sync(0xffffffffu, good, 0);
+        };
+        while (ok && at.s < a.num_seqs && at.s <= end.s) {
+            // The next sequence with rows, from at.s on: 32 at a time.
+            const int s = at.s + lane;
+            Seq q{0, 0, 0, false};
+            if (s < a.num_seqs) q = sequence(a, s, false);
+            const unsigned some = __ballot_sync(0xffffffffu, q.rows > 0);
+            if (!some) {
+                at = Pos{at.s + 32, 0, 0, 0};
+                continue;
+            }
+            const int src = __ffs(some) - 1;
+            if (src > 0) at = Pos{at.s + src, 0, 0, 0};
+            q.row0 = __shfl_sync(0xffffffffu, q.row0, src);
+            q.rows = __shfl_sync(0xffffffffu, q.rows, src);
+            q.ctx = __shfl_sync(0xffffffffu, q.ctx, src);
+            q.empty = __shfl_sync(0xffffffffu, q.empty, src);
+            const int per = NT * p.tile_tokens, items = (q.rows - 1) / per + 1;
+            for (; ok && at.h < a.kv_heads; ++at.h, at.i = 0) {
+                for (; ok && at.i < items; ++at.i, at.t = 0) {
+                    const bool last = at.s == end.s && at.h == end.h && at.i == end.i;
+                    const bool past = at.s > end.s || (at.s == end.s && (at.h > end.h || (at.h == end.h && at.i > end.i)));
+                    if (past || (last && end.t <= at.t)) goto planned;
+                    Item it{};
+                    it.seq = at.s;
+                    it.head = at.h;
+                    const int tok0 = at.i * per;
+                    it.row0 = q.row0 + tok0;
+                    it.tokens = min(per, q.rows - tok0);
+                    it.key0 = q.ctx + tok0;
+                    it.base = q.row0;
+                    it.tiles = q.empty ? 0 : (it.key0 + it.tokens - 1) / KEYS + 1;
+                    it.t0 = at.t;
+                    it.t1 = last ? end.t : it.tiles;
+                    it.two = NT == 2 && it.tokens > p.tile_tokens;
+                    it.slot = it.t0 > 0 ? 2 * (int)blockIdx.x : it.t1 < it.tiles ? 2 * (int)blockIdx.x + 1 : -1;
+                    if (!(ok = publish(it))) break;
+                    if (it.t1 > it.t0) {
+                        if (lane == 0) {
+                            if (qn > 0) ok = wait(&q_empty, (qn - 1) & 1);
+                            if (ok) {
+                                const int tiles = it.two ? 2 : 1;
+                                const uint32_t bytes = (uint32_t)p.tile_tokens * a.group * 128;
+                                mbar_expect_tx(&q_full, tiles * G::kSlabs * bytes);
+                                for (int x = 0; x < tiles; ++x)
+                                    for (int c = 0; c < G::kSlabs; ++c)
+                                        tma_load_3d(smem_u32(sq) + x * G::kQTile + c * (128 * 128), &tq, c * 64,
+                                                    it.head * a.group, it.row0 + x * p.tile_tokens, &q_full);
+                            }
+                        }
+                        ++qn;
+                        ok = __shfl_sync(0xffffffffu, ok, 0);
+                    }
+                }
+            }
+            at = Pos{at.s + 1, 0, 0, 0};
+        }
+    planned:
+        if (ok) {
+            Item it{};
+            it.end = 1;
+            publish(it);
+        }
+        if (!ok && lane == 0) {
+            const long long t0 = clock64();
+            while (clock64() - t0 < 20000000ll) {}
+        }
+    } else if (warp >= 12) {
+        // ================= V tiles by hand; fp8 conversion =================
+        const int t128 = tid & 127;
+        unsigned pos = 0, kt = 0, go_ph = 0;
+        bool ok = true;
+        auto together = [&](bool good) -> bool {  // all four warps, and whether all are well
+            int r;
+            __syncwarp();
+            asm volatile(
+                "{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %1, 0;\n\t"
+                "barrier.cta.red.and.aligned.pred q, 2, 128, p;\n\tselp.b32 %0, 1, 0, q;\n\t}"
+                : "=r"(r) : "r"((int)good) : "memory");
+            return r != 0;
+        };
+        for (; ok; ++item_n) {
+            const unsigned ring = item_n % kItemRing;
+            ok = together(wait(&item_full[ring], (item_n / kItemRing) & 1));
+            if (!ok) break;
+            const Item it = s_item[ring];
+            if (it.end) break;
+            const int n = it.t1 - it.t0, ahead = NT == 2 && it.two ? ahead_rows : ahead_keys;
+            const int careful = first_careful(it), len = it.key0 + it.tokens;
+            auto note = [&](int key) {
+                const int b = key - careful * KEYS;
+                if (b >= 0 && b < kFlagWords * 32) {
+                    atomicOr(&s_flag[ring][b >> 5], 1u << (b & 31));
+                    s_flag[ring][kFlagWords] = 1;
+                }
+            };
+            if constexpr (SRC != kPagedFp8) {
+                for (int t = max(it.t0, careful); t < it.t1; ++t) {
+                    const unsigned at = pos + v_at(t - it.t0, n, ahead);
+                    // The K/V warp has seen the stage empty; one turn of this
+                    // barrier per tile filled here.
+                    ok = together(wait(&by_hand_go[at % ST], (go_ph >> (at % ST)) & 1));
+                    if (!ok) break;
+                    go_ph ^= 1u << (at % ST);
+                    unsigned char *dst = skv + (at % ST) * G::kTile;
+                    constexpr int kUnits = D / 8;                       // 16-byte units of a row
+                    constexpr int kEach = KEYS * kUnits / 128, kBatch = kEach < 8 ? kEach : 8;
+#pragma unroll 1
+                    for (int b = 0; b < kEach; b += kBatch) {
+                        uint4 x[kBatch];
+#pragma unroll
+                        for (int e = 0; e < kBatch; ++e) {
+                            const int i = (b + e) * 128 + t128, r = i / kUnits, u = i % kUnits, key = t * KEYS + r;
+                            x[e] = make_uint4(0, 0, 0, 0);
+                            if (key >= len) continue;
+                            const T *src = static_cast<const T *>(a.v) + (long long)it.head * D + u * 8;
+                            if constexpr (SRC == kPaged) {
+                                const int blk = __ldg(a.tables + (long long)it.seq * a.table_stride + key / a.block_size);
+                                if (blk < 0 || blk >= a.num_blocks) continue;
+                                src += (a.layer_row0 + (long long)blk * a.block_size + key % a.block_size) * a.kv_heads * D;
+                            } else {
+                                src += (long long)(it.base + key) * a.kv_stride;
+                            }
+                            x[e] = *reinterpret_cast<const uint4 *>(src);
+                        }
+#pragma unroll
+                        for (int e = 0; e < kBatch; ++e) {
+                            const int i = (b + e) * 128 + t128, r = i / kUnits, u = i % kUnits;
+                            uint32_t wds[4] = {x[e].x, x[e].y, x[e].z, x[e].w};
+                            uint32_t bad = 0;
+#pragma unroll
+                            for (int k = 0; k < 4; ++k) bad |= nonfinite_mask<T>(wds[k]);
+                            if (bad) {
+#pragma unroll
+                                for (int k = 0; k < 4; ++k) {
+                                    const uint32_t m = nonfinite_mask<T>(wds[k]);
+                                    if (m & 0x8000u) wds[k] &= 0xffff0000u;
+                                    if (m & 0x80000000u) wds[k] &= 0x0000ffffu;
+                                }
+                                note(t * KEYS + r);
+                            }
+                            *reinterpret_cast<uint4 *>(dst + (u / 8) * G::kSlab + r * 128 + (((u % 8) ^ (r & 7)) << 4)) =
+                                make_uint4(wds[0], wds[1], wds[2], wds[3]);
+                        }
+                    }
+                    fence_async();
+                    together(true);
+                    if (t128 == 0) mbar_arrive(&kv_full[at % ST]);
+                }
+            } else {
+                for (int f = 0; f < 2 * n && ok; ++f) {
+                    bool is_k;
+                    int j;
+                    const int lead = min(ahead, n), both = n - lead;
+                    if (f < lead) is_k = true, j = f;
+                    else if (f - lead < 2 * both) is_k = (f - lead) & 1, j = ((f - lead) >> 1) + (is_k ? ahead : 0);
+                    else is_k = false, j = both + (f - lead - 2 * both);
+                    const int t = it.t0 + j;
+                    const unsigned at = pos + f;
+                    bool good = wait(&raw_full[at % RS], (at / RS) & 1);
+                    good = good && wait(&kv_empty[at % ST], ((at / ST) & 1) ^ 1);
+                    ok = together(good);
+                    if (!ok) break;
+                    unsigned char *dst = skv + (at % ST) * G::kTile;
+                    const unsigned char *src = sraw + (at % RS) * G::kRawTile;
+                    const unsigned bits = s_mask[(kt + j) % kMaskRing];
+                    constexpr int kUnits = D / 16, kEach = KEYS * kUnits / 128;
+#pragma unroll
+                    for (int e = 0; e < kEach; ++e) {
+                        const int i = e * 128 + t128, r = i / kUnits, u = i % kUnits;
+                        uint4 x = *reinterpret_cast<const uint4 *>(src + r * D + u * 16);
+                        // Values that no row may meet are zeros.
+                        const bool gone = !is_k && (t * KEYS + r >= len || !((bits >> (r / 16)) & 1u));
+                        if (gone) x = make_uint4(0, 0, 0, 0);
+                        if (!is_k && t >= careful) {
+                            uint32_t *w4 = reinterpret_cast<uint32_t *>(&x);
+#pragma unroll
+                            for (int k = 0; k < 4; ++k) {
+                                const uint32_t hit = ((w4[k] & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u;  // NaN codes
+                                if (hit) {
+                                    w4[k] &= ~((hit >> 7) * 0xffu);
+                                    note(t * KEYS + r);
+                                }
+                            }
+                        }
+                        const uint32_t w4[4] = {x.x, x.y, x.z, x.w};
+                        uint4 lo, hi;
+                        lo.x = codes_to<T>(w4[0]), lo.y = codes_to<T>(w4[0] >> 16);
+                        lo.z = codes_to<T>(w4[1]), lo.w = codes_to<T>(w4[1] >> 16);
+                        hi.x = codes_to<T>(w4[2]), hi.y = codes_to<T>(w4[2] >> 16);
+                        hi.z = codes_to<T>(w4[3]), hi.w = codes_to<T>(w4[3] >> 16);
+                        unsigned char *row = dst + (u / 4) * G::kSlab + r * 128;
+                        const int c = 2 * (u % 4);
+                        *reinterpret_cast<uint4 *>(row + ((c ^ (r & 7)) << 4)) = lo;
+                        *reinterpret_cast<uint4 *>(row + (((c + 1) ^ (r & 7)) << 4)) = hi;
+                    }
+                    fence_async();
+                    together(true);
+                    if (t128 == 0) {
+                        mbar_arrive(&kv_full[at % ST]);
+                        mbar_arrive(&raw_empty[at % RS]);
+                    }
+                }
+            }
+            if (!ok) break;
+            pos += 2 * n;
+            kt += n;
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&item_empty[ring]);
+        }
+    }
+    __syncwarp();
+    fence_before();
+    __syncthreads();
+    if (warp == 0) {
+        fence_after();
+        tmem_free(tmem, 512);
     }
 }
 
-template <typename T, typename KV>
-cudaError_t launch_simple(const PrefillLaunch &a, int sms, cudaStream_t st) {
-    const long long warps = (long long)a.max_new * a.kv_heads * a.group;
-    const dim3 grid((unsigned)a.num_seqs, (unsigned)std::max<long long>(1, std::min<long long>((warps + 7) / 8, sms * 8)));
-    auto kern = a.head_dim == 64 ? prefill_attention_kernel<T, KV, 64>
-                : a.head_dim == 128 ? prefill_attention_kernel<T, KV, 128> : prefill_attention_kernel<T, KV, 256>;
-    return launch_pdl(kern, grid, dim3(256), 0, st, a);
+// Joins the partials of one split item, from the CTA whose share the item
+// begins in on: out = sum_i 2^(m_i - M) O_i / sum_i 2^(m_i - M) l_i, in the
+// order of the keys. A warp per row.
+constexpr int kJoinRows = 32;
+template <typename T, int D, int ROW_TILES>
+__global__ void __launch_bounds__(256) prefill_join_kernel(const __grid_constant__ Params p, int ctas) {
+    __shared__ int s_slot[512];
+    __shared__ int s_count;
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    const PrefillLaunch &a = p.a;
+    const int b = blockIdx.x;
+    const Header h = p.headers[2 * b + 1];
+    if (!h.valid) return;
+    const int group = a.group, r0 = blockIdx.y * kJoinRows, w = r0 / 128;
+    if (w && !h.two) return;
+    if (((r0 & 127) / group) + w * p.tile_tokens >= h.tokens || (r0 & 127) / group >= p.tile_tokens) return;
+    for (int i = threadIdx.x; i < ctas; i += 256)
+        s_slot[i] = i <= b ? 0 : p.headers[2 * i].valid * (p.headers[2 * i].last ? 2 : 1);
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        int n = 0;
+        for (int i = b + 1; i < ctas; ++i) {
+            const int v = s_slot[i];
+            if (!v) continue;
+            s_slot[n++] = 2 * i;
+            if (v == 2) break;
+        }
+        s_count = n;
+    }
+    __syncthreads();
+    const int count = s_count + 1, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    constexpr int kRows = ROW_TILES * 128, E = D / 32;
+    const float v_scale = a.v_scale ? __ldg(a.v_scale + h.head) : 1.f;
+    for (int r = r0 + warp; r < r0 + kJoinRows; r += 8) {
+        const int row = r & 127, tau = row / group, token = tau + w * p.tile_tokens;
+        if (tau >= p.tile_tokens || token >= h.tokens) continue;
+        auto slot = [&](int i) { return (long long)(i == 0 ? 2 * b + 1 : s_slot[i - 1]) * kRows + r; };
+        float M = -INFINITY;
+        for (int i = lane; i < count; i += 32) M = fmaxf(M, p.part_ml[slot(i)].x);
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
+        float L = 0.f, acc[E];
+#pragma unroll
+        for (int e = 0; e < E; ++e) acc[e] = 0.f;
+#pragma unroll 4
+        for (int i = 0; i < count; ++i) {
+            const float2 ml = p.part_ml[slot(i)];
+            const float f = ml.x == -INFINITY ? 0.f : ex2(ml.x - M);
+            L = fmaf(ml.y, f, L);
+            const float *o = p.part_o + slot(i) * D + lane * E;
+            float x[E];
+            if constexpr (E == 2) *reinterpret_cast<float2 *>(x) = *reinterpret_cast<const float2 *>(o);
+            else
+#pragma unroll
+                for (int e = 0; e < E; e += 4) *reinterpret_cast<float4 *>(x + e) = *reinterpret_cast<const float4 *>(o + e);
+#pragma unroll
+            for (int e = 0; e < E; ++e) acc[e] = fmaf(x[e], f, acc[e]);
+        }
+        const float inv = L == 0.f ? 0.f : v_scale / L;
+        const long long out_row = (long long)(h.row0 + token) * (a.kv_heads * group) + (long long)h.head * group + (row - tau * group);
+        uint32_t packed[E / 2];
+#pragma unroll
+        for (int e = 0; e < E; e += 2) packed[e / 2] = pack2<T>(acc[e] * inv, acc[e + 1] * inv);
+        uint32_t *out = reinterpret_cast<uint32_t *>(static_cast<T *>(a.out) + out_row * D + lane * E);
+        if constexpr (E == 2) *out = packed[0];
+        else if constexpr (E == 4) *reinterpret_cast<uint2 *>(out) = make_uint2(packed[0], packed[1]);
+        else *reinterpret_cast<uint4 *>(out) = make_uint4(packed[0], packed[1], packed[2], packed[3]);
+        if (lane == 0 && a.lse) a.lse[out_row] = L == 0.f ? -INFINITY : (M + log2f(L)) * 0.69314718055994531f;
+    }
+}
+
+PFN_cuTensorMapEncodeTiled_v12000 encoder() {
+    static const PFN_cuTensorMapEncodeTiled_v12000 f = [] {
+        void *fn = nullptr;
+        cudaDriverEntryPointQueryResult q{};
+        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &fn, cudaEnableDefault, &q) != cudaSuccess ||
+            q != cudaDriverEntryPointSuccess)
+            fn = nullptr;
+        return reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(fn);
+    }();
+    return f;
+}
+
+// [rows][cols] elements, row pitch `stride`, boxes of box_rows x box_cols.
+bool map_2d(CUtensorMap *m, CUtensorMapDataType t, int es, const void *base, long long cols, long long rows,
+            long long stride, int box_cols, int box_rows, CUtensorMapSwizzle swizzle) {
+    const cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows};
+    const cuuint64_t strides[1] = {(cuuint64_t)(stride * es)};
+    const cuuint32_t box[2] = {(cuuint32_t)box_cols, (cuuint32_t)box_rows}, ones[2] = {1, 1};
+    return encoder()(m, t, 2, const_cast<void *>(base), dims, strides, box, ones, CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle,
+                     CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <typename T, int D, Source SRC>
+cudaError_t launch_tiles(const PrefillLaunch &a, const PrefillWorkspace &ws, int sms, cudaStream_t st) {
+    using G = Geom<D, SRC>;
+    if (!encoder()) return cudaErrorNotSupported;
+    const CUtensorMapDataType t = std::is_same_v<T, __half> ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+    const int heads = a.kv_heads * a.group, tile_tokens = 128 / a.group;
+    alignas(64) CUtensorMap tq, tk, tv;
+    {
+        // [tokens][heads][D]; a box is 64 elements of a tile's tokens and the group's heads: its rows in order.
+        const cuuint64_t dims[3] = {(cuuint64_t)D, (cuuint64_t)heads, (cuuint64_t)a.num_tokens};
+        const cuuint64_t strides[2] = {(cuuint64_t)D * 2, (cuuint64_t)a.q_stride * 2};
+        const cuuint32_t box[3] = {64, (cuuint32_t)a.group, (cuuint32_t)tile_tokens}, ones[3] = {1, 1, 1};
+        if (encoder()(&tq, t, 3, const_cast<void *>(a.q), dims, strides, box, ones, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                      CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                      CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
+            return cudaErrorInvalidValue;
+    }
+    const long long entry = (long long)a.kv_heads * D;
+    bool ok;
+    if constexpr (SRC == kRows) {
+        ok = map_2d(&tk, t, 2, a.k, entry, a.num_tokens, a.kv_stride, 64, G::kKeys, CU_TENSOR_MAP_SWIZZLE_128B) &&
+             map_2d(&tv, t, 2, a.v, entry, a.num_tokens, a.kv_stride, 64, G::kKeys, CU_TENSOR_MAP_SWIZZLE_128B);
+    } else if constexpr (SRC == kPagedFp8) {
+        ok = map_2d(&tk, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, a.k, entry, a.pool_rows, entry, D, 16, CU_TENSOR_MAP_SWIZZLE_NONE) &&
+             map_2d(&tv, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, a.v, entry, a.pool_rows, entry, D, 16, CU_TENSOR_MAP_SWIZZLE_NONE);
+    } else {
+        ok = map_2d(&tk, t, 2, a.k, entry, a.pool_rows, entry, 64, 16, CU_TENSOR_MAP_SWIZZLE_128B) &&
+             map_2d(&tv, t, 2, a.v, entry, a.pool_rows, entry, 64, 16, CU_TENSOR_MAP_SWIZZLE_128B);
+    }
+    if (!ok) return cudaErrorInvalidValue;
+    Params p{a, tile_tokens, nullptr, nullptr, nullptr};
+    unsigned char *at = static_cast<unsigned char *>(ws.base);
+    p.part_o = reinterpret_cast<float *>(at);
+    at += (size_t)2 * ws.ctas * G::kSlotRows * D * sizeof(float);
+    p.part_ml = reinterpret_cast<float2 *>(at);
+    at += (size_t)2 * ws.ctas * G::kSlotRows * sizeof(float2);
+    p.headers = reinterpret_cast<Header *>(at);
+    const int ctas = std::min(sms, ws.ctas);
+    auto kern = prefill_attention_kernel<T, D, SRC>;
+    cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, G::kSmem);
+    if (e != cudaSuccess) return e;
+    if ((e = launch_pdl(kern, dim3((unsigned)ctas), dim3(kPrefillThreads), G::kSmem, st, tq, tk, tv, p)) != cudaSuccess) return e;
+    return launch_pdl(prefill_join_kernel<T, D, G::kRowTiles>, dim3((unsigned)ctas, G::kSlotRows / kJoinRows), dim3(256), 0, st, p, ctas);
+}
+
+template <typename T, Source SRC>
+cudaError_t launch_source(const PrefillLaunch &a, const PrefillWorkspace &ws, int sms, cudaStream_t st) {
+    switch (a.head_dim) {
+        case 64: return launch_tiles<T, 64, SRC>(a, ws, sms, st);
+        case 128: return launch_tiles<T, 128, SRC>(a, ws, sms, st);
+        case 256: return launch_tiles<T, 256, SRC>(a, ws, sms, st);
+        default: return cudaErrorInvalidValue;
+    }
+}
+
+template <typename T>
+cudaError_t launch_type(const PrefillLaunch &a, DType kv, const PrefillWorkspace &ws, int sms, cudaStream_t st) {
+    if (!a.tables) return launch_source<T, kRows>(a, ws, sms, st);
+    return kv == DType::FP8_E4M3 ? launch_source<T, kPagedFp8>(a, ws, sms, st) : launch_source<T, kPaged>(a, ws, sms, st);
 }
 
 }  // namespace
 
-cudaError_t launch_prefill_attention(const PrefillLaunch &a, DType query, DType kv, int sms, cudaStream_t st) {
-    if (a.num_seqs <= 0) return cudaSuccess;
-    const bool fp8 = kv == DType::FP8_E4M3;
-    if (query == DType::BF16)
-        return fp8 ? launch_simple<__nv_bfloat16, uint8_t>(a, sms, st) : launch_simple<__nv_bfloat16, __nv_bfloat16>(a, sms, st);
-    if (query == DType::F16)
-        return fp8 ? launch_simple<__half, uint8_t>(a, sms, st) : launch_simple<__half, __half>(a, sms, st);
+size_t prefill_workspace_bytes(int head_dim, int ctas) {
+    const size_t rows = head_dim == 256 ? 128 : 256;
+    return (size_t)2 * ctas * (rows * (head_dim * sizeof(float) + sizeof(float2)) + sizeof(Header));
+}
+
+cudaError_t launch_prefill_attention(const PrefillLaunch &a, DType query, DType kv, const PrefillWorkspace &ws, int sms,
+                                     cudaStream_t st) {
+    if (a.num_seqs <= 0 || a.num_tokens <= 0) return cudaSuccess;
+    if (ws.ctas > 512) return cudaErrorInvalidValue;
+    if (query == DType::BF16) return launch_type<__nv_bfloat16>(a, kv, ws, sms, st);
+    if (query == DType::F16) return launch_type<__half>(a, kv, ws, sms, st);
     return cudaErrorInvalidValue;
 }
 
