@@ -74,6 +74,9 @@ static_assert(2 * (kSoftmaxRegs + kOtherRegs) * 128 <= 128 * kPrefillThreads, "r
 // than this (base 2): weights stay below 2^8, sums and products keep their
 // relative precision, and most tiles skip the rescale of O.
 constexpr float kLazy = 8.0f;
+// One pair of weights in this many is computed on the FMA units, the others by
+// the special-function unit, whose rate (16 a clock) bounds the softmax.
+constexpr int kPolyEvery = 4;
 
 enum Source { kPaged = 0, kPagedFp8 = 1, kRows = 2 };
 
@@ -366,14 +369,14 @@ prefill_attention_kernel(const __grid_constant__ CUtensorMap tq, const __grid_co
         const int w = warp >> 2, row = tid & 127;
         const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
         const int group = a.group, tau = row / group, hq = row - tau * group;
-        unsigned s_ph[2] = {0, 0}, of_ph[2] = {0, 0}, pv_n = 0, pair_n = 0;
+        unsigned s_ph = 0, of_ph[2] = {0, 0}, pv_n = 0, pair_n = 0;  // s_ph: a parity bit per S buffer
         unsigned kt = 0;  // key tiles of earlier items
         bool ok = true;
         for (; ok; ++item_n) {
             const unsigned ring = item_n % kItemRing;
             ok = wait(&item_full[ring], (item_n / kItemRing) & 1);
             if (!__all_sync(0xffffffffu, ok)) break;
-            const Item it = s_item[ring];
+            const Item &it = s_item[ring];
             if (it.end) break;
             const int n = it.t1 - it.t0;
             const bool two = NT == 2 && it.two, keys = NT == 2 && !it.two;
@@ -396,33 +399,46 @@ prefill_attention_kernel(const __grid_constant__ CUtensorMap tq, const __grid_co
                 const int t = it.t0 + (keys ? 2 * j + w : j);
                 const int buf = NT == 1 ? j & 1 : w;
                 const uint32_t s_addr = tmem + lanes + buf * G::kSCols;
-                ok = wait(&s_full[buf], s_ph[buf] & 1);
+                ok = wait(&s_full[buf], (s_ph >> buf) & 1);
                 if (!__all_sync(0xffffffffu, ok)) break;
-                ++s_ph[buf];
+                s_ph ^= 1u << buf;
                 fence_after();
                 if (warp_live) {
-                    uint32_t sr[KEYS];
-#pragma unroll
-                    for (int c = 0; c < KEYS / 32; ++c) tmem_ld32(s_addr + c * 32, sr + c * 32);
-                    wait_ld();
-                    float *s = reinterpret_cast<float *>(sr);
-                    const unsigned blocks = SRC == kRows ? 0xffu : s_mask[(kt + t - it.t0) % kMaskRing];
+                    const unsigned blocks = SRC == kRows ? ~0u : s_mask[(kt + t - it.t0) % kMaskRing];
                     constexpr unsigned kAll = (1u << G::kGranules) - 1;
-                    if (t >= careful || (SRC != kRows && (blocks & kAll) != kAll)) {
-                        const int lim = limit - t * KEYS;
+                    const bool masked = t >= careful || (SRC != kRows && (blocks & kAll) != kAll);
+                    const int lim = limit - t * KEYS;
+                    // The scores are read twice, 32 at a time, rather than held:
+                    // 128 of them beside the rest do not fit the registers.
+                    constexpr int kChunks = KEYS / 32;
+                    uint32_t ra[32], rb[32];
+                    auto hide = [&](float *x, int c) {
 #pragma unroll
-                        for (int i = 0; i < KEYS; ++i)
-                            if (i >= lim || !((blocks >> (i / 16)) & 1u)) s[i] = -INFINITY;
+                        for (int i = 0; i < 32; ++i)
+                            if (c * 32 + i >= lim || !((blocks >> (c * 2 + i / 16)) & 1u)) x[i] = -INFINITY;
+                    };
+                    // The row's maximum; NaN among the scores makes it NaN, and with it
+                    // the row. (An infinite one gives NaN weights too.)
+                    float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+                    tmem_ld32(s_addr, ra);
+#pragma unroll
+                    for (int c = 0; c < kChunks; ++c) {
+                        uint32_t *cur = c & 1 ? rb : ra, *nxt = c & 1 ? ra : rb;
+                        wait_ld32(cur);
+                        if (c + 1 < kChunks) tmem_ld32(s_addr + (c + 1) * 32, nxt);
+                        float *x = reinterpret_cast<float *>(cur);
+                        if (masked) hide(x, c);
+#pragma unroll
+                        for (int i = 0; i < 32; i += 8)
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) mx[e] = max3(mx[e], x[i + e], x[i + 4 + e]);
                     }
-                    float mx[4] = {s[0], s[1], s[2], s[3]};
-#pragma unroll
-                    for (int i = 4; i < KEYS; i += 4)
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) mx[e] = fmaxf(mx[e], s[i + e]);
-                    const float mt = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * scale;
-                    const bool grew = mt > m + kLazy || (m == -INFINITY && mt > m);
+                    tmem_ld32(s_addr, ra);
+                    const float mt = max3(max_nan(mx[0], mx[1]), mx[2], mx[3]) * scale;
+                    const bool grew = !(mt <= m + kLazy);
                     if (__any_sync(0xffffffffu, grew)) {
-                        const float mn = fmaxf(m, mt);
+                        float mn = max_nan(m, mt);
+                        if (mn == INFINITY) mn = NAN;
                         const float corr = m == -INFINITY ? 0.f : ex2(m - mn);
                         l *= corr;
                         m = mn;
@@ -440,7 +456,7 @@ prefill_attention_kernel(const __grid_constant__ CUtensorMap tq, const __grid_co
                             for (int c = 0; c < D / 32; ++c) {
                                 uint32_t o[32];
                                 tmem_ld32(o_addr + c * 32, o);
-                                wait_ld();
+                                wait_ld32(o);
 #pragma unroll
                                 for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * corr);
                                 tmem_st32(o_addr + c * 32, o);
@@ -450,20 +466,38 @@ prefill_attention_kernel(const __grid_constant__ CUtensorMap tq, const __grid_co
                     const float ref = m == -INFINITY ? 0.f : m;  // nothing yet: weights 2^-inf = 0
                     const uint64_t sc2 = pair(scale, scale), mr2 = pair(-ref, -ref);
                     uint64_t sum[2] = {pair(l, 0.f), pair(0.f, 0.f)};
+                    // Masked tiles take every weight from the special-function
+                    // unit: a hidden key's is 0 there, and 2^-125 from the polynomial.
+                    auto weights = [&](auto with_mask) {
+                        constexpr bool MASKED = decltype(with_mask)::value;
 #pragma unroll
-                    for (int c = 0; c < KEYS / 64; ++c) {
-                        uint32_t pk[32];
+                        for (int c = 0; c < kChunks; ++c) {
+                            uint32_t *cur = c & 1 ? rb : ra, *nxt = c & 1 ? ra : rb;
+                            wait_ld32(cur);
+                            if (c + 1 < kChunks) tmem_ld32(s_addr + (c + 1) * 32, nxt);
+                            float *s = reinterpret_cast<float *>(cur);
+                            if (MASKED) hide(s, c);
+                            uint32_t pk[16];
 #pragma unroll
-                        for (int i = 0; i < 32; ++i) {
-                            float x, y;
-                            unpair(fma2(pair(s[c * 64 + 2 * i], s[c * 64 + 2 * i + 1]), sc2, mr2), x, y);
-                            x = ex2(x);
-                            y = ex2(y);
-                            sum[i & 1] = add2(sum[i & 1], pair(x, y));
-                            pk[i] = pack2<T>(x, y);
+                            for (int i = 0; i < 16; ++i) {
+                                float x, y;
+                                const uint64_t xy = fma2(pair(s[2 * i], s[2 * i + 1]), sc2, mr2);
+                                if (!MASKED && i % kPolyEvery == kPolyEvery - 1) {
+                                    ex2_poly(xy, x, y);
+                                } else {
+                                    unpair(xy, x, y);
+                                    x = ex2(x);
+                                    y = ex2(y);
+                                }
+                                sum[i & 1] = add2(sum[i & 1], pair(x, y));
+                                pk[i] = pack2<T>(x, y);
+                            }
+                            // Over scores that this row has read already.
+                            tmem_st16(s_addr + c * 16, pk);
                         }
-                        tmem_st32(s_addr + c * 32, pk);
-                    }
+                    };
+                    if (masked) weights(std::true_type{});
+                    else weights(std::false_type{});
                     float u, v;
                     unpair(add2(sum[0], sum[1]), u, v);
                     l = u + v;
@@ -536,7 +570,7 @@ prefill_attention_kernel(const __grid_constant__ CUtensorMap tq, const __grid_co
                         if (!use[h]) continue;
                         uint32_t r[32];
                         tmem_ld32(tmem + lanes + G::kOCol + h * D + c, r);
-                        wait_ld();
+                        wait_ld32(r);
 #pragma unroll
                         for (int i = 0; i < 32; ++i) o[i] = fmaf(__uint_as_float(r[i]), f[h], o[i]);
                     }
@@ -614,26 +648,29 @@ prefill_attention_kernel(const __grid_constant__ CUtensorMap tq, const __grid_co
         }
     } else if (warp == 8) {
         // ================= the products =================
-        if (lane == 0) {
+        if (elect_one()) {
             constexpr uint32_t id_s = instr_desc<T>(128, KEYS, false), id_o = instr_desc<T>(128, D, true);
             const uint32_t q0 = smem_u32(sq), kv0 = smem_u32(skv);
             unsigned pos = 0, p_ph[2] = {0, 0}, ou[2] = {0, 0}, qn = 0;
             bool ok = true;
             auto stage = [&](unsigned at) { return at % ST; };
             auto full = [&](unsigned at) { return wait(&kv_full[at % ST], (at / ST) & 1); };
+            // Descriptors of the first tiles; an address moves the low word by
+            // its 16-byte units (shared addresses fit its 14 bits).
+            const uint64_t dq = smem_desc(q0, 16, 1024), dk = smem_desc(kv0, 16, 1024), dv = smem_desc(kv0, G::kSlab, 1024);
             auto scores = [&](int qt, int buf, unsigned at) {
-                const uint32_t kb = kv0 + stage(at) * G::kTile, qb = q0 + qt * G::kQTile;
+                const uint64_t qd = dq + qt * (G::kQTile / 16), kd = dk + stage(at) * (G::kTile / 16);
 #pragma unroll
                 for (int k = 0; k < D / 16; ++k)
-                    mma_ss(tmem + buf * G::kSCols, smem_desc(qb + (k / 4) * (128 * 128) + (k % 4) * 32, 16, 1024),
-                           smem_desc(kb + (k / 4) * G::kSlab + (k % 4) * 32, 16, 1024), id_s, k > 0);
+                    mma_ss(tmem + buf * G::kSCols, qd + (k / 4) * (128 * 128 / 16) + (k % 4) * 2,
+                           kd + (k / 4) * (G::kSlab / 16) + (k % 4) * 2, id_s, k > 0);
             };
             auto values = [&](int buf, int ob, unsigned at, bool accumulate) {
-                const uint32_t vb = kv0 + stage(at) * G::kTile;
+                const uint64_t vd = dv + stage(at) * (G::kTile / 16);
 #pragma unroll
                 for (int k = 0; k < KEYS / 16; ++k)
-                    mma_ts(tmem + G::kOCol + ob * D, tmem + buf * G::kSCols + k * 8,
-                           smem_desc(vb + k * 2048, G::kSlab, 1024), id_o, accumulate || k > 0);
+                    mma_ts(tmem + G::kOCol + ob * D, tmem + buf * G::kSCols + k * 8, vd + k * (2048 / 16), id_o,
+                           accumulate || k > 0);
             };
             auto o_ready = [&](int ob) { return ou[ob] == 0 || wait(&o_free[ob], (ou[ob] - 1) & 1); };
             for (; ok; ++item_n) {

@@ -17,6 +17,17 @@ __device__ __forceinline__ uint32_t smem_u32(const void *p) {
     return static_cast<uint32_t>(__cvta_generic_to_shared(p));
 }
 
+// True in one lane of a converged warp. The single-thread roles run under it
+// rather than under lane == 0: the operands of tcgen05.mma and of TMA sit in
+// uniform registers, and code that is known to run in one lane fills them
+// without a loop over lanes (measured: a 128 x 128 x 16 product went from
+// about 300 cycles to its 64).
+__device__ __forceinline__ bool elect_one() {
+    uint32_t p;
+    asm volatile("{\n\t.reg .pred q;\n\telect.sync _|q, 0xffffffff;\n\tselp.u32 %0, 1, 0, q;\n\t}" : "=r"(p));
+    return p != 0;
+}
+
 // ---- mbarriers ---------------------------------------------------------------
 
 __device__ __forceinline__ void mbar_init(uint64_t *bar, uint32_t count) {
@@ -81,7 +92,6 @@ __device__ __forceinline__ void tmem_free(uint32_t base, uint32_t columns) {
 }
 __device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
-__device__ __forceinline__ void wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
 // 32 columns of the warp's 32 lanes: a thread gets its lane's row.
@@ -95,6 +105,20 @@ __device__ __forceinline__ void tmem_ld32(uint32_t addr, uint32_t *r) {
           "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
           "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
         : "r"(addr));
+}
+// Waits for the thread's loads; the registers pass through, so that no use of
+// them is moved ahead of it.
+__device__ __forceinline__ void wait_ld32(uint32_t *r) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]), "+r"(r[16]), "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]), "+r"(r[22]), "+r"(r[23]), "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29]), "+r"(r[30]), "+r"(r[31])
+                 :
+                 : "memory");
+}
+__device__ __forceinline__ void tmem_st16(uint32_t addr, const uint32_t *r) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], "
+        "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15};" ::"r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(addr)
+        : "memory");
 }
 __device__ __forceinline__ void tmem_st32(uint32_t addr, const uint32_t *r) {
     asm volatile(
@@ -172,6 +196,18 @@ __device__ __forceinline__ float ex2(float x) {
     return y;
 }
 
+// The largest of three, NaN if one is.
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
+}
+__device__ __forceinline__ float max_nan(float a, float b) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
+}
+
 // Two f32 values as a packed pair of T, `lo` in the low half.
 template <typename T>
 __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
@@ -207,6 +243,30 @@ __device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
     uint64_t r;
     asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
     return r;
+}
+
+// 2^x of a pair on the FMA units, for x <= 2^6 (below -125: about 2^-125): x =
+// n + f with n the nearest integer and |f| <= 1/2; 2^f by a polynomial of
+// degree 4, the minimax fit of its relative error on that interval (Remez
+// exchange; 2.7e-6 with f32 arithmetic), and n into the exponent.
+__device__ __forceinline__ void ex2_poly(uint64_t x2, float &a, float &b) {
+    float x, y;
+    unpair(x2, x, y);
+    x2 = pair(fmaxf(x, -125.f), fmaxf(y, -125.f));
+    const float shift = 12582912.f;  // 1.5 * 2^23: its sum's low bits are n
+    const uint64_t t = add2(x2, pair(shift, shift));
+    const uint64_t n = add2(t, pair(-shift, -shift));
+    const uint64_t f = fma2(n, pair(-1.f, -1.f), x2);
+    uint64_t r = pair(0x1.3997d6p-7f, 0x1.3997d6p-7f);
+    r = fma2(r, f, pair(0x1.ca1444p-5f, 0x1.ca1444p-5f));
+    r = fma2(r, f, pair(0x1.ec06dap-3f, 0x1.ec06dap-3f));
+    r = fma2(r, f, pair(0x1.62e0dcp-1f, 0x1.62e0dcp-1f));
+    r = fma2(r, f, pair(0x1.ffffe8p-1f, 0x1.ffffe8p-1f));
+    float tx, ty;
+    unpair(t, tx, ty);
+    unpair(r, a, b);
+    a = __int_as_float((__float_as_int(tx) << 23) + __float_as_int(a));
+    b = __int_as_float((__float_as_int(ty) << 23) + __float_as_int(b));
 }
 
 }  // namespace tc
