@@ -64,7 +64,8 @@ constexpr int kDeviceCode = 9;                            // PKV_ERR_DEVICE
 constexpr long long kWaitCycles = 4000000000ll;           // about 2 s
 constexpr int kPrefillThreads = 512;
 constexpr int kItemRing = 4;
-constexpr int kMaskRing = 32;
+constexpr int kMaskRing = 32;                             // key tiles whose block masks are kept
+constexpr int kRowRing = 4;                               // and whose pool rows (K runs 2 tiles before V)
 constexpr int kFlagWords = 12;                            // 3 key tiles of 128 bits
 // Registers a thread after the split of the launch's 128 x 512: softmax
 // threads hold a row of 128 scores, the others a few addresses.
@@ -244,12 +245,12 @@ prefill_attention_kernel(const __grid_constant__ CUtensorMap tq, const __grid_co
     constexpr int NT = G::kRowTiles, KEYS = G::kKeys, ST = G::kStages, RS = G::kRawStages ? G::kRawStages : 1;
     extern __shared__ __align__(1024) unsigned char smem[];
     __shared__ __align__(8) uint64_t kv_full[ST], kv_empty[ST], raw_full[RS], raw_empty[RS], by_hand_go[ST];
-    __shared__ __align__(8) uint64_t s_full[2], p_full[2], o_full[2], o_free[2], pv_done, pair_bar, q_full, q_empty, drain;
+    __shared__ __align__(8) uint64_t s_full[2], p_half[2], p_full[2], o_full[2], o_free[2], pv_done, pair_bar, q_full, q_empty, drain;
     __shared__ __align__(8) uint64_t item_full[kItemRing], item_empty[kItemRing];
     __shared__ Item s_item[kItemRing];
     __shared__ unsigned s_flag[kItemRing][kFlagWords + 1];
     __shared__ unsigned char s_mask[kMaskRing];
-    __shared__ long long s_scan[kPrefillThreads / 32];
+    __shared__ int s_row[kRowRing][8];
     __shared__ Pos s_range[2];
     __shared__ uint32_t s_tmem;
     __shared__ volatile int s_failed;
@@ -258,6 +259,7 @@ prefill_attention_kernel(const __grid_constant__ CUtensorMap tq, const __grid_co
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     unsigned char *sq = smem, *skv = smem + NT * G::kQTile, *sraw = skv + ST * G::kTile;
     float2 *stat = reinterpret_cast<float2 *>(sraw + G::kRawStages * G::kRawTile);
+    long long *s_scan = reinterpret_cast<long long *>(stat);  // while the share is found
 
     if (smem_u32(smem) & 1023u) {  // the swizzle's atoms would not line up
         if (tid == 0) record_error(a.err, kDeviceCode, blockIdx.x);
@@ -268,7 +270,7 @@ prefill_attention_kernel(const __grid_constant__ CUtensorMap tq, const __grid_co
         for (int i = 0; i < ST; ++i) mbar_init(&kv_full[i], 1), mbar_init(&kv_empty[i], 1), mbar_init(&by_hand_go[i], 1);
         for (int i = 0; i < RS; ++i) mbar_init(&raw_full[i], 1), mbar_init(&raw_empty[i], 1);
         for (int i = 0; i < 2; ++i)
-            mbar_init(&s_full[i], 1), mbar_init(&p_full[i], 128), mbar_init(&o_full[i], 1), mbar_init(&o_free[i], 128);
+            mbar_init(&s_full[i], 1), mbar_init(&p_half[i], 128), mbar_init(&p_full[i], 128), mbar_init(&o_full[i], 1), mbar_init(&o_free[i], 128);
         mbar_init(&pv_done, 1), mbar_init(&pair_bar, 256), mbar_init(&q_full, 1), mbar_init(&q_empty, 1), mbar_init(&drain, 1);
         for (int i = 0; i < kItemRing; ++i) mbar_init(&item_full[i], 1), mbar_init(&item_empty[i], 6 + 4 * NT);
         fence_barrier_init();
@@ -408,32 +410,28 @@ prefill_attention_kernel(const __grid_constant__ CUtensorMap tq, const __grid_co
                     constexpr unsigned kAll = (1u << G::kGranules) - 1;
                     const bool masked = t >= careful || (SRC != kRows && (blocks & kAll) != kAll);
                     const int lim = limit - t * KEYS;
-                    // The scores are read twice, 32 at a time, rather than held:
-                    // 128 of them beside the rest do not fit the registers.
                     constexpr int kChunks = KEYS / 32;
-                    uint32_t ra[32], rb[32];
+                    uint32_t sr[kChunks][32];
                     auto hide = [&](float *x, int c) {
 #pragma unroll
                         for (int i = 0; i < 32; ++i)
                             if (c * 32 + i >= lim || !((blocks >> (c * 2 + i / 16)) & 1u)) x[i] = -INFINITY;
                     };
+#pragma unroll
+                    for (int c = 0; c < kChunks; ++c) tmem_ld32(s_addr + c * 32, sr[c]);
                     // The row's maximum; NaN among the scores makes it NaN, and with it
                     // the row. (An infinite one gives NaN weights too.)
                     float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-                    tmem_ld32(s_addr, ra);
 #pragma unroll
                     for (int c = 0; c < kChunks; ++c) {
-                        uint32_t *cur = c & 1 ? rb : ra, *nxt = c & 1 ? ra : rb;
-                        wait_ld32(cur);
-                        if (c + 1 < kChunks) tmem_ld32(s_addr + (c + 1) * 32, nxt);
-                        float *x = reinterpret_cast<float *>(cur);
+                        wait_ld32(sr[c]);
+                        float *x = reinterpret_cast<float *>(sr[c]);
                         if (masked) hide(x, c);
 #pragma unroll
                         for (int i = 0; i < 32; i += 8)
 #pragma unroll
                             for (int e = 0; e < 4; ++e) mx[e] = max3(mx[e], x[i + e], x[i + 4 + e]);
                     }
-                    tmem_ld32(s_addr, ra);
                     const float mt = max3(max_nan(mx[0], mx[1]), mx[2], mx[3]) * scale;
                     const bool grew = !(mt <= m + kLazy);
                     if (__any_sync(0xffffffffu, grew)) {
@@ -453,13 +451,13 @@ prefill_attention_kernel(const __grid_constant__ CUtensorMap tq, const __grid_co
                             }
                             const uint32_t o_addr = tmem + lanes + G::kOCol + (NT == 2 ? w * D : 0);
 #pragma unroll
-                            for (int c = 0; c < D / 32; ++c) {
-                                uint32_t o[32];
-                                tmem_ld32(o_addr + c * 32, o);
-                                wait_ld32(o);
+                            for (int c = 0; c < D / 16; ++c) {
+                                uint32_t o[16];
+                                tmem_ld16(o_addr + c * 16, o);
+                                wait_ld16(o);
 #pragma unroll
-                                for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * corr);
-                                tmem_st32(o_addr + c * 32, o);
+                                for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * corr);
+                                tmem_st16(o_addr + c * 16, o);
                             }
                         }
                     }
@@ -472,11 +470,7 @@ prefill_attention_kernel(const __grid_constant__ CUtensorMap tq, const __grid_co
                         constexpr bool MASKED = decltype(with_mask)::value;
 #pragma unroll
                         for (int c = 0; c < kChunks; ++c) {
-                            uint32_t *cur = c & 1 ? rb : ra, *nxt = c & 1 ? ra : rb;
-                            wait_ld32(cur);
-                            if (c + 1 < kChunks) tmem_ld32(s_addr + (c + 1) * 32, nxt);
-                            float *s = reinterpret_cast<float *>(cur);
-                            if (MASKED) hide(s, c);
+                            const float *s = reinterpret_cast<const float *>(sr[c]);
                             uint32_t pk[16];
 #pragma unroll
                             for (int i = 0; i < 16; ++i) {
@@ -494,6 +488,11 @@ prefill_attention_kernel(const __grid_constant__ CUtensorMap tq, const __grid_co
                             }
                             // Over scores that this row has read already.
                             tmem_st16(s_addr + c * 16, pk);
+                            if (c == kChunks / 2 - 1) {  // the first half's product may begin
+                                wait_st();
+                                fence_before();
+                                mbar_arrive(&p_half[buf]);
+                            }
                         }
                     };
                     if (masked) weights(std::true_type{});
@@ -504,6 +503,7 @@ prefill_attention_kernel(const __grid_constant__ CUtensorMap tq, const __grid_co
                     wait_st();
                 }
                 fence_before();
+                if (!warp_live) mbar_arrive(&p_half[buf]);
                 mbar_arrive(&p_full[buf]);
             }
             if (!__all_sync(0xffffffffu, ok)) break;
@@ -665,12 +665,16 @@ prefill_attention_kernel(const __grid_constant__ CUtensorMap tq, const __grid_co
                     mma_ss(tmem + buf * G::kSCols, qd + (k / 4) * (128 * 128 / 16) + (k % 4) * 2,
                            kd + (k / 4) * (G::kSlab / 16) + (k % 4) * 2, id_s, k > 0);
             };
-            auto values = [&](int buf, int ob, unsigned at, bool accumulate) {
+            // The product of one half of the tile's keys (a row's weights of the
+            // first half are there while those of the second are computed).
+            auto values = [&](int half, int buf, int ob, unsigned at, bool accumulate) {
                 const uint64_t vd = dv + stage(at) * (G::kTile / 16);
 #pragma unroll
-                for (int k = 0; k < KEYS / 16; ++k)
+                for (int k0 = 0; k0 < KEYS / 32; ++k0) {
+                    const int k = half * (KEYS / 32) + k0;
                     mma_ts(tmem + G::kOCol + ob * D, tmem + buf * G::kSCols + k * 8, vd + k * (2048 / 16), id_o,
                            accumulate || k > 0);
+                }
             };
             auto o_ready = [&](int ob) { return ou[ob] == 0 || wait(&o_free[ob], (ou[ob] - 1) & 1); };
             for (; ok; ++item_n) {
@@ -697,10 +701,13 @@ prefill_attention_kernel(const __grid_constant__ CUtensorMap tq, const __grid_co
                         const unsigned va = pos + v_at(j, n, ahead_rows), ka = pos + k_at(j + 1, ahead_rows);
                         if (!(ok = full(va))) break;
                         if (j < n0) {
-                            if (!(ok = wait(&p_full[0], p_ph[0]++ & 1))) break;
+                            if (!(ok = wait(&p_half[0], p_ph[0] & 1))) break;
                             if (j == 0 && !(ok = o_ready(0))) break;
                             fence_after();
-                            values(0, 0, va, j > 0);
+                            values(0, 0, 0, va, j > 0);
+                            if (!(ok = wait(&p_full[0], p_ph[0]++ & 1))) break;
+                            fence_after();
+                            values(1, 0, 0, va, true);
                             if (j + 1 == n0) commit(&o_full[0]), ++ou[0];
                         }
                         if (j + 1 < n) {
@@ -708,10 +715,13 @@ prefill_attention_kernel(const __grid_constant__ CUtensorMap tq, const __grid_co
                             fence_after();
                             if (j + 1 < n0) scores(0, 0, ka), commit(&s_full[0]);
                         }
-                        if (!(ok = wait(&p_full[1], p_ph[1]++ & 1))) break;
+                        if (!(ok = wait(&p_half[1], p_ph[1] & 1))) break;
                         if (j == 0 && !(ok = o_ready(1))) break;
                         fence_after();
-                        values(1, 1, va, j > 0);
+                        values(0, 1, 1, va, j > 0);
+                        if (!(ok = wait(&p_full[1], p_ph[1]++ & 1))) break;
+                        fence_after();
+                        values(1, 1, 1, va, true);
                         commit(&kv_empty[stage(va)]);
                         if (j + 1 < n) {
                             scores(1, 1, ka);
@@ -738,10 +748,13 @@ prefill_attention_kernel(const __grid_constant__ CUtensorMap tq, const __grid_co
                         const bool first = NT == 2 ? j < 2 : j == 0;
                         const unsigned va = pos + v_at(j, n, ahead_keys), ka = pos + k_at(j + 2, ahead_keys);
                         if (!(ok = full(va))) break;
-                        if (!(ok = wait(&p_full[buf], p_ph[buf]++ & 1))) break;
+                        if (!(ok = wait(&p_half[buf], p_ph[buf] & 1))) break;
                         if (first && !(ok = o_ready(ob))) break;
                         fence_after();
-                        values(buf, ob, va, !first);
+                        values(0, buf, ob, va, !first);
+                        if (!(ok = wait(&p_full[buf], p_ph[buf]++ & 1))) break;
+                        fence_after();
+                        values(1, buf, ob, va, true);
                         commit(&kv_empty[stage(va)]);
                         if (NT == 1) commit(&pv_done);
                         if (j + 2 < n) {
@@ -777,6 +790,12 @@ prefill_attention_kernel(const __grid_constant__ CUtensorMap tq, const __grid_co
             if (it.end) break;
             const int n = it.t1 - it.t0, ahead = NT == 2 && it.two ? ahead_rows : ahead_keys;
             const int careful = first_careful(it), len = it.key0 + it.tokens;
+            auto block_of = [&](int t) {  // of this lane's granule of key tile t
+                const int key = t * KEYS + lane * 16;
+                if (SRC == kRows || lane >= G::kGranules || t >= it.t1 || key >= len) return -1;
+                return __ldg(a.tables + (long long)it.seq * a.table_stride + key / a.block_size);
+            };
+            int next_blk = block_of(it.t0);
             for (int f = 0; f < 2 * n; ++f) {
                 // Fill f of the item: K 0 .. ahead - 1, then V j and K j + ahead in turn.
                 bool is_k;
@@ -788,7 +807,7 @@ prefill_attention_kernel(const __grid_constant__ CUtensorMap tq, const __grid_co
                 const int t = it.t0 + j;
                 const unsigned at = pos + f;
                 if constexpr (SRC == kRows) {
-                    if (lane == 0) {
+                    if (elect_one()) {
                         ok = wait(&kv_empty[at % ST], ((at / ST) & 1) ^ 1);
                         if (ok && !is_k && t >= careful) {
                             mbar_arrive(&by_hand_go[at % ST]);
@@ -800,22 +819,29 @@ prefill_attention_kernel(const __grid_constant__ CUtensorMap tq, const __grid_co
                                             it.head * D + c * 64, it.base + t * KEYS, &kv_full[at % ST]);
                         }
                     }
-                    ok = __shfl_sync(0xffffffffu, ok, 0);
+                    ok = __all_sync(0xffffffffu, ok);
                     if (!ok) break;
                 } else {
                     const bool by_hand = SRC == kPaged && !is_k && t >= careful;
-                    // Lane g brings the tile's 16-key granule g.
-                    const int key = t * KEYS + lane * 16;
-                    const bool have = lane < G::kGranules && key < len;
-                    int blk = -1;
-                    if (have && !by_hand) blk = __ldg(a.tables + (long long)it.seq * a.table_stride + key / a.block_size);
-                    const bool good = have && blk >= 0 && blk < a.num_blocks;
-                    if (have && !good && !by_hand) record_error(a.err, kInvalidBlock, it.seq);
-                    const unsigned bits = __ballot_sync(0xffffffffu, good || (lane < G::kGranules && !have));
-                    const unsigned loads = __ballot_sync(0xffffffffu, good);
                     uint64_t *full = SRC == kPagedFp8 ? &raw_full[at % RS] : &kv_full[at % ST];
                     uint64_t *empty = SRC == kPagedFp8 ? &raw_empty[at % RS] : &kv_empty[at % ST];
                     const unsigned turn = SRC == kPagedFp8 ? at / RS : at / ST;
+                    if (is_k) {
+                        // Lane g finds the pool row of the tile's 16-key granule g (-1:
+                        // none), kept for the tile's V; the next tile's block ids are
+                        // on their way meanwhile.
+                        const int key = t * KEYS + lane * 16;
+                        const bool have = lane < G::kGranules && key < len;
+                        const bool good = have && next_blk >= 0 && next_blk < a.num_blocks;
+                        if (have && !good) record_error(a.err, kInvalidBlock, it.seq);
+                        const unsigned bits = __ballot_sync(0xffffffffu, good || (lane < G::kGranules && !have));
+                        if (lane < G::kGranules)
+                            s_row[(kt + j) % kRowRing][lane] =
+                                good ? (int)(a.layer_row0 + (long long)next_blk * a.block_size + key % a.block_size) : -1;
+                        if (lane == 0) s_mask[(kt + j) % kMaskRing] = (unsigned char)bits;
+                        next_blk = block_of(t + 1);
+                        __syncwarp();
+                    }
                     ok = wait(empty, (turn & 1) ^ 1);
                     ok = __all_sync(0xffffffffu, ok);
                     if (!ok) break;
@@ -823,36 +849,37 @@ prefill_attention_kernel(const __grid_constant__ CUtensorMap tq, const __grid_co
                         if (lane == 0) mbar_arrive(&by_hand_go[at % ST]);
                         continue;
                     }
-                    if (is_k && lane == 0) s_mask[(kt + j) % kMaskRing] = (unsigned char)bits;
-                    const int y = (int)(a.layer_row0 + (long long)blk * a.block_size + key % a.block_size);
-                    if constexpr (SRC == kPagedFp8) {
-                        __syncwarp();
-                        if (lane == 0) mbar_expect_tx(full, __popc(loads) * 16 * D);
-                        __syncwarp();
-                        if (good)
-                            tma_load_2d(raw0 + (at % RS) * G::kRawTile + lane * 16 * D, is_k ? &tk : &tv, it.head * D, y, full);
-                    } else {
-                        unsigned char *dst = skv + (at % ST) * G::kTile;
-                        if (!is_k && loads != (1u << G::kGranules) - 1) {
-                            // A block outside the pool: its values are zeros.
-                            for (int g = 0; g < G::kGranules; ++g) {
-                                if ((loads >> g) & 1u) continue;
-                                for (int i = lane; i < G::kSlabs * 128; i += 32)
-                                    *reinterpret_cast<uint4 *>(dst + (i >> 7) * G::kSlab + g * 2048 + (i & 127) * 16) =
-                                        make_uint4(0, 0, 0, 0);
-                            }
-                            fence_async();
+                    const int *rows = s_row[(kt + j) % kRowRing];
+                    const unsigned loads = __ballot_sync(0xffffffffu, lane < G::kGranules && rows[lane & (G::kGranules - 1)] >= 0);
+                    unsigned char *dst = skv + (at % ST) * G::kTile;
+                    if (SRC == kPaged && !is_k && loads != (1u << G::kGranules) - 1) {
+                        // A block outside the pool: its values are zeros.
+                        for (int g = 0; g < G::kGranules; ++g) {
+                            if ((loads >> g) & 1u) continue;
+                            for (int i = lane; i < G::kSlabs * 128; i += 32)
+                                *reinterpret_cast<uint4 *>(dst + (i >> 7) * G::kSlab + g * 2048 + (i & 127) * 16) =
+                                    make_uint4(0, 0, 0, 0);
                         }
+                        fence_async();
                         __syncwarp();
-                        if (lane == 0) mbar_expect_tx(full, __popc(loads) * 16 * D * 2);
-                        __syncwarp();
-                        if (good) {
+                    }
+                    if (elect_one()) {
+                        const CUtensorMap *map = is_k ? &tk : &tv;
+                        mbar_expect_tx(full, __popc(loads) * (SRC == kPagedFp8 ? 16 * D : 16 * D * 2));
 #pragma unroll
-                            for (int c = 0; c < G::kSlabs; ++c)
-                                tma_load_2d(smem_u32(dst) + c * G::kSlab + lane * 2048, is_k ? &tk : &tv,
-                                            it.head * D + c * 64, y, full);
+                        for (int g = 0; g < G::kGranules; ++g) {
+                            const int y = rows[g];
+                            if (y < 0) continue;
+                            if constexpr (SRC == kPagedFp8) {
+                                tma_load_2d(raw0 + (at % RS) * G::kRawTile + g * 16 * D, map, it.head * D, y, full);
+                            } else {
+#pragma unroll
+                                for (int c = 0; c < G::kSlabs; ++c)
+                                    tma_load_2d(smem_u32(dst) + c * G::kSlab + g * 2048, map, it.head * D + c * 64, y, full);
+                            }
                         }
                     }
+                    __syncwarp();
                 }
             }
             pos += 2 * n;
@@ -920,7 +947,7 @@ prefill_attention_kernel(const __grid_constant__ CUtensorMap tq, const __grid_co
                     it.slot = it.t0 > 0 ? 2 * (int)blockIdx.x : it.t1 < it.tiles ? 2 * (int)blockIdx.x + 1 : -1;
                     if (!(ok = publish(it))) break;
                     if (it.t1 > it.t0) {
-                        if (lane == 0) {
+                        if (elect_one()) {
                             if (qn > 0) ok = wait(&q_empty, (qn - 1) & 1);
                             if (ok) {
                                 const int tiles = it.two ? 2 : 1;
@@ -933,7 +960,7 @@ prefill_attention_kernel(const __grid_constant__ CUtensorMap tq, const __grid_co
                             }
                         }
                         ++qn;
-                        ok = __shfl_sync(0xffffffffu, ok, 0);
+                        ok = __all_sync(0xffffffffu, ok);
                     }
                 }
             }
