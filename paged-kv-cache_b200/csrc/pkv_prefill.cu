@@ -96,8 +96,8 @@ struct Geom {
     static constexpr int kRawTile = kKeys * D;                  // fp8: the tile's codes
     static constexpr int kRawStages = kFp8 ? (D == 64 ? 6 : 3) : 0;
     static constexpr int kGranules = kKeys / 16;
-    static constexpr int kSCols = kKeys;                        // tensor-memory columns of an S buffer
-    static constexpr int kOCol = 2 * kSCols;
+    static constexpr int kSteps = kKeys / 64;                   // 64-key steps of a tile
+    static constexpr int kOCol = kRowTiles * 128;               // after two S buffers of 64 columns a row tile
     static constexpr int kStatBytes = 2 * 128 * 8;
     static constexpr int kSmem = kRowTiles * kQTile + kStages * kTile + kRawStages * kRawTile + kStatBytes;
     static constexpr int kSlotRows = kRowTiles * 128;           // rows of a partial
@@ -245,7 +245,7 @@ prefill_attention_kernel(const __grid_constant__ CUtensorMap tq, const __grid_co
     constexpr int NT = G::kRowTiles, KEYS = G::kKeys, ST = G::kStages, RS = G::kRawStages ? G::kRawStages : 1;
     extern __shared__ __align__(1024) unsigned char smem[];
     __shared__ __align__(8) uint64_t kv_full[ST], kv_empty[ST], raw_full[RS], raw_empty[RS], by_hand_go[ST];
-    __shared__ __align__(8) uint64_t s_full[2], p_half[2], p_full[2], o_full[2], o_free[2], pv_done, pair_bar, q_full, q_empty, drain;
+    __shared__ __align__(8) uint64_t s_full[4], p_full[4], pv_done[2], o_full[2], o_free[2], pair_bar, q_full, q_empty, drain;
     __shared__ __align__(8) uint64_t item_full[kItemRing], item_empty[kItemRing];
     __shared__ Item s_item[kItemRing];
     __shared__ unsigned s_flag[kItemRing][kFlagWords + 1];
@@ -269,9 +269,9 @@ prefill_attention_kernel(const __grid_constant__ CUtensorMap tq, const __grid_co
     if (tid == 32) {
         for (int i = 0; i < ST; ++i) mbar_init(&kv_full[i], 1), mbar_init(&kv_empty[i], 1), mbar_init(&by_hand_go[i], 1);
         for (int i = 0; i < RS; ++i) mbar_init(&raw_full[i], 1), mbar_init(&raw_empty[i], 1);
-        for (int i = 0; i < 2; ++i)
-            mbar_init(&s_full[i], 1), mbar_init(&p_half[i], 128), mbar_init(&p_full[i], 128), mbar_init(&o_full[i], 1), mbar_init(&o_free[i], 128);
-        mbar_init(&pv_done, 1), mbar_init(&pair_bar, 256), mbar_init(&q_full, 1), mbar_init(&q_empty, 1), mbar_init(&drain, 1);
+        for (int i = 0; i < 4; ++i) mbar_init(&s_full[i], 1), mbar_init(&p_full[i], 128);
+        for (int i = 0; i < 2; ++i) mbar_init(&pv_done[i], 1), mbar_init(&o_full[i], 1), mbar_init(&o_free[i], 128);
+        mbar_init(&pair_bar, 256), mbar_init(&q_full, 1), mbar_init(&q_empty, 1), mbar_init(&drain, 1);
         for (int i = 0; i < kItemRing; ++i) mbar_init(&item_full[i], 1), mbar_init(&item_empty[i], 6 + 4 * NT);
         fence_barrier_init();
         s_failed = 0;
@@ -397,40 +397,40 @@ prefill_attention_kernel(const __grid_constant__ CUtensorMap tq, const __grid_co
             float m = -INFINITY, l = 0.f;
             const bool warp_live = __any_sync(0xffffffffu, live);
             const int careful = first_careful(it);
-            for (int j = 0; j < mine; ++j) {
-                const int t = it.t0 + (keys ? 2 * j + w : j);
-                const int buf = NT == 1 ? j & 1 : w;
-                const uint32_t s_addr = tmem + lanes + buf * G::kSCols;
-                ok = wait(&s_full[buf], (s_ph >> buf) & 1);
+            for (int i = 0; i < mine * G::kSteps; ++i) {
+                const int j = i / G::kSteps, t = it.t0 + (keys ? 2 * j + w : j);
+                const int buf = w * 2 + (i & 1);
+                const uint32_t s_addr = tmem + lanes + buf * 64;
+                ok = wait(&s_full[buf], (s_ph >> (i & 1)) & 1);
                 if (!__all_sync(0xffffffffu, ok)) break;
-                s_ph ^= 1u << buf;
+                s_ph ^= 1u << (i & 1);
                 fence_after();
                 if (warp_live) {
-                    const unsigned blocks = SRC == kRows ? ~0u : s_mask[(kt + t - it.t0) % kMaskRing];
-                    constexpr unsigned kAll = (1u << G::kGranules) - 1;
-                    const bool masked = t >= careful || (SRC != kRows && (blocks & kAll) != kAll);
-                    const int lim = limit - t * KEYS;
-                    constexpr int kChunks = KEYS / 32;
-                    uint32_t sr[kChunks][32];
+                    const int first_key = t * KEYS + (i % G::kSteps) * 64;
+                    const unsigned blocks =
+                        SRC == kRows ? 0xfu : (s_mask[(kt + t - it.t0) % kMaskRing] >> (i % G::kSteps * 4)) & 0xfu;
+                    const bool masked = t >= careful || (SRC != kRows && blocks != 0xfu);
+                    const int lim = limit - first_key;
+                    uint32_t sr[2][32];
                     auto hide = [&](float *x, int c) {
 #pragma unroll
-                        for (int i = 0; i < 32; ++i)
-                            if (c * 32 + i >= lim || !((blocks >> (c * 2 + i / 16)) & 1u)) x[i] = -INFINITY;
+                        for (int e = 0; e < 32; ++e)
+                            if (c * 32 + e >= lim || !((blocks >> (c * 2 + e / 16)) & 1u)) x[e] = -INFINITY;
                     };
-#pragma unroll
-                    for (int c = 0; c < kChunks; ++c) tmem_ld32(s_addr + c * 32, sr[c]);
+                    tmem_ld32(s_addr, sr[0]);
+                    tmem_ld32(s_addr + 32, sr[1]);
                     // The row's maximum; NaN among the scores makes it NaN, and with it
                     // the row. (An infinite one gives NaN weights too.)
                     float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-                    for (int c = 0; c < kChunks; ++c) {
+                    for (int c = 0; c < 2; ++c) {
                         wait_ld32(sr[c]);
                         float *x = reinterpret_cast<float *>(sr[c]);
                         if (masked) hide(x, c);
 #pragma unroll
-                        for (int i = 0; i < 32; i += 8)
+                        for (int k = 0; k < 32; k += 8)
 #pragma unroll
-                            for (int e = 0; e < 4; ++e) mx[e] = max3(mx[e], x[i + e], x[i + 4 + e]);
+                            for (int e = 0; e < 4; ++e) mx[e] = max3(mx[e], x[k + e], x[k + 4 + e]);
                     }
                     const float mt = max3(max_nan(mx[0], mx[1]), mx[2], mx[3]) * scale;
                     const bool grew = !(mt <= m + kLazy);
@@ -440,15 +440,13 @@ prefill_attention_kernel(const __grid_constant__ CUtensorMap tq, const __grid_co
                         const float corr = m == -INFINITY ? 0.f : ex2(m - mn);
                         l *= corr;
                         m = mn;
-                        if (j > 0) {
-                            // O holds the tiles before this one: S of this tile was
-                            // issued after their product (head_dim 256: two S buffers,
-                            // so wait for the last product).
-                            if constexpr (NT == 1) {
-                                ok = wait(&pv_done, (pv_n + j - 1) & 1);
-                                if (!__all_sync(0xffffffffu, ok)) break;
-                                fence_after();
-                            }
+                        if (i > 0) {
+                            // O holds the steps before this one, once the last of
+                            // their products is complete (S of this step was issued
+                            // after the one before it).
+                            ok = wait(&pv_done[w], (pv_n + i - 1) & 1);
+                            if (!__all_sync(0xffffffffu, ok)) break;
+                            fence_after();
                             const uint32_t o_addr = tmem + lanes + G::kOCol + (NT == 2 ? w * D : 0);
 #pragma unroll
                             for (int c = 0; c < D / 16; ++c) {
@@ -456,7 +454,7 @@ prefill_attention_kernel(const __grid_constant__ CUtensorMap tq, const __grid_co
                                 tmem_ld16(o_addr + c * 16, o);
                                 wait_ld16(o);
 #pragma unroll
-                                for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * corr);
+                                for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * corr);
                                 tmem_st16(o_addr + c * 16, o);
                             }
                         }
@@ -469,30 +467,25 @@ prefill_attention_kernel(const __grid_constant__ CUtensorMap tq, const __grid_co
                     auto weights = [&](auto with_mask) {
                         constexpr bool MASKED = decltype(with_mask)::value;
 #pragma unroll
-                        for (int c = 0; c < kChunks; ++c) {
+                        for (int c = 0; c < 2; ++c) {
                             const float *s = reinterpret_cast<const float *>(sr[c]);
                             uint32_t pk[16];
 #pragma unroll
-                            for (int i = 0; i < 16; ++i) {
+                            for (int e = 0; e < 16; ++e) {
                                 float x, y;
-                                const uint64_t xy = fma2(pair(s[2 * i], s[2 * i + 1]), sc2, mr2);
-                                if (!MASKED && i % kPolyEvery == kPolyEvery - 1) {
+                                const uint64_t xy = fma2(pair(s[2 * e], s[2 * e + 1]), sc2, mr2);
+                                if (!MASKED && e % kPolyEvery == kPolyEvery - 1) {
                                     ex2_poly(xy, x, y);
                                 } else {
                                     unpair(xy, x, y);
                                     x = ex2(x);
                                     y = ex2(y);
                                 }
-                                sum[i & 1] = add2(sum[i & 1], pair(x, y));
-                                pk[i] = pack2<T>(x, y);
+                                sum[e & 1] = add2(sum[e & 1], pair(x, y));
+                                pk[e] = pack2<T>(x, y);
                             }
                             // Over scores that this row has read already.
                             tmem_st16(s_addr + c * 16, pk);
-                            if (c == kChunks / 2 - 1) {  // the first half's product may begin
-                                wait_st();
-                                fence_before();
-                                mbar_arrive(&p_half[buf]);
-                            }
                         }
                     };
                     if (masked) weights(std::true_type{});
@@ -503,11 +496,10 @@ prefill_attention_kernel(const __grid_constant__ CUtensorMap tq, const __grid_co
                     wait_st();
                 }
                 fence_before();
-                if (!warp_live) mbar_arrive(&p_half[buf]);
                 mbar_arrive(&p_full[buf]);
             }
             if (!__all_sync(0xffffffffu, ok)) break;
-            if (NT == 1) pv_n += n;
+            pv_n += mine * G::kSteps;
             kt += n;
 
             // ---- epilogue: this row's O (key items: the two halves merged) ----
@@ -649,34 +641,40 @@ prefill_attention_kernel(const __grid_constant__ CUtensorMap tq, const __grid_co
     } else if (warp == 8) {
         // ================= the products =================
         if (elect_one()) {
-            constexpr uint32_t id_s = instr_desc<T>(128, KEYS, false), id_o = instr_desc<T>(128, D, true);
+            constexpr uint32_t id_s = instr_desc<T>(128, 64, false), id_o = instr_desc<T>(128, D, true);
             const uint32_t q0 = smem_u32(sq), kv0 = smem_u32(skv);
-            unsigned pos = 0, p_ph[2] = {0, 0}, ou[2] = {0, 0}, qn = 0;
+            unsigned pos = 0, p_ph = 0, ou[2] = {0, 0}, qn = 0;
             bool ok = true;
             auto stage = [&](unsigned at) { return at % ST; };
             auto full = [&](unsigned at) { return wait(&kv_full[at % ST], (at / ST) & 1); };
             // Descriptors of the first tiles; an address moves the low word by
             // its 16-byte units (shared addresses fit its 14 bits).
             const uint64_t dq = smem_desc(q0, 16, 1024), dk = smem_desc(kv0, 16, 1024), dv = smem_desc(kv0, G::kSlab, 1024);
-            auto scores = [&](int qt, int buf, unsigned at) {
-                const uint64_t qd = dq + qt * (G::kQTile / 16), kd = dk + stage(at) * (G::kTile / 16);
+            // Step h (64 keys) of the tile at ring place `at`: its scores for row
+            // tile qt into S buffer b of warpgroup w, and its product with V.
+            auto scores = [&](int qt, int w, int b, unsigned at, int h) {
+                const uint64_t qd = dq + qt * (G::kQTile / 16), kd = dk + stage(at) * (G::kTile / 16) + h * (64 * 128 / 16);
 #pragma unroll
                 for (int k = 0; k < D / 16; ++k)
-                    mma_ss(tmem + buf * G::kSCols, qd + (k / 4) * (128 * 128 / 16) + (k % 4) * 2,
+                    mma_ss(tmem + (w * 2 + b) * 64, qd + (k / 4) * (128 * 128 / 16) + (k % 4) * 2,
                            kd + (k / 4) * (G::kSlab / 16) + (k % 4) * 2, id_s, k > 0);
+                commit(&s_full[w * 2 + b]);
             };
-            // The product of one half of the tile's keys (a row's weights of the
-            // first half are there while those of the second are computed).
-            auto values = [&](int half, int buf, int ob, unsigned at, bool accumulate) {
-                const uint64_t vd = dv + stage(at) * (G::kTile / 16);
+            // False when a wait gave up.
+            auto values = [&](int w, int b, unsigned at, int h, bool first) {
+                if (!wait(&p_full[w * 2 + b], (p_ph >> (w * 2 + b)) & 1)) return false;
+                p_ph ^= 1u << (w * 2 + b);
+                // The first product overwrites the O that the last item's epilogue read.
+                if (first && ou[w] > 0 && !wait(&o_free[w], (ou[w] - 1) & 1)) return false;
+                fence_after();
+                const uint64_t vd = dv + stage(at) * (G::kTile / 16) + h * (64 * 128 / 16);
 #pragma unroll
-                for (int k0 = 0; k0 < KEYS / 32; ++k0) {
-                    const int k = half * (KEYS / 32) + k0;
-                    mma_ts(tmem + G::kOCol + ob * D, tmem + buf * G::kSCols + k * 8, vd + k * (2048 / 16), id_o,
-                           accumulate || k > 0);
-                }
+                for (int k = 0; k < 4; ++k)
+                    mma_ts(tmem + G::kOCol + w * D, tmem + (w * 2 + b) * 64 + k * 8, vd + k * (2048 / 16), id_o,
+                           !first || k > 0);
+                commit(&pv_done[w]);
+                return true;
             };
-            auto o_ready = [&](int ob) { return ou[ob] == 0 || wait(&o_free[ob], (ou[ob] - 1) & 1); };
             for (; ok; ++item_n) {
                 const unsigned ring = item_n % kItemRing;
                 if (!wait(&item_full[ring], (item_n / kItemRing) & 1)) break;
@@ -689,43 +687,31 @@ prefill_attention_kernel(const __grid_constant__ CUtensorMap tq, const __grid_co
                 ++qn;
                 fence_after();
                 if (NT == 2 && it.two) {
+                    // Row items: the two warpgroups in turn, each tile's steps in order.
                     const int n0 = max(0, min(it.t1, (it.key0 + min(p.tile_tokens, it.tokens) + KEYS - 1) / KEYS) - it.t0);
                     if (!(ok = full(pos))) break;
                     fence_after();
-                    if (n0 > 0) scores(0, 0, pos), commit(&s_full[0]);
-                    scores(1, 1, pos);
-                    commit(&s_full[1]);
+#pragma unroll
+                    for (int h = 0; h < G::kSteps; ++h) {
+                        if (n0 > 0) scores(0, 0, h, pos, h);
+                        scores(1, 1, h, pos, h);
+                    }
                     commit(&kv_empty[stage(pos)]);
                     if (n == 1) commit(&q_empty);
-                    for (int j = 0; j < n; ++j) {
+                    for (int j = 0; j < n && ok; ++j) {
                         const unsigned va = pos + v_at(j, n, ahead_rows), ka = pos + k_at(j + 1, ahead_rows);
-                        if (!(ok = full(va))) break;
-                        if (j < n0) {
-                            if (!(ok = wait(&p_half[0], p_ph[0] & 1))) break;
-                            if (j == 0 && !(ok = o_ready(0))) break;
-                            fence_after();
-                            values(0, 0, 0, va, j > 0);
-                            if (!(ok = wait(&p_full[0], p_ph[0]++ & 1))) break;
-                            fence_after();
-                            values(1, 0, 0, va, true);
-                            if (j + 1 == n0) commit(&o_full[0]), ++ou[0];
+                        ok = full(va) && (j + 1 >= n || full(ka));
+#pragma unroll
+                        for (int h = 0; h < G::kSteps; ++h) {
+                            if (ok && j < n0) ok = values(0, h, va, h, j == 0 && h == 0);
+                            if (ok && j + 1 < n0) scores(0, 0, h, ka, h);
+                            if (ok) ok = values(1, h, va, h, j == 0 && h == 0);
+                            if (ok && j + 1 < n) scores(1, 1, h, ka, h);
                         }
-                        if (j + 1 < n) {
-                            if (!(ok = full(ka))) break;
-                            fence_after();
-                            if (j + 1 < n0) scores(0, 0, ka), commit(&s_full[0]);
-                        }
-                        if (!(ok = wait(&p_half[1], p_ph[1] & 1))) break;
-                        if (j == 0 && !(ok = o_ready(1))) break;
-                        fence_after();
-                        values(0, 1, 1, va, j > 0);
-                        if (!(ok = wait(&p_full[1], p_ph[1]++ & 1))) break;
-                        fence_after();
-                        values(1, 1, 1, va, true);
+                        if (!ok) break;
                         commit(&kv_empty[stage(va)]);
+                        if (j + 1 == n0) commit(&o_full[0]), ++ou[0];
                         if (j + 1 < n) {
-                            scores(1, 1, ka);
-                            commit(&s_full[1]);
                             commit(&kv_empty[stage(ka)]);
                             if (j + 2 == n) commit(&q_empty);
                         } else {
@@ -734,38 +720,35 @@ prefill_attention_kernel(const __grid_constant__ CUtensorMap tq, const __grid_co
                         }
                     }
                 } else {
-                    for (int i = 0; i < min(2, n); ++i) {
+                    // Key items: tiles alternate between the warpgroups. head_dim
+                    // 256: one warpgroup, whose S buffers the tiles alternate between.
+                    for (int i = 0; i < min(2, n) && ok; ++i) {
                         if (!(ok = full(pos + i))) break;
                         fence_after();
-                        scores(0, i, pos + i);
-                        commit(&s_full[i]);
+#pragma unroll
+                        for (int h = 0; h < G::kSteps; ++h) scores(0, NT == 2 ? i : 0, NT == 2 ? h : i, pos + i, h);
                         commit(&kv_empty[stage(pos + i)]);
                     }
                     if (!ok) break;
                     if (n <= 2) commit(&q_empty);
                     for (int j = 0; j < n; ++j) {
-                        const int buf = j & 1, ob = NT == 2 ? buf : 0;
-                        const bool first = NT == 2 ? j < 2 : j == 0;
+                        const int w = NT == 2 ? j & 1 : 0;
                         const unsigned va = pos + v_at(j, n, ahead_keys), ka = pos + k_at(j + 2, ahead_keys);
-                        if (!(ok = full(va))) break;
-                        if (!(ok = wait(&p_half[buf], p_ph[buf] & 1))) break;
-                        if (first && !(ok = o_ready(ob))) break;
-                        fence_after();
-                        values(0, buf, ob, va, !first);
-                        if (!(ok = wait(&p_full[buf], p_ph[buf]++ & 1))) break;
-                        fence_after();
-                        values(1, buf, ob, va, true);
+                        ok = full(va);
+#pragma unroll
+                        for (int h = 0; h < G::kSteps; ++h) {
+                            const int b = NT == 2 ? h : j & 1;
+                            if (ok) ok = values(w, b, va, h, h == 0 && (NT == 2 ? j < 2 : j == 0));
+                            if (ok && h == 0 && j + 2 < n) ok = full(ka);
+                            if (ok && j + 2 < n) scores(0, w, b, ka, h);
+                        }
+                        if (!ok) break;
                         commit(&kv_empty[stage(va)]);
-                        if (NT == 1) commit(&pv_done);
                         if (j + 2 < n) {
-                            if (!(ok = full(ka))) break;
-                            fence_after();
-                            scores(0, buf, ka);
-                            commit(&s_full[buf]);
                             commit(&kv_empty[stage(ka)]);
                             if (j + 3 == n) commit(&q_empty);
                         }
-                        if (NT == 2 ? j + 2 >= n : j + 1 == n) commit(&o_full[ob]), ++ou[ob];
+                        if (NT == 2 ? j + 2 >= n : j + 1 == n) commit(&o_full[w]), ++ou[w];
                     }
                 }
                 pos += 2 * n;
