@@ -65,7 +65,6 @@ constexpr long long kWaitCycles = 4000000000ll;           // about 2 s
 constexpr int kPrefillThreads = 512;
 constexpr int kItemRing = 4;
 constexpr int kMaskRing = 32;                             // key tiles whose block masks are kept
-constexpr int kRowRing = 4;                               // and whose pool rows (K runs 2 tiles before V)
 constexpr int kFlagWords = 12;                            // 3 key tiles of 128 bits
 // Registers a thread after the split of the launch's 128 x 512: softmax
 // threads hold a row of 128 scores, the others a few addresses.
@@ -81,8 +80,8 @@ constexpr int kPolyEvery = 4;
 
 enum Source { kPaged = 0, kPagedFp8 = 1, kRows = 2 };
 
-// Tile geometry. Operand tiles are slabs of 64 elements: [D / 64][rows][128 B],
-// 128-byte swizzled (16-byte chunk c of row r at c ^ (r % 8)).
+// Tile geometry. Operand tiles are slabs of 64 elements (128 bytes) a row,
+// 128-byte swizzled: 16-byte chunk c of row r at c ^ (r % 8).
 template <int D, Source SRC>
 struct Geom {
     static constexpr int kRowTiles = D == 256 ? 1 : 2;          // 128-row tiles per item
@@ -90,7 +89,10 @@ struct Geom {
     static constexpr int kSlabs = D / 64;
     static constexpr int kQTile = 128 * D * 2;
     static constexpr int kTile = kKeys * D * 2;                 // one K or V tile
-    static constexpr int kSlab = kKeys * 128;
+    // A tile of packed rows is [slab][row][128 B] (one box a slab); a paged one
+    // [8 rows][slab][row of 8][128 B], so that one box brings a page's 16 rows.
+    static constexpr int kSlab = SRC == kRows ? kKeys * 128 : 1024;      // bytes between slabs
+    static constexpr int kGroup8 = SRC == kRows ? 1024 : 1024 * kSlabs;  // and between groups of 8 rows
     static constexpr bool kFp8 = SRC == kPagedFp8;
     static constexpr int kStages = kFp8 ? (D == 64 ? 6 : 3) : (D == 64 ? 10 : 5);
     static constexpr int kRawTile = kKeys * D;                  // fp8: the tile's codes
@@ -121,7 +123,8 @@ struct Header {          // of a partial slot
 struct Params {
     PrefillLaunch a;
     int tile_tokens;     // tokens per 128-row tile: 128 / group
-    float *part_o;       // [2 * ctas][slot rows][D]
+    int wide;            // out takes 32-byte stores
+    float4 *part_o;      // [2 * ctas][slot rows / 128][D / 4][128]: a column of rows is contiguous
     float2 *part_ml;     // [2 * ctas][slot rows]: reference point (base 2), sum
     Header *headers;     // [2 * ctas]
 };
@@ -165,14 +168,15 @@ __device__ __forceinline__ Seq sequence(const PrefillLaunch &a, int s, bool repo
 // ends at key ctx + min((i + 1) * per, rows).
 template <int ROW_TILES>
 struct Costs {
-    long long ctx, per, rows, items, last;
+    long long ctx, per, rows, last;
+    int items;
     bool empty;
     __device__ __forceinline__ Costs(const Seq &q, int tile_tokens) {
         ctx = q.ctx;
         per = (long long)ROW_TILES * tile_tokens;
         rows = q.rows;
         empty = q.empty;
-        items = (rows + per - 1) / per;
+        items = q.rows > 0 ? (q.rows - 1) / (ROW_TILES * tile_tokens) + 1 : 0;
         const bool two = ROW_TILES == 2 && rows - (items - 1) * per > tile_tokens;
         last = empty ? kItemCost : (two ? 2 : 1) * (ctx + rows) + kItemCost;
     }
@@ -227,14 +231,23 @@ __device__ __forceinline__ uint32_t nonfinite_mask(uint32_t w) {  // a bit 15 / 
 __device__ __forceinline__ float wide(__nv_bfloat16 x) { return __bfloat162float(x); }
 __device__ __forceinline__ float wide(__half x) { return __half2float(x); }
 
-// Two E4M3 codes as a pair of T, exactly.
+// E4M3 codes as T, without the conversion unit (it shares the special-function
+// unit's issue with the softmax): sign, 4 exponent and 3 mantissa bits moved to
+// where T has them give value * 2^-8 (f16) or * 2^-120 (bf16), subnormals
+// included. f16 keeps the factor, which the scales undo; bf16 undoes it here,
+// exactly. A NaN code would come out as 480, so words that hold one are patched.
 template <typename T>
-__device__ __forceinline__ uint32_t codes_to(uint32_t two) {
-    uint32_t h;
-    asm("{\n\t.reg .b16 a, b;\n\tmov.b32 {a, b}, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, a;\n\t}" : "=r"(h) : "r"(two));
-    if constexpr (std::is_same_v<T, __half>) return h;
-    const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&h));
-    return pack2<__nv_bfloat16>(f.x, f.y);
+constexpr float kCodeScale = std::is_same_v<T, __half> ? 256.f : 1.f;
+template <typename T>
+__device__ __forceinline__ uint32_t codes_to(uint32_t spread) {  // two codes, each the high byte of its half
+    if constexpr (std::is_same_v<T, __half>) {
+        return (spread & 0x80008000u) | ((spread & 0x7f007f00u) >> 1);
+    } else {
+        const uint32_t w = (spread & 0x80008000u) | ((spread & 0x7f007f00u) >> 4);
+        uint32_t r;
+        asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(w), "r"(0x7b807b80u));  // 2^120
+        return r;
+    }
 }
 
 template <typename T, int D, Source SRC>
@@ -250,7 +263,6 @@ prefill_attention_kernel(const __grid_constant__ CUtensorMap tq, const __grid_co
     __shared__ Item s_item[kItemRing];
     __shared__ unsigned s_flag[kItemRing][kFlagWords + 1];
     __shared__ unsigned char s_mask[kMaskRing];
-    __shared__ int s_row[kRowRing][8];
     __shared__ Pos s_range[2];
     __shared__ uint32_t s_tmem;
     __shared__ volatile int s_failed;
@@ -272,7 +284,7 @@ prefill_attention_kernel(const __grid_constant__ CUtensorMap tq, const __grid_co
         for (int i = 0; i < 4; ++i) mbar_init(&s_full[i], 1), mbar_init(&p_full[i], 128);
         for (int i = 0; i < 2; ++i) mbar_init(&pv_done[i], 1), mbar_init(&o_full[i], 1), mbar_init(&o_free[i], 128);
         mbar_init(&pair_bar, 256), mbar_init(&q_full, 1), mbar_init(&q_empty, 1), mbar_init(&drain, 1);
-        for (int i = 0; i < kItemRing; ++i) mbar_init(&item_full[i], 1), mbar_init(&item_empty[i], 6 + 4 * NT);
+        for (int i = 0; i < kItemRing; ++i) mbar_init(&item_full[i], 1), mbar_init(&item_empty[i], 7 + 4 * NT);
         fence_barrier_init();
         s_failed = 0;
     }
@@ -393,7 +405,7 @@ prefill_attention_kernel(const __grid_constant__ CUtensorMap tq, const __grid_co
             int others = two && w ? max(0, min(it.t1, (it.key0 + min(p.tile_tokens, it.tokens) + KEYS - 1) / KEYS) - it.t0) : n;
             if (keys) mine = (n - w + 1) / 2, others = (n - (w ^ 1) + 1) / 2;
             float scale = a.scale_log2, v_scale = 1.f;
-            if constexpr (SRC == kPagedFp8) scale *= __ldg(a.k_scale + it.head), v_scale = __ldg(a.v_scale + it.head);
+            if constexpr (SRC == kPagedFp8) scale *= __ldg(a.k_scale + it.head) * kCodeScale<T>, v_scale = __ldg(a.v_scale + it.head) * kCodeScale<T>;
             float m = -INFINITY, l = 0.f;
             const bool warp_live = __any_sync(0xffffffffu, live);
             const int careful = first_careful(it);
@@ -415,7 +427,12 @@ prefill_attention_kernel(const __grid_constant__ CUtensorMap tq, const __grid_co
                     auto hide = [&](float *x, int c) {
 #pragma unroll
                         for (int e = 0; e < 32; ++e)
-                            if (c * 32 + e >= lim || !((blocks >> (c * 2 + e / 16)) & 1u)) x[e] = -INFINITY;
+                            if (c * 32 + e >= lim) x[e] = -INFINITY;
+                        if (SRC != kRows && blocks != 0xfu) {
+#pragma unroll
+                            for (int e = 0; e < 32; ++e)
+                                if (!((blocks >> (c * 2 + e / 16)) & 1u)) x[e] = -INFINITY;
+                        }
                     };
                     tmem_ld32(s_addr, sr[0]);
                     tmem_ld32(s_addr + 32, sr[1]);
@@ -462,34 +479,27 @@ prefill_attention_kernel(const __grid_constant__ CUtensorMap tq, const __grid_co
                     const float ref = m == -INFINITY ? 0.f : m;  // nothing yet: weights 2^-inf = 0
                     const uint64_t sc2 = pair(scale, scale), mr2 = pair(-ref, -ref);
                     uint64_t sum[2] = {pair(l, 0.f), pair(0.f, 0.f)};
-                    // Masked tiles take every weight from the special-function
-                    // unit: a hidden key's is 0 there, and 2^-125 from the polynomial.
-                    auto weights = [&](auto with_mask) {
-                        constexpr bool MASKED = decltype(with_mask)::value;
 #pragma unroll
-                        for (int c = 0; c < 2; ++c) {
-                            const float *s = reinterpret_cast<const float *>(sr[c]);
-                            uint32_t pk[16];
+                    for (int c = 0; c < 2; ++c) {
+                        const float *s = reinterpret_cast<const float *>(sr[c]);
+                        uint32_t pk[16];
 #pragma unroll
-                            for (int e = 0; e < 16; ++e) {
-                                float x, y;
-                                const uint64_t xy = fma2(pair(s[2 * e], s[2 * e + 1]), sc2, mr2);
-                                if (!MASKED && e % kPolyEvery == kPolyEvery - 1) {
-                                    ex2_poly(xy, x, y);
-                                } else {
-                                    unpair(xy, x, y);
-                                    x = ex2(x);
-                                    y = ex2(y);
-                                }
-                                sum[e & 1] = add2(sum[e & 1], pair(x, y));
-                                pk[e] = pack2<T>(x, y);
+                        for (int e = 0; e < 16; ++e) {
+                            float x, y;
+                            const uint64_t xy = fma2(pair(s[2 * e], s[2 * e + 1]), sc2, mr2);
+                            if (e % kPolyEvery == kPolyEvery - 1) {
+                                ex2_poly(xy, x, y);
+                            } else {
+                                unpair(xy, x, y);
+                                x = ex2(x);
+                                y = ex2(y);
                             }
-                            // Over scores that this row has read already.
-                            tmem_st16(s_addr + c * 16, pk);
+                            sum[e & 1] = add2(sum[e & 1], pair(x, y));
+                            pk[e] = pack2<T>(x, y);
                         }
-                    };
-                    if (masked) weights(std::true_type{});
-                    else weights(std::false_type{});
+                        // Over scores that this row has read already.
+                        tmem_st16(s_addr + c * 16, pk);
+                    }
                     float u, v;
                     unpair(add2(sum[0], sum[1]), u, v);
                     l = u + v;
@@ -512,59 +522,58 @@ prefill_attention_kernel(const __grid_constant__ CUtensorMap tq, const __grid_co
                 ++of_ph[ob];
             }
             int c0 = 0, c1 = D;
-            float f[2] = {1.f, 0.f};
-            bool use[2] = {true, false};
-            if constexpr (NT == 2) {
-                use[0] = w == 0 ? mine > 0 : false;
-                use[1] = w == 1 ? mine > 0 : false;
-                f[w] = 1.f;
-                f[w ^ 1] = 0.f;
-                if (keys) {
-                    stat[w * 128 + row] = make_float2(m, l);
-                    mbar_arrive(&pair_bar);
-                    ok = wait(&pair_bar, pair_n++ & 1);
+            // Factors of the two accumulators; a row item has one.
+            float f0 = w == 0 ? 1.f : 0.f, f1 = w == 1 ? 1.f : 0.f;
+            bool use0 = w == 0 && mine > 0, use1 = w == 1 && mine > 0;
+            if (keys) {
+                stat[w * 128 + row] = make_float2(m, l);
+                mbar_arrive(&pair_bar);
+                ok = wait(&pair_bar, pair_n++ & 1);
+                if (!__all_sync(0xffffffffu, ok)) break;
+                const float2 other = stat[(w ^ 1) * 128 + row];
+                const float mm = fmaxf(m, other.x);
+                const float mine_f = m == -INFINITY ? 0.f : ex2(m - mm);
+                const float other_f = other.x == -INFINITY ? 0.f : ex2(other.x - mm);
+                // A NaN sum stays: 0 * NaN.
+                l = l * mine_f + other.y * other_f;
+                m = mm;
+                f0 = w == 0 ? mine_f : other_f;
+                f1 = w == 0 ? other_f : mine_f;
+                use0 = n > 0;
+                use1 = n > 1;
+                // Each warpgroup stores half of the elements (of 64, the first all).
+                c0 = w * (D == 64 ? 64 : D / 2);
+                c1 = D == 64 ? 64 : c0 + D / 2;
+                // The wait above covers this warpgroup's half alone.
+                if (others > 0) {
+                    ok = wait(&o_full[w ^ 1], of_ph[w ^ 1] & 1);
                     if (!__all_sync(0xffffffffu, ok)) break;
-                    const float2 other = stat[(w ^ 1) * 128 + row];
-                    const float mm = fmaxf(m, other.x);
-                    const float mine_f = m == -INFINITY ? 0.f : ex2(m - mm);
-                    const float other_f = other.x == -INFINITY ? 0.f : ex2(other.x - mm);
-                    // A NaN sum stays: 0 * NaN.
-                    l = l * mine_f + other.y * other_f;
-                    m = mm;
-                    f[w] = mine_f;
-                    f[w ^ 1] = other_f;
-                    use[0] = n > 0;
-                    use[1] = n > 1;
-                    c0 = w * (D / 2);
-                    c1 = c0 + D / 2;
-                    // The wait above covers this warpgroup's half alone.
-                    if (others > 0) {
-                        ok = wait(&o_full[w ^ 1], of_ph[w ^ 1] & 1);
-                        if (!__all_sync(0xffffffffu, ok)) break;
-                    }
                 }
-                of_ph[w ^ 1] += others > 0;
-            } else {
-                use[0] = n > 0;
             }
+            if (NT == 2) of_ph[w ^ 1] += others > 0;
             fence_after();
             const unsigned flagged = s_flag[ring][kFlagWords];
             const float inv = l == 0.f ? 0.f : v_scale / l;
 #pragma unroll 1
-            for (int c = c0; c < c1; c += 32) {
-                float o[32];
-#pragma unroll
-                for (int i = 0; i < 32; ++i) o[i] = 0.f;
+            for (int c = c0; c < c1 && warp_live; c += 64) {
+                float o[64];
                 __syncwarp();
-                if (warp_live) {
 #pragma unroll
-                    for (int h = 0; h < NT; ++h) {
-                        if (!use[h]) continue;
-                        uint32_t r[32];
-                        tmem_ld32(tmem + lanes + G::kOCol + h * D + c, r);
+                for (int k = 0; k < 2; ++k) {
+                    uint32_t r[32];
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) o[k * 32 + i] = 0.f;
+                    if (use0) {
+                        tmem_ld32(tmem + lanes + G::kOCol + c + k * 32, r);
                         wait_ld32(r);
 #pragma unroll
-                        for (int i = 0; i < 32; ++i) o[i] = fmaf(__uint_as_float(r[i]), f[h], o[i]);
+                        for (int i = 0; i < 32; ++i) o[k * 32 + i] = __uint_as_float(r[i]) * f0;
+                    }
+                    if (NT == 2 && use1) {
+                        tmem_ld32(tmem + lanes + G::kOCol + D + c + k * 32, r);
+                        wait_ld32(r);
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) o[k * 32 + i] = fmaf(__uint_as_float(r[i]), f1, o[k * 32 + i]);
                     }
                 }
                 if (live && flagged) {
@@ -573,47 +582,73 @@ prefill_attention_kernel(const __grid_constant__ CUtensorMap tq, const __grid_co
                         if (!((s_flag[ring][b >> 5] >> (b & 31)) & 1u)) continue;
                         const int key = careful * KEYS + b;
                         if (key >= limit) continue;
-                        if constexpr (SRC == kPagedFp8) {
-                            const int blk = __ldg(a.tables + (long long)it.seq * a.table_stride + key / a.block_size);
-                            const uint8_t *v = static_cast<const uint8_t *>(a.v) +
-                                               (a.layer_row0 + (long long)blk * a.block_size + key % a.block_size) * a.kv_heads * D +
-                                               (long long)it.head * D + c;
-                            for (int i = 0; i < 32; ++i)
-                                if ((__ldg(v + i) & 0x7fu) == 0x7fu) o[i] = NAN;
+                        long long at;
+                        if constexpr (SRC == kRows) {
+                            at = (long long)(it.base + key) * a.kv_stride;
                         } else {
-                            const T *v = static_cast<const T *>(a.v);
-                            if constexpr (SRC == kPaged) {
-                                const int blk = __ldg(a.tables + (long long)it.seq * a.table_stride + key / a.block_size);
-                                v += (a.layer_row0 + (long long)blk * a.block_size + key % a.block_size) * a.kv_heads * D;
-                            } else {
-                                v += (long long)(it.base + key) * a.kv_stride;
-                            }
-                            v += (long long)it.head * D + c;
+                            const int blk = __ldg(a.tables + (long long)it.seq * a.table_stride + key / a.block_size);
+                            at = (a.layer_row0 + (long long)blk * a.block_size + key % a.block_size) * a.kv_heads * D;
+                        }
+                        at += (long long)it.head * D + c;
 #pragma unroll
-                            for (int i = 0; i < 32; ++i) {
-                                const float x = wide(v[i]);
+                        for (int i = 0; i < 64; ++i) {
+                            if constexpr (SRC == kPagedFp8) {
+                                if ((__ldg(static_cast<const uint8_t *>(a.v) + at + i) & 0x7fu) == 0x7fu) o[i] = NAN;
+                            } else {
+                                const float x = wide(static_cast<const T *>(a.v)[at + i]);
                                 if (!isfinite(x)) o[i] += x;
                             }
                         }
                     }
                 }
-                if (!live) {
-                } else if (it.slot < 0) {
-                    T *out = static_cast<T *>(a.out) + out_row * D + c;
+                if (it.slot >= 0) {
+                    float4 *part = p.part_o + (((long long)it.slot * NT + (two ? w : 0)) * (D / 4) + c / 4) * 128 + row;
+                    if (live) {
 #pragma unroll
-                    for (int i = 0; i < 32; i += 8) {
-                        uint4 x;
-                        x.x = pack2<T>(o[i] * inv, o[i + 1] * inv);
-                        x.y = pack2<T>(o[i + 2] * inv, o[i + 3] * inv);
-                        x.z = pack2<T>(o[i + 4] * inv, o[i + 5] * inv);
-                        x.w = pack2<T>(o[i + 6] * inv, o[i + 7] * inv);
-                        *reinterpret_cast<uint4 *>(out + i) = x;
+                        for (int i = 0; i < 16; ++i)
+                            part[i * 128] = make_float4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
                     }
-                } else {
-                    float *part = p.part_o + ((long long)it.slot * G::kSlotRows + (two ? w * 128 : 0) + row) * D + c;
+                    continue;
+                }
+                uint32_t x[32];
 #pragma unroll
-                    for (int i = 0; i < 32; i += 4)
-                        *reinterpret_cast<float4 *>(part + i) = make_float4(o[i], o[i + 1], o[i + 2], o[i + 3]);
+                for (int i = 0; i < 32; ++i) x[i] = pack2<T>(o[2 * i] * inv, o[2 * i + 1] * inv);
+                if (!p.wide) {
+                    uint4 *out = reinterpret_cast<uint4 *>(static_cast<T *>(a.out) + out_row * D + c);
+#pragma unroll
+                    for (int i = 0; i < 8; ++i)
+                        if (live) out[i] = make_uint4(x[4 * i], x[4 * i + 1], x[4 * i + 2], x[4 * i + 3]);
+                    continue;
+                }
+                // A lane has a row of its own: a store would meet 32 lines. Four lanes
+                // exchange 32-byte pieces of their four rows, so that each has one
+                // piece of every row and a store covers whole lines (measured: an
+                // item's stores 5,300 -> 2,000 cycles).
+                const bool hi = lane & 2, lo = lane & 1;
+                uint32_t y[2][16];
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    const uint32_t other = __shfl_xor_sync(0xffffffffu, hi ? x[i] : x[16 + i], 2);
+                    const uint32_t own = hi ? x[16 + i] : x[i];
+                    y[0][i] = hi ? other : own;
+                    y[1][i] = hi ? own : other;
+                }
+#pragma unroll
+                for (int k = 0; k < 2; ++k) {
+                    uint32_t z[2][8];
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        const uint32_t other = __shfl_xor_sync(0xffffffffu, lo ? y[k][i] : y[k][8 + i], 1);
+                        const uint32_t own = lo ? y[k][8 + i] : y[k][i];
+                        z[0][i] = lo ? other : own;
+                        z[1][i] = lo ? own : other;
+                    }
+#pragma unroll
+                    for (int q = 0; q < 2; ++q) {
+                        const int from = (lane & ~3) | (2 * k + q);
+                        const long long r = __shfl_sync(0xffffffffu, live ? out_row : -1, from);
+                        if (r >= 0) store32(static_cast<T *>(a.out) + r * D + c + (lane & 3) * 16, z[q]);
+                    }
                 }
             }
             __syncwarp();
@@ -649,11 +684,12 @@ prefill_attention_kernel(const __grid_constant__ CUtensorMap tq, const __grid_co
             auto full = [&](unsigned at) { return wait(&kv_full[at % ST], (at / ST) & 1); };
             // Descriptors of the first tiles; an address moves the low word by
             // its 16-byte units (shared addresses fit its 14 bits).
-            const uint64_t dq = smem_desc(q0, 16, 1024), dk = smem_desc(kv0, 16, 1024), dv = smem_desc(kv0, G::kSlab, 1024);
+            const uint64_t dq = smem_desc(q0, 16, 1024), dk = smem_desc(kv0, 16, G::kGroup8),
+                           dv = smem_desc(kv0, G::kSlab, G::kGroup8);
             // Step h (64 keys) of the tile at ring place `at`: its scores for row
             // tile qt into S buffer b of warpgroup w, and its product with V.
             auto scores = [&](int qt, int w, int b, unsigned at, int h) {
-                const uint64_t qd = dq + qt * (G::kQTile / 16), kd = dk + stage(at) * (G::kTile / 16) + h * (64 * 128 / 16);
+                const uint64_t qd = dq + qt * (G::kQTile / 16), kd = dk + stage(at) * (G::kTile / 16) + h * (8 * G::kGroup8 / 16);
 #pragma unroll
                 for (int k = 0; k < D / 16; ++k)
                     mma_ss(tmem + (w * 2 + b) * 64, qd + (k / 4) * (128 * 128 / 16) + (k % 4) * 2,
@@ -667,10 +703,10 @@ prefill_attention_kernel(const __grid_constant__ CUtensorMap tq, const __grid_co
                 // The first product overwrites the O that the last item's epilogue read.
                 if (first && ou[w] > 0 && !wait(&o_free[w], (ou[w] - 1) & 1)) return false;
                 fence_after();
-                const uint64_t vd = dv + stage(at) * (G::kTile / 16) + h * (64 * 128 / 16);
+                const uint64_t vd = dv + stage(at) * (G::kTile / 16) + h * (8 * G::kGroup8 / 16);
 #pragma unroll
                 for (int k = 0; k < 4; ++k)
-                    mma_ts(tmem + G::kOCol + w * D, tmem + (w * 2 + b) * 64 + k * 8, vd + k * (2048 / 16), id_o,
+                    mma_ts(tmem + G::kOCol + w * D, tmem + (w * 2 + b) * 64 + k * 8, vd + k * (2 * G::kGroup8 / 16), id_o,
                            !first || k > 0);
                 commit(&pv_done[w]);
                 return true;
@@ -703,14 +739,16 @@ prefill_attention_kernel(const __grid_constant__ CUtensorMap tq, const __grid_co
                         ok = full(va) && (j + 1 >= n || full(ka));
 #pragma unroll
                         for (int h = 0; h < G::kSteps; ++h) {
-                            if (ok && j < n0) ok = values(0, h, va, h, j == 0 && h == 0);
+                            if (ok && j < n0) {
+                                ok = values(0, h, va, h, j == 0 && h == 0);
+                                if (ok && h + 1 == G::kSteps && j + 1 == n0) commit(&o_full[0]), ++ou[0];
+                            }
                             if (ok && j + 1 < n0) scores(0, 0, h, ka, h);
                             if (ok) ok = values(1, h, va, h, j == 0 && h == 0);
                             if (ok && j + 1 < n) scores(1, 1, h, ka, h);
                         }
                         if (!ok) break;
                         commit(&kv_empty[stage(va)]);
-                        if (j + 1 == n0) commit(&o_full[0]), ++ou[0];
                         if (j + 1 < n) {
                             commit(&kv_empty[stage(ka)]);
                             if (j + 2 == n) commit(&q_empty);
@@ -758,8 +796,13 @@ prefill_attention_kernel(const __grid_constant__ CUtensorMap tq, const __grid_co
             const long long t0 = clock64();
             while (!mbar_try_wait(&drain, 0) && clock64() - t0 < kWaitCycles) {}
         }
-    } else if (warp == 9) {
-        // ================= K and V by TMA =================
+    } else if (warp == 9 || warp == 11) {
+        // ================= K (warp 9) and V (warp 11) by TMA =================
+        // Each takes its own places of the ring. The products free places in
+        // order and each warp skips at most two, fewer than the ring holds, so
+        // a stage's parity tells its turns apart.
+        const bool is_k = warp == 9;
+        const CUtensorMap *map = is_k ? &tk : &tv;
         unsigned pos = 0, kt = 0;
         bool ok = true;
         const uint32_t kv0 = smem_u32(skv), raw0 = smem_u32(sraw);
@@ -773,97 +816,81 @@ prefill_attention_kernel(const __grid_constant__ CUtensorMap tq, const __grid_co
             if (it.end) break;
             const int n = it.t1 - it.t0, ahead = NT == 2 && it.two ? ahead_rows : ahead_keys;
             const int careful = first_careful(it), len = it.key0 + it.tokens;
-            auto block_of = [&](int t) {  // of this lane's granule of key tile t
+            // Pages, 32 granules of 16 keys at a time: lane i of `rows` holds the pool
+            // row of granule base + i (-1: past the keys or outside the pool); the
+            // block ids of the next 32 are on their way meanwhile.
+            constexpr int kGroup = 32 / G::kGranules;  // key tiles per 32 granules
+            auto block_at = [&](int t) {
                 const int key = t * KEYS + lane * 16;
-                if (SRC == kRows || lane >= G::kGranules || t >= it.t1 || key >= len) return -1;
+                if (SRC == kRows || t >= it.t1 || key >= len) return -1;
                 return __ldg(a.tables + (long long)it.seq * a.table_stride + key / a.block_size);
             };
-            int next_blk = block_of(it.t0);
-            for (int f = 0; f < 2 * n; ++f) {
-                // Fill f of the item: K 0 .. ahead - 1, then V j and K j + ahead in turn.
-                bool is_k;
-                int j;
-                const int lead = min(ahead, n), both = n - lead;
-                if (f < lead) is_k = true, j = f;
-                else if (f - lead < 2 * both) is_k = (f - lead) & 1, j = ((f - lead) >> 1) + (is_k ? ahead : 0);
-                else is_k = false, j = both + (f - lead - 2 * both);
+            int rows = -1, next = block_at(it.t0);
+            unsigned usable = 0;  // granules whose keys count, or that a mask hides anyway
+            for (int j = 0; j < n; ++j) {
                 const int t = it.t0 + j;
-                const unsigned at = pos + f;
+                const unsigned at = pos + (is_k ? k_at(j, ahead) : v_at(j, n, ahead));
+                if (SRC != kRows && j % kGroup == 0) {
+                    const int key = t * KEYS + lane * 16;
+                    const bool have = key < len && t + lane / G::kGranules < it.t1;
+                    const bool good = have && next >= 0 && next < a.num_blocks;
+                    if (is_k && have && !good) record_error(a.err, kInvalidBlock, it.seq);
+                    rows = good ? (int)(a.layer_row0 + (long long)next * a.block_size + key % a.block_size) : -1;
+                    usable = __ballot_sync(0xffffffffu, good || !have);
+                    next = block_at(t + kGroup);
+                }
+                const bool by_hand = SRC != kPagedFp8 && !is_k && t >= careful;
+                uint64_t *full = SRC == kPagedFp8 ? &raw_full[at % RS] : &kv_full[at % ST];
+                uint64_t *empty = SRC == kPagedFp8 ? &raw_empty[at % RS] : &kv_empty[at % ST];
+                const unsigned turn = SRC == kPagedFp8 ? at / RS : at / ST;
+                ok = wait(empty, (turn & 1) ^ 1);
+                if (!__all_sync(0xffffffffu, ok)) break;
+                if (by_hand) {
+                    if (elect_one()) mbar_arrive(&by_hand_go[at % ST]);
+                    __syncwarp();
+                    continue;
+                }
                 if constexpr (SRC == kRows) {
                     if (elect_one()) {
-                        ok = wait(&kv_empty[at % ST], ((at / ST) & 1) ^ 1);
-                        if (ok && !is_k && t >= careful) {
-                            mbar_arrive(&by_hand_go[at % ST]);
-                        } else if (ok) {
-                            mbar_expect_tx(&kv_full[at % ST], G::kTile);
+                        mbar_expect_tx(full, G::kTile);
 #pragma unroll
-                            for (int c = 0; c < G::kSlabs; ++c)
-                                tma_load_2d(kv0 + (at % ST) * G::kTile + c * G::kSlab, is_k ? &tk : &tv,
-                                            it.head * D + c * 64, it.base + t * KEYS, &kv_full[at % ST]);
-                        }
+                        for (int c = 0; c < G::kSlabs; ++c)
+                            tma_load_2d(kv0 + (at % ST) * G::kTile + c * G::kSlab, map, it.head * D + c * 64,
+                                        it.base + t * KEYS, full);
                     }
-                    ok = __all_sync(0xffffffffu, ok);
-                    if (!ok) break;
                 } else {
-                    const bool by_hand = SRC == kPaged && !is_k && t >= careful;
-                    uint64_t *full = SRC == kPagedFp8 ? &raw_full[at % RS] : &kv_full[at % ST];
-                    uint64_t *empty = SRC == kPagedFp8 ? &raw_empty[at % RS] : &kv_empty[at % ST];
-                    const unsigned turn = SRC == kPagedFp8 ? at / RS : at / ST;
-                    if (is_k) {
-                        // Lane g finds the pool row of the tile's 16-key granule g (-1:
-                        // none), kept for the tile's V; the next tile's block ids are
-                        // on their way meanwhile.
-                        const int key = t * KEYS + lane * 16;
-                        const bool have = lane < G::kGranules && key < len;
-                        const bool good = have && next_blk >= 0 && next_blk < a.num_blocks;
-                        if (have && !good) record_error(a.err, kInvalidBlock, it.seq);
-                        const unsigned bits = __ballot_sync(0xffffffffu, good || (lane < G::kGranules && !have));
-                        if (lane < G::kGranules)
-                            s_row[(kt + j) % kRowRing][lane] =
-                                good ? (int)(a.layer_row0 + (long long)next_blk * a.block_size + key % a.block_size) : -1;
-                        if (lane == 0) s_mask[(kt + j) % kMaskRing] = (unsigned char)bits;
-                        next_blk = block_of(t + 1);
-                        __syncwarp();
+                    int y[G::kGranules], loads = 0;
+#pragma unroll
+                    for (int g = 0; g < G::kGranules; ++g) {
+                        y[g] = __shfl_sync(0xffffffffu, rows, j % kGroup * G::kGranules + g);
+                        loads += y[g] >= 0;
                     }
-                    ok = wait(empty, (turn & 1) ^ 1);
-                    ok = __all_sync(0xffffffffu, ok);
-                    if (!ok) break;
-                    if (by_hand) {
-                        if (lane == 0) mbar_arrive(&by_hand_go[at % ST]);
-                        continue;
-                    }
-                    const int *rows = s_row[(kt + j) % kRowRing];
-                    const unsigned loads = __ballot_sync(0xffffffffu, lane < G::kGranules && rows[lane & (G::kGranules - 1)] >= 0);
-                    unsigned char *dst = skv + (at % ST) * G::kTile;
-                    if (SRC == kPaged && !is_k && loads != (1u << G::kGranules) - 1) {
+                    const unsigned bits = (usable >> (j % kGroup * G::kGranules)) & ((1u << G::kGranules) - 1);
+                    if (SRC == kPaged && !is_k && loads < G::kGranules) {
                         // A block outside the pool: its values are zeros.
-                        for (int g = 0; g < G::kGranules; ++g) {
-                            if ((loads >> g) & 1u) continue;
-                            for (int i = lane; i < G::kSlabs * 128; i += 32)
-                                *reinterpret_cast<uint4 *>(dst + (i >> 7) * G::kSlab + g * 2048 + (i & 127) * 16) =
-                                    make_uint4(0, 0, 0, 0);
-                        }
+                        unsigned char *dst = skv + (at % ST) * G::kTile;
+#pragma unroll
+                        for (int g = 0; g < G::kGranules; ++g)
+                            for (int i = lane; y[g] < 0 && i < G::kSlabs * 128; i += 32)
+                                *reinterpret_cast<uint4 *>(dst + g * 2 * G::kGroup8 + i * 16) = make_uint4(0, 0, 0, 0);
                         fence_async();
                         __syncwarp();
                     }
                     if (elect_one()) {
-                        const CUtensorMap *map = is_k ? &tk : &tv;
-                        mbar_expect_tx(full, __popc(loads) * (SRC == kPagedFp8 ? 16 * D : 16 * D * 2));
+                        if (is_k) s_mask[(kt + j) % kMaskRing] = (unsigned char)bits;
+                        mbar_expect_tx(full, loads * (SRC == kPagedFp8 ? 16 * D : 16 * D * 2));
 #pragma unroll
                         for (int g = 0; g < G::kGranules; ++g) {
-                            const int y = rows[g];
-                            if (y < 0) continue;
-                            if constexpr (SRC == kPagedFp8) {
-                                tma_load_2d(raw0 + (at % RS) * G::kRawTile + g * 16 * D, map, it.head * D, y, full);
-                            } else {
-#pragma unroll
-                                for (int c = 0; c < G::kSlabs; ++c)
-                                    tma_load_2d(smem_u32(dst) + c * G::kSlab + g * 2048, map, it.head * D + c * 64, y, full);
-                            }
+                            if (y[g] < 0) continue;
+                            if constexpr (SRC == kPagedFp8)
+                                tma_load_2d(raw0 + (at % RS) * G::kRawTile + g * 16 * D, map, it.head * D, y[g], full);
+                            else
+                                tma_load_4d(kv0 + (at % ST) * G::kTile + g * 2 * G::kGroup8, map, 0, 0,
+                                            it.head * G::kSlabs, y[g] >> 3, full);
                         }
                     }
-                    __syncwarp();
                 }
+                __syncwarp();
             }
             pos += 2 * n;
             kt += n;
@@ -1033,7 +1060,7 @@ prefill_attention_kernel(const __grid_constant__ CUtensorMap tq, const __grid_co
                                 }
                                 note(t * KEYS + r);
                             }
-                            *reinterpret_cast<uint4 *>(dst + (u / 8) * G::kSlab + r * 128 + (((u % 8) ^ (r & 7)) << 4)) =
+                            *reinterpret_cast<uint4 *>(dst + (u / 8) * G::kSlab + (r >> 3) * G::kGroup8 + (r & 7) * 128 + (((u % 8) ^ (r & 7)) << 4)) =
                                 make_uint4(wds[0], wds[1], wds[2], wds[3]);
                         }
                     }
@@ -1066,24 +1093,26 @@ prefill_attention_kernel(const __grid_constant__ CUtensorMap tq, const __grid_co
                         // Values that no row may meet are zeros.
                         const bool gone = !is_k && (t * KEYS + r >= len || !((bits >> (r / 16)) & 1u));
                         if (gone) x = make_uint4(0, 0, 0, 0);
-                        if (!is_k && t >= careful) {
-                            uint32_t *w4 = reinterpret_cast<uint32_t *>(&x);
-#pragma unroll
-                            for (int k = 0; k < 4; ++k) {
-                                const uint32_t hit = ((w4[k] & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u;  // NaN codes
-                                if (hit) {
-                                    w4[k] &= ~((hit >> 7) * 0xffu);
-                                    note(t * KEYS + r);
-                                }
-                            }
-                        }
                         const uint32_t w4[4] = {x.x, x.y, x.z, x.w};
-                        uint4 lo, hi;
-                        lo.x = codes_to<T>(w4[0]), lo.y = codes_to<T>(w4[0] >> 16);
-                        lo.z = codes_to<T>(w4[1]), lo.w = codes_to<T>(w4[1] >> 16);
-                        hi.x = codes_to<T>(w4[2]), hi.y = codes_to<T>(w4[2] >> 16);
-                        hi.z = codes_to<T>(w4[3]), hi.w = codes_to<T>(w4[3] >> 16);
-                        unsigned char *row = dst + (u / 4) * G::kSlab + r * 128;
+                        uint32_t y[8], nans = 0;
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) {
+                            nans |= ((w4[k] & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u;
+                            y[2 * k] = codes_to<T>(__byte_perm(w4[k], 0, 0x1404));
+                            y[2 * k + 1] = codes_to<T>(__byte_perm(w4[k], 0, 0x3424));
+                        }
+                        if (nans) {  // rare: a NaN, or, in a value tile that a row masks, 0 and a note
+                            const bool zero = !is_k && t >= careful;
+                            for (int k = 0; k < 4; ++k)
+                                for (int q = 0; q < 4; ++q) {
+                                    if (((w4[k] >> (8 * q)) & 0x7fu) != 0x7fu) continue;
+                                    uint32_t &h = y[2 * k + q / 2];
+                                    h = (h & (q & 1 ? 0x0000ffffu : 0xffff0000u)) | (zero ? 0u : q & 1 ? 0x7fff0000u : 0x7fffu);
+                                }
+                            if (zero) note(t * KEYS + r);
+                        }
+                        const uint4 lo = make_uint4(y[0], y[1], y[2], y[3]), hi = make_uint4(y[4], y[5], y[6], y[7]);
+                        unsigned char *row = dst + (u / 4) * G::kSlab + (r >> 3) * G::kGroup8 + (r & 7) * 128;
                         const int c = 2 * (u % 4);
                         *reinterpret_cast<uint4 *>(row + ((c ^ (r & 7)) << 4)) = lo;
                         *reinterpret_cast<uint4 *>(row + (((c + 1) ^ (r & 7)) << 4)) = hi;
@@ -1114,73 +1143,70 @@ prefill_attention_kernel(const __grid_constant__ CUtensorMap tq, const __grid_co
 
 // Joins the partials of one split item, from the CTA whose share the item
 // begins in on: out = sum_i 2^(m_i - M) O_i / sum_i 2^(m_i - M) l_i, in the
-// order of the keys. A warp per row.
-constexpr int kJoinRows = 32;
+// order of the keys. A thread takes a row and 32 of its elements; a warp's
+// loads are contiguous.
 template <typename T, int D, int ROW_TILES>
-__global__ void __launch_bounds__(256) prefill_join_kernel(const __grid_constant__ Params p, int ctas) {
+__global__ void __launch_bounds__(128) prefill_join_kernel(const __grid_constant__ Params p, int ctas) {
     __shared__ int s_slot[512];
     __shared__ int s_count;
-    asm volatile("griddepcontrol.wait;" ::: "memory");
+    pdl_wait();
     const PrefillLaunch &a = p.a;
-    const int b = blockIdx.x;
+    const int b = blockIdx.x, w = blockIdx.y / (D / 32), c = blockIdx.y % (D / 32) * 32;
     const Header h = p.headers[2 * b + 1];
-    if (!h.valid) return;
-    const int group = a.group, r0 = blockIdx.y * kJoinRows, w = r0 / 128;
-    if (w && !h.two) return;
-    if (((r0 & 127) / group) + w * p.tile_tokens >= h.tokens || (r0 & 127) / group >= p.tile_tokens) return;
-    for (int i = threadIdx.x; i < ctas; i += 256)
-        s_slot[i] = i <= b ? 0 : p.headers[2 * i].valid * (p.headers[2 * i].last ? 2 : 1);
-    __syncthreads();
-    if (threadIdx.x == 0) {
+    if (!h.valid || (w && !h.two)) return;
+    const int lane = threadIdx.x & 31;
+    if (threadIdx.x < 32) {  // the later pieces: up to the one that ends the item
         int n = 0;
-        for (int i = b + 1; i < ctas; ++i) {
-            const int v = s_slot[i];
-            if (!v) continue;
-            s_slot[n++] = 2 * i;
-            if (v == 2) break;
+        for (int i0 = b + 1; i0 < ctas; i0 += 32) {
+            const int i = i0 + lane;
+            int valid = 0, last = 0;
+            if (i < ctas) valid = p.headers[2 * i].valid, last = valid && p.headers[2 * i].last;
+            unsigned some = __ballot_sync(0xffffffffu, valid);
+            const unsigned end = __ballot_sync(0xffffffffu, last);
+            if (end) some &= (2u << (__ffs(end) - 1)) - 1;
+            if ((some >> lane) & 1u) s_slot[n + __popc(some & ((1u << lane) - 1))] = 2 * i;
+            n += __popc(some);
+            if (end) break;
         }
-        s_count = n;
+        if (lane == 0) s_count = n;
     }
     __syncthreads();
-    const int count = s_count + 1, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    constexpr int kRows = ROW_TILES * 128, E = D / 32;
-    const float v_scale = a.v_scale ? __ldg(a.v_scale + h.head) : 1.f;
-    for (int r = r0 + warp; r < r0 + kJoinRows; r += 8) {
-        const int row = r & 127, tau = row / group, token = tau + w * p.tile_tokens;
-        if (tau >= p.tile_tokens || token >= h.tokens) continue;
-        auto slot = [&](int i) { return (long long)(i == 0 ? 2 * b + 1 : s_slot[i - 1]) * kRows + r; };
-        float M = -INFINITY;
-        for (int i = lane; i < count; i += 32) M = fmaxf(M, p.part_ml[slot(i)].x);
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
-        float L = 0.f, acc[E];
-#pragma unroll
-        for (int e = 0; e < E; ++e) acc[e] = 0.f;
+    const int group = a.group, row = threadIdx.x, tau = row / group, token = tau + w * p.tile_tokens;
+    if (tau >= p.tile_tokens || token >= h.tokens) return;
+    const int count = s_count + 1;
+    auto slot = [&](int i) { return (long long)(i == 0 ? 2 * b + 1 : s_slot[i - 1]) * ROW_TILES + w; };
+    float M = -INFINITY;
 #pragma unroll 4
-        for (int i = 0; i < count; ++i) {
-            const float2 ml = p.part_ml[slot(i)];
-            const float f = ml.x == -INFINITY ? 0.f : ex2(ml.x - M);
-            L = fmaf(ml.y, f, L);
-            const float *o = p.part_o + slot(i) * D + lane * E;
-            float x[E];
-            if constexpr (E == 2) *reinterpret_cast<float2 *>(x) = *reinterpret_cast<const float2 *>(o);
-            else
+    for (int i = 0; i < count; ++i) M = fmaxf(M, p.part_ml[slot(i) * 128 + row].x);
+    float L = 0.f, acc[32];
 #pragma unroll
-                for (int e = 0; e < E; e += 4) *reinterpret_cast<float4 *>(x + e) = *reinterpret_cast<const float4 *>(o + e);
+    for (int e = 0; e < 32; ++e) acc[e] = 0.f;
+#pragma unroll 2
+    for (int i = 0; i < count; ++i) {
+        const long long at = slot(i);
+        const float2 ml = p.part_ml[at * 128 + row];
+        const float f = ml.x == -INFINITY ? 0.f : ex2(ml.x - M);
+        L = fmaf(ml.y, f, L);
+        const float4 *o = p.part_o + (at * (D / 4) + c / 4) * 128 + row;
 #pragma unroll
-            for (int e = 0; e < E; ++e) acc[e] = fmaf(x[e], f, acc[e]);
+        for (int e = 0; e < 8; ++e) {
+            const float4 x = __ldcs(o + e * 128);
+            acc[4 * e] = fmaf(x.x, f, acc[4 * e]);
+            acc[4 * e + 1] = fmaf(x.y, f, acc[4 * e + 1]);
+            acc[4 * e + 2] = fmaf(x.z, f, acc[4 * e + 2]);
+            acc[4 * e + 3] = fmaf(x.w, f, acc[4 * e + 3]);
         }
-        const float inv = L == 0.f ? 0.f : v_scale / L;
-        const long long out_row = (long long)(h.row0 + token) * (a.kv_heads * group) + (long long)h.head * group + (row - tau * group);
-        uint32_t packed[E / 2];
-#pragma unroll
-        for (int e = 0; e < E; e += 2) packed[e / 2] = pack2<T>(acc[e] * inv, acc[e + 1] * inv);
-        uint32_t *out = reinterpret_cast<uint32_t *>(static_cast<T *>(a.out) + out_row * D + lane * E);
-        if constexpr (E == 2) *out = packed[0];
-        else if constexpr (E == 4) *reinterpret_cast<uint2 *>(out) = make_uint2(packed[0], packed[1]);
-        else *reinterpret_cast<uint4 *>(out) = make_uint4(packed[0], packed[1], packed[2], packed[3]);
-        if (lane == 0 && a.lse) a.lse[out_row] = L == 0.f ? -INFINITY : (M + log2f(L)) * 0.69314718055994531f;
     }
+    const float v_scale = a.v_scale ? __ldg(a.v_scale + h.head) * kCodeScale<T> : 1.f;
+    const float inv = L == 0.f ? 0.f : v_scale / L;
+    const long long out_row = (long long)(h.row0 + token) * (a.kv_heads * group) + (long long)h.head * group + (row - tau * group);
+    T *out = static_cast<T *>(a.out) + out_row * D + c;
+#pragma unroll
+    for (int e = 0; e < 32; e += 8)
+        *reinterpret_cast<uint4 *>(out + e) =
+            make_uint4(pack2<T>(acc[e] * inv, acc[e + 1] * inv), pack2<T>(acc[e + 2] * inv, acc[e + 3] * inv),
+                       pack2<T>(acc[e + 4] * inv, acc[e + 5] * inv), pack2<T>(acc[e + 6] * inv, acc[e + 7] * inv));
+    if (c == 0 && a.lse) a.lse[out_row] = L == 0.f ? -INFINITY : (M + log2f(L)) * 0.69314718055994531f;
 }
 
 PFN_cuTensorMapEncodeTiled_v12000 encoder() {
@@ -1203,6 +1229,17 @@ bool map_2d(CUtensorMap *m, CUtensorMapDataType t, int es, const void *base, lon
     const cuuint32_t box[2] = {(cuuint32_t)box_cols, (cuuint32_t)box_rows}, ones[2] = {1, 1};
     return encoder()(m, t, 2, const_cast<void *>(base), dims, strides, box, ones, CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle,
                      CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+// A pool plane as [rows / 8][slabs of 64][8 rows][64]: a box is 16 rows of a
+// head, groups of 8 rows outermost, as the paged tile has them.
+bool map_pages(CUtensorMap *m, CUtensorMapDataType t, const void *base, long long entry, long long rows, int slabs) {
+    const cuuint64_t dims[4] = {64, 8, (cuuint64_t)(entry / 64), (cuuint64_t)(rows / 8)};
+    const cuuint64_t strides[3] = {(cuuint64_t)(entry * 2), 128, (cuuint64_t)(entry * 16)};
+    const cuuint32_t box[4] = {64, 8, (cuuint32_t)slabs, 2}, ones[4] = {1, 1, 1, 1};
+    return encoder()(m, t, 4, const_cast<void *>(base), dims, strides, box, ones, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                     CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                     CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
 template <typename T, int D, Source SRC>
@@ -1231,13 +1268,12 @@ cudaError_t launch_tiles(const PrefillLaunch &a, const PrefillWorkspace &ws, int
         ok = map_2d(&tk, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, a.k, entry, a.pool_rows, entry, D, 16, CU_TENSOR_MAP_SWIZZLE_NONE) &&
              map_2d(&tv, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, a.v, entry, a.pool_rows, entry, D, 16, CU_TENSOR_MAP_SWIZZLE_NONE);
     } else {
-        ok = map_2d(&tk, t, 2, a.k, entry, a.pool_rows, entry, 64, 16, CU_TENSOR_MAP_SWIZZLE_128B) &&
-             map_2d(&tv, t, 2, a.v, entry, a.pool_rows, entry, 64, 16, CU_TENSOR_MAP_SWIZZLE_128B);
+        ok = map_pages(&tk, t, a.k, entry, a.pool_rows, D / 64) && map_pages(&tv, t, a.v, entry, a.pool_rows, D / 64);
     }
     if (!ok) return cudaErrorInvalidValue;
-    Params p{a, tile_tokens, nullptr, nullptr, nullptr};
+    Params p{a, tile_tokens, aligned(a.out, 32), nullptr, nullptr, nullptr};
     unsigned char *at = static_cast<unsigned char *>(ws.base);
-    p.part_o = reinterpret_cast<float *>(at);
+    p.part_o = reinterpret_cast<float4 *>(at);
     at += (size_t)2 * ws.ctas * G::kSlotRows * D * sizeof(float);
     p.part_ml = reinterpret_cast<float2 *>(at);
     at += (size_t)2 * ws.ctas * G::kSlotRows * sizeof(float2);
@@ -1247,7 +1283,7 @@ cudaError_t launch_tiles(const PrefillLaunch &a, const PrefillWorkspace &ws, int
     cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, G::kSmem);
     if (e != cudaSuccess) return e;
     if ((e = launch_pdl(kern, dim3((unsigned)ctas), dim3(kPrefillThreads), G::kSmem, st, tq, tk, tv, p)) != cudaSuccess) return e;
-    return launch_pdl(prefill_join_kernel<T, D, G::kRowTiles>, dim3((unsigned)ctas, G::kSlotRows / kJoinRows), dim3(256), 0, st, p, ctas);
+    return launch_pdl(prefill_join_kernel<T, D, G::kRowTiles>, dim3((unsigned)ctas, G::kRowTiles * (D / 32)), dim3(128), 0, st, p, ctas);
 }
 
 template <typename T, Source SRC>

@@ -75,6 +75,13 @@ __device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap *map
         "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(smem_u32(bar))
         : "memory");
 }
+__device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap *map, int x, int y, int z, int w, uint64_t *bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
+        " [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(dst),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(w), "r"(smem_u32(bar))
+        : "memory");
+}
 __device__ __forceinline__ void prefetch_map(const CUtensorMap *map) {
     asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(map)) : "memory");
 }
@@ -201,6 +208,13 @@ __device__ __forceinline__ void reg_dealloc() {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
 }
 
+// 32 bytes to 32-byte aligned global memory.
+__device__ __forceinline__ void store32(void *p, const uint32_t *x) {
+    asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(x[0]), "r"(x[1]), "r"(x[2]),
+                 "r"(x[3]), "r"(x[4]), "r"(x[5]), "r"(x[6]), "r"(x[7])
+                 : "memory");
+}
+
 // ---- arithmetic ------------------------------------------------------------------------
 
 __device__ __forceinline__ float ex2(float x) {
@@ -258,23 +272,24 @@ __device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
     return r;
 }
 
-// 2^x of a pair on the FMA units, for x <= 2^6 (below -125: about 2^-125): x =
-// n + f with n the nearest integer and |f| <= 1/2; 2^f by a polynomial of
-// degree 4, the minimax fit of its relative error on that interval (Remez
-// exchange; 2.7e-6 with f32 arithmetic), and n into the exponent.
+// 2^x of a pair on the FMA units, for x <= 2^6: x = n + f with n the nearest
+// integer and |f| <= 1/2; 2^f = 1 + f q(f), q of degree 3 by a minimax fit of
+// the relative error on that interval (2.9e-6 with f32 arithmetic); n is added
+// to the exponent. From -127 down n = -127 and f = 0, and 1.0 with its exponent
+// less 127 is the bit pattern of 0: what is hidden has the weight 0.
 __device__ __forceinline__ void ex2_poly(uint64_t x2, float &a, float &b) {
     float x, y;
     unpair(x2, x, y);
-    x2 = pair(fmaxf(x, -125.f), fmaxf(y, -125.f));
+    x2 = pair(fmaxf(x, -127.f), fmaxf(y, -127.f));
     const float shift = 12582912.f;  // 1.5 * 2^23: its sum's low bits are n
     const uint64_t t = add2(x2, pair(shift, shift));
     const uint64_t n = add2(t, pair(-shift, -shift));
     const uint64_t f = fma2(n, pair(-1.f, -1.f), x2);
-    uint64_t r = pair(0x1.3997d6p-7f, 0x1.3997d6p-7f);
-    r = fma2(r, f, pair(0x1.ca1444p-5f, 0x1.ca1444p-5f));
-    r = fma2(r, f, pair(0x1.ec06dap-3f, 0x1.ec06dap-3f));
-    r = fma2(r, f, pair(0x1.62e0dcp-1f, 0x1.62e0dcp-1f));
-    r = fma2(r, f, pair(0x1.ffffe8p-1f, 0x1.ffffe8p-1f));
+    uint64_t r = pair(0x1.3a02ccp-7f, 0x1.3a02ccp-7f);
+    r = fma2(r, f, pair(0x1.c9fc46p-5f, 0x1.c9fc46p-5f));
+    r = fma2(r, f, pair(0x1.ec0378p-3f, 0x1.ec0378p-3f));
+    r = fma2(r, f, pair(0x1.62e12cp-1f, 0x1.62e12cp-1f));
+    r = fma2(r, f, pair(1.f, 1.f));
     float tx, ty;
     unpair(t, tx, ty);
     unpair(r, a, b);
