@@ -99,6 +99,12 @@ struct Geom {
     static constexpr int kRawStages = kFp8 ? (D == 64 ? 6 : 3) : 0;
     static constexpr int kGranules = kKeys / 16;
     static constexpr int kSteps = kKeys / 64;                   // 64-key steps of a tile
+    // head_dim 128: the scores of a tile's two steps by one product of N = 128
+    // (N = 64 reads Q from shared memory twice as often as it can: its products
+    // took 2,900 cycles a tile in place of 2,100), although the next scores then
+    // wait for both steps' weights. 64: the softmax is longer than the products
+    // in any case, and two buffers keep it from waiting.
+    static constexpr bool kWide = D == 128;
     static constexpr int kOCol = kRowTiles * 128;               // after two S buffers of 64 columns a row tile
     static constexpr int kStatBytes = 2 * 128 * 8;
     static constexpr int kSmem = kRowTiles * kQTile + kStages * kTile + kRawStages * kRawTile + kStatBytes;
@@ -413,10 +419,12 @@ prefill_attention_kernel(const __grid_constant__ CUtensorMap tq, const __grid_co
                 const int j = i / G::kSteps, t = it.t0 + (keys ? 2 * j + w : j);
                 const int buf = w * 2 + (i & 1);
                 const uint32_t s_addr = tmem + lanes + buf * 64;
-                ok = wait(&s_full[buf], (s_ph >> (i & 1)) & 1);
-                if (!__all_sync(0xffffffffu, ok)) break;
-                s_ph ^= 1u << (i & 1);
-                fence_after();
+                if (!G::kWide || !(i & 1)) {
+                    ok = wait(&s_full[buf], (s_ph >> (i & 1)) & 1);
+                    if (!__all_sync(0xffffffffu, ok)) break;
+                    s_ph ^= 1u << (i & 1);
+                    fence_after();
+                }
                 if (warp_live) {
                     const int first_key = t * KEYS + (i % G::kSteps) * 64;
                     const unsigned blocks =
@@ -450,7 +458,8 @@ prefill_attention_kernel(const __grid_constant__ CUtensorMap tq, const __grid_co
                             for (int e = 0; e < 4; ++e) mx[e] = max3(mx[e], x[k + e], x[k + 4 + e]);
                     }
                     const float mt = max3(max_nan(mx[0], mx[1]), mx[2], mx[3]) * scale;
-                    const bool grew = !(mt <= m + kLazy);
+                    // (Rows of no token hold whatever Q's shared memory held: never.)
+                    const bool grew = live && !(mt <= m + kLazy);
                     if (__any_sync(0xffffffffu, grew)) {
                         float mn = max_nan(m, mt);
                         if (mn == INFINITY) mn = NAN;
@@ -676,8 +685,9 @@ prefill_attention_kernel(const __grid_constant__ CUtensorMap tq, const __grid_co
     } else if (warp == 8) {
         // ================= the products =================
         if (elect_one()) {
-            constexpr uint32_t id_s = instr_desc<T>(128, 64, false), id_o = instr_desc<T>(128, D, true);
+            constexpr uint32_t id_s = instr_desc<T>(128, G::kWide ? 128 : 64, false), id_o = instr_desc<T>(128, D, true);
             const uint32_t q0 = smem_u32(sq), kv0 = smem_u32(skv);
+            constexpr int kScores = G::kWide ? 1 : G::kSteps;  // products a tile's scores take
             unsigned pos = 0, p_ph = 0, ou[2] = {0, 0}, qn = 0;
             bool ok = true;
             auto stage = [&](unsigned at) { return at % ST; };
@@ -686,8 +696,9 @@ prefill_attention_kernel(const __grid_constant__ CUtensorMap tq, const __grid_co
             // its 16-byte units (shared addresses fit its 14 bits).
             const uint64_t dq = smem_desc(q0, 16, 1024), dk = smem_desc(kv0, 16, G::kGroup8),
                            dv = smem_desc(kv0, G::kSlab, G::kGroup8);
-            // Step h (64 keys) of the tile at ring place `at`: its scores for row
-            // tile qt into S buffer b of warpgroup w, and its product with V.
+            // Step h (64 keys; with kWide, step 0 both) of the tile at ring place
+            // `at`: its scores for row tile qt into S buffer b of warpgroup w, and
+            // its product with V.
             auto scores = [&](int qt, int w, int b, unsigned at, int h) {
                 const uint64_t qd = dq + qt * (G::kQTile / 16), kd = dk + stage(at) * (G::kTile / 16) + h * (8 * G::kGroup8 / 16);
 #pragma unroll
@@ -728,7 +739,7 @@ prefill_attention_kernel(const __grid_constant__ CUtensorMap tq, const __grid_co
                     if (!(ok = full(pos))) break;
                     fence_after();
 #pragma unroll
-                    for (int h = 0; h < G::kSteps; ++h) {
+                    for (int h = 0; h < kScores; ++h) {
                         if (n0 > 0) scores(0, 0, h, pos, h);
                         scores(1, 1, h, pos, h);
                     }
@@ -737,24 +748,27 @@ prefill_attention_kernel(const __grid_constant__ CUtensorMap tq, const __grid_co
                     for (int j = 0; j < n && ok; ++j) {
                         const unsigned va = pos + v_at(j, n, ahead_rows), ka = pos + k_at(j + 1, ahead_rows);
                         ok = full(va) && (j + 1 >= n || full(ka));
+                        const bool first = j == 0;
+                        auto turn = [&](int w, int h, int tiles) {  // a step of warpgroup w
+                            if (!ok || j >= tiles) return;
+                            ok = values(w, h, va, h, first && h == 0);
+                            if (!ok) return;
+                            const bool done = h + 1 == G::kSteps;
+                            if (done && j + 1 == tiles) commit(&o_full[w]), ++ou[w];
+                            if (j + 1 < tiles && (done || !G::kWide)) scores(w, w, G::kWide ? 0 : h, ka, G::kWide ? 0 : h);
+                        };
+                        if constexpr (G::kWide) {
 #pragma unroll
-                        for (int h = 0; h < G::kSteps; ++h) {
-                            if (ok && j < n0) {
-                                ok = values(0, h, va, h, j == 0 && h == 0);
-                                if (ok && h + 1 == G::kSteps && j + 1 == n0) commit(&o_full[0]), ++ou[0];
-                            }
-                            if (ok && j + 1 < n0) scores(0, 0, h, ka, h);
-                            if (ok) ok = values(1, h, va, h, j == 0 && h == 0);
-                            if (ok && j + 1 < n) scores(1, 1, h, ka, h);
+                            for (int x = 0; x < 2 * G::kSteps; ++x) turn(x / G::kSteps, x % G::kSteps, x / G::kSteps ? n : n0);
+                        } else {
+#pragma unroll
+                            for (int x = 0; x < 2 * G::kSteps; ++x) turn(x & 1, x >> 1, x & 1 ? n : n0);
                         }
                         if (!ok) break;
                         commit(&kv_empty[stage(va)]);
                         if (j + 1 < n) {
                             commit(&kv_empty[stage(ka)]);
                             if (j + 2 == n) commit(&q_empty);
-                        } else {
-                            commit(&o_full[1]);
-                            ++ou[1];
                         }
                     }
                 } else {
@@ -764,7 +778,7 @@ prefill_attention_kernel(const __grid_constant__ CUtensorMap tq, const __grid_co
                         if (!(ok = full(pos + i))) break;
                         fence_after();
 #pragma unroll
-                        for (int h = 0; h < G::kSteps; ++h) scores(0, NT == 2 ? i : 0, NT == 2 ? h : i, pos + i, h);
+                        for (int h = 0; h < kScores; ++h) scores(0, NT == 2 ? i : 0, NT == 2 ? h : i, pos + i, h);
                         commit(&kv_empty[stage(pos + i)]);
                     }
                     if (!ok) break;
@@ -778,7 +792,8 @@ prefill_attention_kernel(const __grid_constant__ CUtensorMap tq, const __grid_co
                             const int b = NT == 2 ? h : j & 1;
                             if (ok) ok = values(w, b, va, h, h == 0 && (NT == 2 ? j < 2 : j == 0));
                             if (ok && h == 0 && j + 2 < n) ok = full(ka);
-                            if (ok && j + 2 < n) scores(0, w, b, ka, h);
+                            if (ok && j + 2 < n && !G::kWide) scores(0, w, b, ka, h);
+                            if (ok && j + 2 < n && G::kWide && h + 1 == G::kSteps) scores(0, w, 0, ka, 0);
                         }
                         if (!ok) break;
                         commit(&kv_empty[stage(va)]);
