@@ -106,7 +106,7 @@ struct Geom {
     // in any case, and two buffers keep it from waiting.
     static constexpr bool kWide = D == 128;
     static constexpr int kOCol = kRowTiles * 128;               // after two S buffers of 64 columns a row tile
-    static constexpr int kStatBytes = 2 * 128 * 8;
+    static constexpr int kStatBytes = 2 * 128 * 8 + (SRC == kPagedFp8 ? 2 * 256 * 4 : 0);  // and the query rows' factors
     static constexpr int kSmem = kRowTiles * kQTile + kStages * kTile + kRawStages * kRawTile + kStatBytes;
     static constexpr int kSlotRows = kRowTiles * 128;           // rows of a partial
     static_assert(kOCol + kRowTiles * D <= 512, "tensor memory");
@@ -237,23 +237,11 @@ __device__ __forceinline__ uint32_t nonfinite_mask(uint32_t w) {  // a bit 15 / 
 __device__ __forceinline__ float wide(__nv_bfloat16 x) { return __bfloat162float(x); }
 __device__ __forceinline__ float wide(__half x) { return __half2float(x); }
 
-// E4M3 codes as T, without the conversion unit (it shares the special-function
-// unit's issue with the softmax): sign, 4 exponent and 3 mantissa bits moved to
-// where T has them give value * 2^-8 (f16) or * 2^-120 (bf16), subnormals
-// included. f16 keeps the factor, which the scales undo; bf16 undoes it here,
-// exactly. A NaN code would come out as 480, so words that hold one are patched.
-template <typename T>
-constexpr float kCodeScale = std::is_same_v<T, __half> ? 256.f : 1.f;
-template <typename T>
-__device__ __forceinline__ uint32_t codes_to(uint32_t spread) {  // two codes, each the high byte of its half
-    if constexpr (std::is_same_v<T, __half>) {
-        return (spread & 0x80008000u) | ((spread & 0x7f007f00u) >> 1);
-    } else {
-        const uint32_t w = (spread & 0x80008000u) | ((spread & 0x7f007f00u) >> 4);
-        uint32_t r;
-        asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(w), "r"(0x7b807b80u));  // 2^120
-        return r;
-    }
+// Two E4M3 codes (the low half of `two`) as f16, exactly.
+__device__ __forceinline__ uint32_t codes_to_f16(uint32_t two) {
+    uint32_t h;
+    asm("{\n\t.reg .b16 a, b;\n\tmov.b32 {a, b}, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, a;\n\t}" : "=r"(h) : "r"(two));
+    return h;
 }
 
 template <typename T, int D, Source SRC>
@@ -262,9 +250,15 @@ prefill_attention_kernel(const __grid_constant__ CUtensorMap tq, const __grid_co
                          const __grid_constant__ CUtensorMap tv, const __grid_constant__ Params p) {
     using G = Geom<D, SRC>;
     constexpr int NT = G::kRowTiles, KEYS = G::kKeys, ST = G::kStages, RS = G::kRawStages ? G::kRawStages : 1;
+    // Type of the products' operands. E4M3 codes become f16, which one conversion
+    // gives exactly, and so do bf16 queries over them: each row times the power
+    // of two that brings its largest element to [2^13, 2^14), its inverse joining
+    // the row's softmax scale.
+    using M = std::conditional_t<SRC == kPagedFp8, __half, T>;
+    constexpr bool kScaleQ = !std::is_same_v<M, T>;
     extern __shared__ __align__(1024) unsigned char smem[];
     __shared__ __align__(8) uint64_t kv_full[ST], kv_empty[ST], raw_full[RS], raw_empty[RS], by_hand_go[ST];
-    __shared__ __align__(8) uint64_t s_full[4], p_full[4], pv_done[2], o_full[2], o_free[2], pair_bar, q_full, q_empty, drain;
+    __shared__ __align__(8) uint64_t s_full[4], p_full[4], pv_done[2], o_full[2], o_free[2], pair_bar, q_full, q_raw, q_empty, drain;
     __shared__ __align__(8) uint64_t item_full[kItemRing], item_empty[kItemRing];
     __shared__ Item s_item[kItemRing];
     __shared__ unsigned s_flag[kItemRing][kFlagWords + 1];
@@ -277,6 +271,7 @@ prefill_attention_kernel(const __grid_constant__ CUtensorMap tq, const __grid_co
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     unsigned char *sq = smem, *skv = smem + NT * G::kQTile, *sraw = skv + ST * G::kTile;
     float2 *stat = reinterpret_cast<float2 *>(sraw + G::kRawStages * G::kRawTile);
+    float *q_factor = reinterpret_cast<float *>(stat + 2 * 128);
     long long *s_scan = reinterpret_cast<long long *>(stat);  // while the share is found
 
     if (smem_u32(smem) & 1023u) {  // the swizzle's atoms would not line up
@@ -289,8 +284,8 @@ prefill_attention_kernel(const __grid_constant__ CUtensorMap tq, const __grid_co
         for (int i = 0; i < RS; ++i) mbar_init(&raw_full[i], 1), mbar_init(&raw_empty[i], 1);
         for (int i = 0; i < 4; ++i) mbar_init(&s_full[i], 1), mbar_init(&p_full[i], 128);
         for (int i = 0; i < 2; ++i) mbar_init(&pv_done[i], 1), mbar_init(&o_full[i], 1), mbar_init(&o_free[i], 128);
-        mbar_init(&pair_bar, 256), mbar_init(&q_full, 1), mbar_init(&q_empty, 1), mbar_init(&drain, 1);
-        for (int i = 0; i < kItemRing; ++i) mbar_init(&item_full[i], 1), mbar_init(&item_empty[i], 7 + 4 * NT);
+        mbar_init(&pair_bar, 256), mbar_init(&q_full, 1), mbar_init(&q_raw, 1), mbar_init(&q_empty, 1), mbar_init(&drain, 1);
+        for (int i = 0; i < kItemRing; ++i) mbar_init(&item_full[i], 1), mbar_init(&item_empty[i], 1 + 2 + 4 + 4 * NT);
         fence_barrier_init();
         s_failed = 0;
     }
@@ -389,7 +384,7 @@ prefill_attention_kernel(const __grid_constant__ CUtensorMap tq, const __grid_co
         const int w = warp >> 2, row = tid & 127;
         const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
         const int group = a.group, tau = row / group, hq = row - tau * group;
-        unsigned s_ph = 0, of_ph[2] = {0, 0}, pv_n = 0, pair_n = 0;  // s_ph: a parity bit per S buffer
+        unsigned s_ph = 0, of_ph[2] = {0, 0}, pv_n = 0, pair_n = 0, qn = 0;  // s_ph: a parity bit per S buffer
         unsigned kt = 0;  // key tiles of earlier items
         bool ok = true;
         for (; ok; ++item_n) {
@@ -411,7 +406,7 @@ prefill_attention_kernel(const __grid_constant__ CUtensorMap tq, const __grid_co
             int others = two && w ? max(0, min(it.t1, (it.key0 + min(p.tile_tokens, it.tokens) + KEYS - 1) / KEYS) - it.t0) : n;
             if (keys) mine = (n - w + 1) / 2, others = (n - (w ^ 1) + 1) / 2;
             float scale = a.scale_log2, v_scale = 1.f;
-            if constexpr (SRC == kPagedFp8) scale *= __ldg(a.k_scale + it.head) * kCodeScale<T>, v_scale = __ldg(a.v_scale + it.head) * kCodeScale<T>;
+            if constexpr (SRC == kPagedFp8) scale *= __ldg(a.k_scale + it.head), v_scale = __ldg(a.v_scale + it.head);
             float m = -INFINITY, l = 0.f;
             const bool warp_live = __any_sync(0xffffffffu, live);
             const int careful = first_careful(it);
@@ -425,6 +420,7 @@ prefill_attention_kernel(const __grid_constant__ CUtensorMap tq, const __grid_co
                     s_ph ^= 1u << (i & 1);
                     fence_after();
                 }
+                if (kScaleQ && i == 0) scale *= q_factor[(qn & 1) * 256 + (two ? w * 128 : 0) + row];
                 if (warp_live) {
                     const int first_key = t * KEYS + (i % G::kSteps) * 64;
                     const unsigned blocks =
@@ -504,7 +500,7 @@ prefill_attention_kernel(const __grid_constant__ CUtensorMap tq, const __grid_co
                                 y = ex2(y);
                             }
                             sum[e & 1] = add2(sum[e & 1], pair(x, y));
-                            pk[e] = pack2<T>(x, y);
+                            pk[e] = pack2<M>(x, y);
                         }
                         // Over scores that this row has read already.
                         tmem_st16(s_addr + c * 16, pk);
@@ -519,6 +515,7 @@ prefill_attention_kernel(const __grid_constant__ CUtensorMap tq, const __grid_co
             }
             if (!__all_sync(0xffffffffu, ok)) break;
             pv_n += mine * G::kSteps;
+            qn += n > 0;
             kt += n;
 
             // ---- epilogue: this row's O (key items: the two halves merged) ----
@@ -684,47 +681,59 @@ prefill_attention_kernel(const __grid_constant__ CUtensorMap tq, const __grid_co
         }
     } else if (warp == 8) {
         // ================= the products =================
+        // One lane issues them all, the warpgroups' in turn: its order keeps one
+        // warpgroup in its softmax while the other's products run (with a lane per
+        // warpgroup the two fell into step: 0.99 -> 1.04 ms on 2,048 rows over 32 k
+        // keys).
         if (elect_one()) {
-            constexpr uint32_t id_s = instr_desc<T>(128, G::kWide ? 128 : 64, false), id_o = instr_desc<T>(128, D, true);
-            const uint32_t q0 = smem_u32(sq), kv0 = smem_u32(skv);
+            constexpr uint32_t id_s = instr_desc<M>(128, G::kWide ? 128 : 64, false), id_o = instr_desc<M>(128, D, true);
+            constexpr uint32_t hi_q = desc_hi(1024), hi_kv = desc_hi(G::kGroup8);
             constexpr int kScores = G::kWide ? 1 : G::kSteps;  // products a tile's scores take
-            unsigned pos = 0, p_ph = 0, ou[2] = {0, 0}, qn = 0;
+            const uint32_t lo_q = desc_lo(smem_u32(sq), 16), lo_k = desc_lo(smem_u32(skv), 16),
+                           lo_v = desc_lo(smem_u32(skv), G::kSlab);
+            unsigned place = 0, turn = 0;  // of the K/V ring, taken in order
+            unsigned p_ph = 0, ou[2] = {0, 0}, qn = 0;
             bool ok = true;
-            auto stage = [&](unsigned at) { return at % ST; };
-            auto full = [&](unsigned at) { return wait(&kv_full[at % ST], (at / ST) & 1); };
-            // Descriptors of the first tiles; an address moves the low word by
-            // its 16-byte units (shared addresses fit its 14 bits).
-            const uint64_t dq = smem_desc(q0, 16, 1024), dk = smem_desc(kv0, 16, G::kGroup8),
-                           dv = smem_desc(kv0, G::kSlab, G::kGroup8);
-            // Step h (64 keys; with kWide, step 0 both) of the tile at ring place
-            // `at`: its scores for row tile qt into S buffer b of warpgroup w, and
-            // its product with V.
-            auto scores = [&](int qt, int w, int b, unsigned at, int h) {
-                const uint64_t qd = dq + qt * (G::kQTile / 16), kd = dk + stage(at) * (G::kTile / 16) + h * (8 * G::kGroup8 / 16);
+            struct Tile {
+                unsigned stage, parity;
+            };
+            auto take = [&]() {
+                const Tile x{place, turn};
+                if (++place == ST) place = 0, turn ^= 1;
+                return x;
+            };
+            auto full = [&](const Tile &x) {
+                ok = ok && wait(&kv_full[x.stage], x.parity);
+                return ok;
+            };
+            // Step h (64 keys; with kWide, step 0 both) of tile x: its scores for row
+            // tile qt into S buffer b of warpgroup w.
+            auto scores = [&](int qt, int w, int b, const Tile &x, int h) {
+                const uint32_t q = lo_q + qt * (G::kQTile / 16),
+                               k = lo_k + x.stage * (G::kTile / 16) + h * (8 * G::kGroup8 / 16);
 #pragma unroll
-                for (int k = 0; k < D / 16; ++k)
-                    mma_ss(tmem + (w * 2 + b) * 64, qd + (k / 4) * (128 * 128 / 16) + (k % 4) * 2,
-                           kd + (k / 4) * (G::kSlab / 16) + (k % 4) * 2, id_s, k > 0);
+                for (int i = 0; i < D / 16; ++i)
+                    mma_ss<hi_q, hi_kv>(tmem + (w * 2 + b) * 64, q + (i / 4) * (128 * 128 / 16) + (i % 4) * 2,
+                                        k + (i / 4) * (G::kSlab / 16) + (i % 4) * 2, id_s, i > 0);
                 commit(&s_full[w * 2 + b]);
             };
-            // False when a wait gave up.
-            auto values = [&](int w, int b, unsigned at, int h, bool first) {
-                if (!wait(&p_full[w * 2 + b], (p_ph >> (w * 2 + b)) & 1)) return false;
+            // O += P V of step h, its weights in S buffer b of warpgroup w.
+            auto values = [&](int w, int b, const Tile &x, int h, bool first) {
+                if (!ok || !(ok = wait(&p_full[w * 2 + b], (p_ph >> (w * 2 + b)) & 1))) return;
                 p_ph ^= 1u << (w * 2 + b);
                 // The first product overwrites the O that the last item's epilogue read.
-                if (first && ou[w] > 0 && !wait(&o_free[w], (ou[w] - 1) & 1)) return false;
+                if (first && ou[w] > 0 && !(ok = wait(&o_free[w], (ou[w] - 1) & 1))) return;
                 fence_after();
-                const uint64_t vd = dv + stage(at) * (G::kTile / 16) + h * (8 * G::kGroup8 / 16);
+                const uint32_t v = lo_v + x.stage * (G::kTile / 16) + h * (8 * G::kGroup8 / 16);
 #pragma unroll
-                for (int k = 0; k < 4; ++k)
-                    mma_ts(tmem + G::kOCol + w * D, tmem + (w * 2 + b) * 64 + k * 8, vd + k * (2 * G::kGroup8 / 16), id_o,
-                           !first || k > 0);
+                for (int i = 0; i < 4; ++i)
+                    mma_ts<hi_kv>(tmem + G::kOCol + w * D, tmem + (w * 2 + b) * 64 + i * 8, v + i * (2 * G::kGroup8 / 16),
+                                  id_o, !first || i > 0);
                 commit(&pv_done[w]);
-                return true;
             };
             for (; ok; ++item_n) {
                 const unsigned ring = item_n % kItemRing;
-                if (!wait(&item_full[ring], (item_n / kItemRing) & 1)) break;
+                if (!(ok = wait(&item_full[ring], (item_n / kItemRing) & 1))) break;
                 const Item it = s_item[ring];
                 mbar_arrive(&item_empty[ring]);
                 if (it.end) break;
@@ -734,77 +743,75 @@ prefill_attention_kernel(const __grid_constant__ CUtensorMap tq, const __grid_co
                 ++qn;
                 fence_after();
                 if (NT == 2 && it.two) {
-                    // Row items: the two warpgroups in turn, each tile's steps in order.
+                    // Row items: both warpgroups take every tile; the first row tile may
+                    // end one early.
                     const int n0 = max(0, min(it.t1, (it.key0 + min(p.tile_tokens, it.tokens) + KEYS - 1) / KEYS) - it.t0);
-                    if (!(ok = full(pos))) break;
+                    Tile k = take();
+                    if (!full(k)) break;
                     fence_after();
 #pragma unroll
                     for (int h = 0; h < kScores; ++h) {
-                        if (n0 > 0) scores(0, 0, h, pos, h);
-                        scores(1, 1, h, pos, h);
+                        if (n0 > 0) scores(0, 0, h, k, h);
+                        scores(1, 1, h, k, h);
                     }
-                    commit(&kv_empty[stage(pos)]);
+                    commit(&kv_empty[k.stage]);
                     if (n == 1) commit(&q_empty);
-                    for (int j = 0; j < n && ok; ++j) {
-                        const unsigned va = pos + v_at(j, n, ahead_rows), ka = pos + k_at(j + 1, ahead_rows);
-                        ok = full(va) && (j + 1 >= n || full(ka));
-                        const bool first = j == 0;
-                        auto turn = [&](int w, int h, int tiles) {  // a step of warpgroup w
-                            if (!ok || j >= tiles) return;
-                            ok = values(w, h, va, h, first && h == 0);
+                    for (int j = 0; j < n; ++j) {
+                        const Tile v = take();
+                        if (j + 1 < n) k = take();
+                        if (!full(v) || (j + 1 < n && !full(k))) break;
+                        auto step = [&](int w, int h, int tiles) {
+                            if (j >= tiles) return;
+                            values(w, h, v, h, j == 0 && h == 0);
                             if (!ok) return;
                             const bool done = h + 1 == G::kSteps;
                             if (done && j + 1 == tiles) commit(&o_full[w]), ++ou[w];
-                            if (j + 1 < tiles && (done || !G::kWide)) scores(w, w, G::kWide ? 0 : h, ka, G::kWide ? 0 : h);
+                            if (j + 1 < tiles && (done || !G::kWide)) scores(w, w, G::kWide ? 0 : h, k, G::kWide ? 0 : h);
                         };
-                        if constexpr (G::kWide) {
 #pragma unroll
-                            for (int x = 0; x < 2 * G::kSteps; ++x) turn(x / G::kSteps, x % G::kSteps, x / G::kSteps ? n : n0);
-                        } else {
-#pragma unroll
-                            for (int x = 0; x < 2 * G::kSteps; ++x) turn(x & 1, x >> 1, x & 1 ? n : n0);
+                        for (int x = 0; x < 2 * G::kSteps; ++x) {
+                            if constexpr (G::kWide) step(x / G::kSteps, x % G::kSteps, x / G::kSteps ? n : n0);
+                            else step(x & 1, x >> 1, x & 1 ? n : n0);
                         }
                         if (!ok) break;
-                        commit(&kv_empty[stage(va)]);
-                        if (j + 1 < n) {
-                            commit(&kv_empty[stage(ka)]);
-                            if (j + 2 == n) commit(&q_empty);
-                        }
+                        commit(&kv_empty[v.stage]);
+                        if (j + 1 < n) commit(&kv_empty[k.stage]);
+                        if (j + 2 == n) commit(&q_empty);
                     }
                 } else {
-                    // Key items: tiles alternate between the warpgroups. head_dim
-                    // 256: one warpgroup, whose S buffers the tiles alternate between.
-                    for (int i = 0; i < min(2, n) && ok; ++i) {
-                        if (!(ok = full(pos + i))) break;
+                    // Key items: tiles alternate between the warpgroups. head_dim 256: one
+                    // warpgroup, whose S buffers the tiles alternate between.
+                    for (int i = 0; i < min(ahead_keys, n); ++i) {
+                        const Tile k = take();
+                        if (!full(k)) break;
                         fence_after();
 #pragma unroll
-                        for (int h = 0; h < kScores; ++h) scores(0, NT == 2 ? i : 0, NT == 2 ? h : i, pos + i, h);
-                        commit(&kv_empty[stage(pos + i)]);
+                        for (int h = 0; h < kScores; ++h) scores(0, NT == 2 ? i : 0, NT == 2 ? h : i, k, h);
+                        commit(&kv_empty[k.stage]);
                     }
                     if (!ok) break;
-                    if (n <= 2) commit(&q_empty);
+                    if (n <= ahead_keys) commit(&q_empty);
                     for (int j = 0; j < n; ++j) {
                         const int w = NT == 2 ? j & 1 : 0;
-                        const unsigned va = pos + v_at(j, n, ahead_keys), ka = pos + k_at(j + 2, ahead_keys);
-                        ok = full(va);
+                        const bool more = j + ahead_keys < n;
+                        const Tile v = take();
+                        Tile k = v;
+                        if (more) k = take();
+                        if (!full(v)) break;
 #pragma unroll
                         for (int h = 0; h < G::kSteps; ++h) {
                             const int b = NT == 2 ? h : j & 1;
-                            if (ok) ok = values(w, b, va, h, h == 0 && (NT == 2 ? j < 2 : j == 0));
-                            if (ok && h == 0 && j + 2 < n) ok = full(ka);
-                            if (ok && j + 2 < n && !G::kWide) scores(0, w, b, ka, h);
-                            if (ok && j + 2 < n && G::kWide && h + 1 == G::kSteps) scores(0, w, 0, ka, 0);
+                            values(w, b, v, h, h == 0 && j < NT);
+                            if (more && h == 0) full(k);
+                            if (ok && more && (!G::kWide || h + 1 == G::kSteps)) scores(0, w, G::kWide ? 0 : b, k, G::kWide ? 0 : h);
                         }
                         if (!ok) break;
-                        commit(&kv_empty[stage(va)]);
-                        if (j + 2 < n) {
-                            commit(&kv_empty[stage(ka)]);
-                            if (j + 3 == n) commit(&q_empty);
-                        }
-                        if (NT == 2 ? j + 2 >= n : j + 1 == n) commit(&o_full[w]), ++ou[w];
+                        commit(&kv_empty[v.stage]);
+                        if (more) commit(&kv_empty[k.stage]);
+                        if (j + ahead_keys + 1 == n) commit(&q_empty);
+                        if (j + NT >= n) commit(&o_full[w]), ++ou[w];
                     }
                 }
-                pos += 2 * n;
             }
             // Nothing may be in flight when tensor memory is freed.
             commit(&drain);
@@ -977,11 +984,12 @@ prefill_attention_kernel(const __grid_constant__ CUtensorMap tq, const __grid_co
                             if (ok) {
                                 const int tiles = it.two ? 2 : 1;
                                 const uint32_t bytes = (uint32_t)p.tile_tokens * a.group * 128;
-                                mbar_expect_tx(&q_full, tiles * G::kSlabs * bytes);
+                                uint64_t *bar = kScaleQ ? &q_raw : &q_full;
+                                mbar_expect_tx(bar, tiles * G::kSlabs * bytes);
                                 for (int x = 0; x < tiles; ++x)
                                     for (int c = 0; c < G::kSlabs; ++c)
                                         tma_load_3d(smem_u32(sq) + x * G::kQTile + c * (128 * 128), &tq, c * 64,
-                                                    it.head * a.group, it.row0 + x * p.tile_tokens, &q_full);
+                                                    it.head * a.group, it.row0 + x * p.tile_tokens, bar);
                             }
                         }
                         ++qn;
@@ -1003,16 +1011,17 @@ prefill_attention_kernel(const __grid_constant__ CUtensorMap tq, const __grid_co
         }
     } else if (warp >= 12) {
         // ================= V tiles by hand; fp8 conversion =================
+        constexpr int kT = 128;
         const int t128 = tid & 127;
-        unsigned pos = 0, kt = 0, go_ph = 0;
+        unsigned pos = 0, kt = 0, go_ph = 0, qn = 0;
         bool ok = true;
-        auto together = [&](bool good) -> bool {  // all four warps, and whether all are well
+        auto together = [&](bool good) -> bool {  // all of these warps, and whether all are well
             int r;
             __syncwarp();
             asm volatile(
                 "{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %1, 0;\n\t"
-                "barrier.cta.red.and.aligned.pred q, 2, 128, p;\n\tselp.b32 %0, 1, 0, q;\n\t}"
-                : "=r"(r) : "r"((int)good) : "memory");
+                "barrier.cta.red.and.aligned.pred q, 2, %2, p;\n\tselp.b32 %0, 1, 0, q;\n\t}"
+                : "=r"(r) : "r"((int)good), "n"(kT) : "memory");
             return r != 0;
         };
         for (; ok; ++item_n) {
@@ -1040,15 +1049,15 @@ prefill_attention_kernel(const __grid_constant__ CUtensorMap tq, const __grid_co
                     go_ph ^= 1u << (at % ST);
                     unsigned char *dst = skv + (at % ST) * G::kTile;
                     constexpr int kUnits = D / 8;                       // 16-byte units of a row
-                    constexpr int kEach = KEYS * kUnits / 128, kBatch = kEach < 8 ? kEach : 8;
+                    constexpr int kBatch = 8;
 #pragma unroll 1
-                    for (int b = 0; b < kEach; b += kBatch) {
+                    for (int b = t128; b < KEYS * kUnits; b += kBatch * kT) {
                         uint4 x[kBatch];
 #pragma unroll
                         for (int e = 0; e < kBatch; ++e) {
-                            const int i = (b + e) * 128 + t128, r = i / kUnits, u = i % kUnits, key = t * KEYS + r;
+                            const int i = b + e * kT, r = i / kUnits, u = i % kUnits, key = t * KEYS + r;
                             x[e] = make_uint4(0, 0, 0, 0);
-                            if (key >= len) continue;
+                            if (key >= len || r >= KEYS) continue;
                             const T *src = static_cast<const T *>(a.v) + (long long)it.head * D + u * 8;
                             if constexpr (SRC == kPaged) {
                                 const int blk = __ldg(a.tables + (long long)it.seq * a.table_stride + key / a.block_size);
@@ -1061,7 +1070,8 @@ prefill_attention_kernel(const __grid_constant__ CUtensorMap tq, const __grid_co
                         }
 #pragma unroll
                         for (int e = 0; e < kBatch; ++e) {
-                            const int i = (b + e) * 128 + t128, r = i / kUnits, u = i % kUnits;
+                            const int i = b + e * kT, r = i / kUnits, u = i % kUnits;
+                            if (r >= KEYS) break;
                             uint32_t wds[4] = {x[e].x, x[e].y, x[e].z, x[e].w};
                             uint32_t bad = 0;
 #pragma unroll
@@ -1084,6 +1094,41 @@ prefill_attention_kernel(const __grid_constant__ CUtensorMap tq, const __grid_co
                     if (t128 == 0) mbar_arrive(&kv_full[at % ST]);
                 }
             } else {
+                if (kScaleQ && n > 0) {
+                    // A thread to a row; its factor is kept per item (the softmax
+                    // of the last item may still read the other).
+                    ok = together(wait(&q_raw, qn & 1));
+                    if (!ok) break;
+                    for (int r = t128; r < (it.two ? 256 : 128); r += kT) {
+                        unsigned char *q = sq + (r >> 7) * G::kQTile + (r & 127) * 128;
+                        float top = 0.f;
+#pragma unroll 4
+                        for (int c = 0; c < D / 8; ++c) {
+                            const uint4 x = *reinterpret_cast<const uint4 *>(q + (c >> 3) * (128 * 128) + (c & 7) * 16);
+                            const __nv_bfloat162 *e = reinterpret_cast<const __nv_bfloat162 *>(&x);
+                            const __nv_bfloat162 y = __hmax2(__hmax2(__habs2(e[0]), __habs2(e[1])), __hmax2(__habs2(e[2]), __habs2(e[3])));
+                            top = fmaxf(top, fmaxf(__low2float(y), __high2float(y)));
+                        }
+                        int ex = 14;
+                        if (top > 0.f && top < INFINITY) frexpf(top, &ex);
+                        const float up = ldexpf(1.f, 14 - ex);
+                        q_factor[(qn & 1) * 256 + r] = ldexpf(1.f, ex - 14);
+#pragma unroll 4
+                        for (int c = 0; c < D / 8; ++c) {
+                            uint4 *at = reinterpret_cast<uint4 *>(q + (c >> 3) * (128 * 128) + (c & 7) * 16);
+                            const uint4 x = *at;
+                            const __nv_bfloat162 *e = reinterpret_cast<const __nv_bfloat162 *>(&x);
+                            uint32_t y[4];
+#pragma unroll
+                            for (int k = 0; k < 4; ++k) y[k] = pack2<__half>(__low2float(e[k]) * up, __high2float(e[k]) * up);
+                            *at = make_uint4(y[0], y[1], y[2], y[3]);
+                        }
+                    }
+                    ++qn;
+                    fence_async();
+                    together(true);
+                    if (t128 == 0) mbar_arrive(&q_full);
+                }
                 for (int f = 0; f < 2 * n && ok; ++f) {
                     bool is_k;
                     int j;
@@ -1100,38 +1145,39 @@ prefill_attention_kernel(const __grid_constant__ CUtensorMap tq, const __grid_co
                     unsigned char *dst = skv + (at % ST) * G::kTile;
                     const unsigned char *src = sraw + (at % RS) * G::kRawTile;
                     const unsigned bits = s_mask[(kt + j) % kMaskRing];
-                    constexpr int kUnits = D / 16, kEach = KEYS * kUnits / 128;
+                    constexpr int kUnits = D / 16;  // of 16 codes a row
+                    // Value tiles with rows that some or all queries must not meet: those
+                    // past the sequence or in blocks outside the pool are zeros, and NaN
+                    // codes are zeros and noted.
+                    const bool edge = !is_k && (t >= careful || bits != (1u << G::kGranules) - 1);
+                    auto convert = [&](auto with_edge) {
+#pragma unroll 4
+                        for (int i = t128; i < KEYS * kUnits; i += kT) {
+                            const int r = i / kUnits, u = i % kUnits;
+                            uint4 x = *reinterpret_cast<const uint4 *>(src + i * 16);
+                            uint32_t *w4 = reinterpret_cast<uint32_t *>(&x);
+                            if constexpr (decltype(with_edge)::value) {
+                                if (t * KEYS + r >= len || !((bits >> (r / 16)) & 1u)) x = make_uint4(0, 0, 0, 0);
 #pragma unroll
-                    for (int e = 0; e < kEach; ++e) {
-                        const int i = e * 128 + t128, r = i / kUnits, u = i % kUnits;
-                        uint4 x = *reinterpret_cast<const uint4 *>(src + r * D + u * 16);
-                        // Values that no row may meet are zeros.
-                        const bool gone = !is_k && (t * KEYS + r >= len || !((bits >> (r / 16)) & 1u));
-                        if (gone) x = make_uint4(0, 0, 0, 0);
-                        const uint32_t w4[4] = {x.x, x.y, x.z, x.w};
-                        uint32_t y[8], nans = 0;
-#pragma unroll
-                        for (int k = 0; k < 4; ++k) {
-                            nans |= ((w4[k] & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u;
-                            y[2 * k] = codes_to<T>(__byte_perm(w4[k], 0, 0x1404));
-                            y[2 * k + 1] = codes_to<T>(__byte_perm(w4[k], 0, 0x3424));
-                        }
-                        if (nans) {  // rare: a NaN, or, in a value tile that a row masks, 0 and a note
-                            const bool zero = !is_k && t >= careful;
-                            for (int k = 0; k < 4; ++k)
-                                for (int q = 0; q < 4; ++q) {
-                                    if (((w4[k] >> (8 * q)) & 0x7fu) != 0x7fu) continue;
-                                    uint32_t &h = y[2 * k + q / 2];
-                                    h = (h & (q & 1 ? 0x0000ffffu : 0xffff0000u)) | (zero ? 0u : q & 1 ? 0x7fff0000u : 0x7fffu);
+                                for (int k = 0; k < 4; ++k) {
+                                    const uint32_t hit = ((w4[k] & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u;
+                                    if (hit && t >= careful) {
+                                        w4[k] &= ~((hit >> 7) * 0xffu);
+                                        note(t * KEYS + r);
+                                    }
                                 }
-                            if (zero) note(t * KEYS + r);
+                            }
+                            unsigned char *row = dst + (u / 4) * G::kSlab + (r >> 3) * G::kGroup8 + (r & 7) * 128;
+                            const int c = 2 * (u % 4);
+#pragma unroll
+                            for (int k = 0; k < 2; ++k)
+                                *reinterpret_cast<uint4 *>(row + (((c + k) ^ (r & 7)) << 4)) =
+                                    make_uint4(codes_to_f16(w4[2 * k]), codes_to_f16(w4[2 * k] >> 16),
+                                               codes_to_f16(w4[2 * k + 1]), codes_to_f16(w4[2 * k + 1] >> 16));
                         }
-                        const uint4 lo = make_uint4(y[0], y[1], y[2], y[3]), hi = make_uint4(y[4], y[5], y[6], y[7]);
-                        unsigned char *row = dst + (u / 4) * G::kSlab + (r >> 3) * G::kGroup8 + (r & 7) * 128;
-                        const int c = 2 * (u % 4);
-                        *reinterpret_cast<uint4 *>(row + ((c ^ (r & 7)) << 4)) = lo;
-                        *reinterpret_cast<uint4 *>(row + (((c + 1) ^ (r & 7)) << 4)) = hi;
-                    }
+                    };
+                    if (edge) convert(std::true_type{});
+                    else convert(std::false_type{});
                     fence_async();
                     together(true);
                     if (t128 == 0) {
@@ -1212,7 +1258,7 @@ __global__ void __launch_bounds__(128) prefill_join_kernel(const __grid_constant
             acc[4 * e + 3] = fmaf(x.w, f, acc[4 * e + 3]);
         }
     }
-    const float v_scale = a.v_scale ? __ldg(a.v_scale + h.head) * kCodeScale<T> : 1.f;
+    const float v_scale = a.v_scale ? __ldg(a.v_scale + h.head) : 1.f;
     const float inv = L == 0.f ? 0.f : v_scale / L;
     const long long out_row = (long long)(h.row0 + token) * (a.kv_heads * group) + (long long)h.head * group + (row - tau * group);
     T *out = static_cast<T *>(a.out) + out_row * D + c;

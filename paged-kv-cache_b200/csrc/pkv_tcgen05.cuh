@@ -155,17 +155,19 @@ __device__ __forceinline__ void tmem_st32(uint32_t addr, const uint32_t *r) {
 // ---- tcgen05.mma --------------------------------------------------------------------
 
 // Shared-memory operand descriptor, 128-byte swizzle. A tile is slabs of 64
-// elements (128 bytes) of the contiguous dimension, each slab [rows][128
-// bytes]; 8 rows (1,024 bytes) are one swizzle atom.
+// elements (128 bytes) of the contiguous dimension; 8 rows (1,024 bytes) are one
+// swizzle atom.
 // - Contiguous dimension = the contraction (Q, K): rows are M or N; `step` is
 //   the distance of 8-row groups; the slab stride does not enter (a descriptor
 //   covers 16 elements of one slab).
 // - Contiguous dimension = N (V): rows are the contraction; `slab` is the
 //   distance of 64-element slabs, `step` that of 8-row groups.
-__device__ __forceinline__ uint64_t smem_desc(uint32_t addr, uint32_t slab, uint32_t step) {
-    return (uint64_t)((addr & 0x3FFFFu) >> 4) | ((uint64_t)(slab >> 4) << 16) | ((uint64_t)(step >> 4) << 32) |
-           (1ull << 46) | (2ull << 61);
+// The low word holds the address (in 16-byte units, 14 bits) and `slab`, and
+// moves with the address; the high word is a constant of the layout.
+__device__ __forceinline__ uint32_t desc_lo(uint32_t addr, uint32_t slab) {
+    return ((addr & 0x3FFFFu) >> 4) | ((slab >> 4) << 16);
 }
+__host__ __device__ constexpr uint32_t desc_hi(uint32_t step) { return (step >> 4) | (1u << 14) | (2u << 29); }
 
 // Instruction descriptor of kind::f16: f32 accumulator, both operands T
 // (f16: 0, bf16: 1), A with the contraction contiguous, B too or, with
@@ -177,19 +179,22 @@ __host__ __device__ constexpr uint32_t instr_desc(int m, int n, bool b_rows) {
            ((uint32_t)(m >> 4) << 24);
 }
 
-__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool accumulate) {
+template <uint32_t A_HI, uint32_t B_HI>
+__device__ __forceinline__ void mma_ss(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, bool accumulate) {
     asm volatile(
-        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
-        "l"(a), "l"(b), "r"(idesc), "r"((uint32_t)accumulate)
+        "{\n\t.reg .pred p;\n\t.reg .b64 da, db;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "mov.b64 da, {%1, %5};\n\tmov.b64 db, {%2, %6};\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %3, p;\n\t}" ::"r"(d),
+        "r"(a), "r"(b), "r"(idesc), "r"((uint32_t)accumulate), "n"(A_HI), "n"(B_HI)
         : "memory");
 }
 // A from tensor memory: lane = row, a 32-bit column = two elements.
-__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool accumulate) {
+template <uint32_t B_HI>
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, bool accumulate) {
     asm volatile(
-        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
-        "r"(a), "l"(b), "r"(idesc), "r"((uint32_t)accumulate)
+        "{\n\t.reg .pred p;\n\t.reg .b64 db;\n\tsetp.ne.b32 p, %4, 0;\n\tmov.b64 db, {%2, %5};\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], db, %3, p;\n\t}" ::"r"(d),
+        "r"(a), "r"(b), "r"(idesc), "r"((uint32_t)accumulate), "n"(B_HI)
         : "memory");
 }
 // One arrival on `bar` once every tcgen05 operation that this thread has
