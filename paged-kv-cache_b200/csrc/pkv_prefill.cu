@@ -268,7 +268,8 @@ prefill_attention_kernel(const __grid_constant__ CUtensorMap tq, const __grid_co
     __shared__ volatile int s_failed;
 
     const PrefillLaunch &a = p.a;
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int tid = threadIdx.x, lane = tid & 31;
+    const int warp = __shfl_sync(0xffffffffu, tid >> 5, 0);  // known to be the same in the whole warp
     unsigned char *sq = smem, *skv = smem + NT * G::kQTile, *sraw = skv + ST * G::kTile;
     float2 *stat = reinterpret_cast<float2 *>(sraw + G::kRawStages * G::kRawTile);
     float *q_factor = reinterpret_cast<float *>(stat + 2 * 128);
@@ -681,16 +682,19 @@ prefill_attention_kernel(const __grid_constant__ CUtensorMap tq, const __grid_co
         }
     } else if (warp == 8) {
         // ================= the products =================
-        // One lane issues them all, the warpgroups' in turn: its order keeps one
-        // warpgroup in its softmax while the other's products run (with a lane per
+        // One warp issues them all, the warpgroups' in turn: its order keeps one
+        // warpgroup in its softmax while the other's products run (with a warp per
         // warpgroup the two fell into step: 0.99 -> 1.04 ms on 2,048 rows over 32 k
-        // keys).
-        if (elect_one()) {
+        // keys). The whole warp runs the loops and one lane issues: what is the same
+        // in all lanes sits in uniform registers, where tcgen05.mma takes its
+        // operands, and need not be moved there for each.
+        {
             constexpr uint32_t id_s = instr_desc<M>(128, G::kWide ? 128 : 64, false), id_o = instr_desc<M>(128, D, true);
             constexpr uint32_t hi_q = desc_hi(1024), hi_kv = desc_hi(G::kGroup8);
             constexpr int kScores = G::kWide ? 1 : G::kSteps;  // products a tile's scores take
             const uint32_t lo_q = desc_lo(smem_u32(sq), 16), lo_k = desc_lo(smem_u32(skv), 16),
                            lo_v = desc_lo(smem_u32(skv), G::kSlab);
+            const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0);
             unsigned place = 0, turn = 0;  // of the K/V ring, taken in order
             unsigned p_ph = 0, ou[2] = {0, 0}, qn = 0;
             bool ok = true;
@@ -702,50 +706,62 @@ prefill_attention_kernel(const __grid_constant__ CUtensorMap tq, const __grid_co
                 if (++place == ST) place = 0, turn ^= 1;
                 return x;
             };
-            auto full = [&](const Tile &x) {
-                ok = ok && wait(&kv_full[x.stage], x.parity);
-                return ok;
+            auto all = [&](bool good) { return ok = __all_sync(0xffffffffu, good) != 0; };
+            auto full = [&](const Tile &x) { return ok && all(wait(&kv_full[x.stage], x.parity)); };
+            auto done_with = [&](uint64_t *bar) {
+                if (elect_one()) commit(bar);
+                __syncwarp();
             };
             // Step h (64 keys; with kWide, step 0 both) of tile x: its scores for row
             // tile qt into S buffer b of warpgroup w.
             auto scores = [&](int qt, int w, int b, const Tile &x, int h) {
                 const uint32_t q = lo_q + qt * (G::kQTile / 16),
                                k = lo_k + x.stage * (G::kTile / 16) + h * (8 * G::kGroup8 / 16);
+                if (elect_one()) {
 #pragma unroll
-                for (int i = 0; i < D / 16; ++i)
-                    mma_ss<hi_q, hi_kv>(tmem + (w * 2 + b) * 64, q + (i / 4) * (128 * 128 / 16) + (i % 4) * 2,
-                                        k + (i / 4) * (G::kSlab / 16) + (i % 4) * 2, id_s, i > 0);
-                commit(&s_full[w * 2 + b]);
+                    for (int i = 0; i < D / 16; ++i)
+                        mma_ss<hi_q, hi_kv>(tm + (w * 2 + b) * 64, q + (i / 4) * (128 * 128 / 16) + (i % 4) * 2,
+                                            k + (i / 4) * (G::kSlab / 16) + (i % 4) * 2, id_s, i > 0);
+                    commit(&s_full[w * 2 + b]);
+                }
+                __syncwarp();
             };
             // O += P V of step h, its weights in S buffer b of warpgroup w.
             auto values = [&](int w, int b, const Tile &x, int h, bool first) {
-                if (!ok || !(ok = wait(&p_full[w * 2 + b], (p_ph >> (w * 2 + b)) & 1))) return;
+                if (!ok || !all(wait(&p_full[w * 2 + b], (p_ph >> (w * 2 + b)) & 1))) return;
                 p_ph ^= 1u << (w * 2 + b);
                 // The first product overwrites the O that the last item's epilogue read.
-                if (first && ou[w] > 0 && !(ok = wait(&o_free[w], (ou[w] - 1) & 1))) return;
+                if (first && ou[w] > 0 && !all(wait(&o_free[w], (ou[w] - 1) & 1))) return;
                 fence_after();
                 const uint32_t v = lo_v + x.stage * (G::kTile / 16) + h * (8 * G::kGroup8 / 16);
+                if (elect_one()) {
 #pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    mma_ts<hi_kv>(tmem + G::kOCol + w * D, tmem + (w * 2 + b) * 64 + i * 8, v + i * (2 * G::kGroup8 / 16),
-                                  id_o, !first || i > 0);
-                commit(&pv_done[w]);
+                    for (int i = 0; i < 4; ++i)
+                        mma_ts<hi_kv>(tm + G::kOCol + w * D, tm + (w * 2 + b) * 64 + i * 8, v + i * (2 * G::kGroup8 / 16),
+                                      id_o, !first || i > 0);
+                    commit(&pv_done[w]);
+                }
+                __syncwarp();
             };
             for (; ok; ++item_n) {
                 const unsigned ring = item_n % kItemRing;
-                if (!(ok = wait(&item_full[ring], (item_n / kItemRing) & 1))) break;
-                const Item it = s_item[ring];
-                mbar_arrive(&item_empty[ring]);
-                if (it.end) break;
-                const int n = it.t1 - it.t0;
+                if (!all(wait(&item_full[ring], (item_n / kItemRing) & 1))) break;
+                const Item &item = s_item[ring];
+                const int end = __shfl_sync(0xffffffffu, item.end, 0), two = __shfl_sync(0xffffffffu, item.two, 0);
+                const int n = __shfl_sync(0xffffffffu, item.t1 - item.t0, 0);
+                // Tiles of the first row tile, which may end one early.
+                const int n0 = __shfl_sync(
+                    0xffffffffu,
+                    max(0, min(item.t1, (item.key0 + min(p.tile_tokens, item.tokens) + KEYS - 1) / KEYS) - item.t0), 0);
+                if (lane == 0) mbar_arrive(&item_empty[ring]);
+                __syncwarp();
+                if (end) break;
                 if (n == 0) continue;
-                if (!(ok = wait(&q_full, qn & 1))) break;
+                if (!all(wait(&q_full, qn & 1))) break;
                 ++qn;
                 fence_after();
-                if (NT == 2 && it.two) {
-                    // Row items: both warpgroups take every tile; the first row tile may
-                    // end one early.
-                    const int n0 = max(0, min(it.t1, (it.key0 + min(p.tile_tokens, it.tokens) + KEYS - 1) / KEYS) - it.t0);
+                if (NT == 2 && two) {
+                    // Row items: both warpgroups take every tile.
                     Tile k = take();
                     if (!full(k)) break;
                     fence_after();
@@ -754,8 +770,8 @@ prefill_attention_kernel(const __grid_constant__ CUtensorMap tq, const __grid_co
                         if (n0 > 0) scores(0, 0, h, k, h);
                         scores(1, 1, h, k, h);
                     }
-                    commit(&kv_empty[k.stage]);
-                    if (n == 1) commit(&q_empty);
+                    done_with(&kv_empty[k.stage]);
+                    if (n == 1) done_with(&q_empty);
                     for (int j = 0; j < n; ++j) {
                         const Tile v = take();
                         if (j + 1 < n) k = take();
@@ -765,7 +781,7 @@ prefill_attention_kernel(const __grid_constant__ CUtensorMap tq, const __grid_co
                             values(w, h, v, h, j == 0 && h == 0);
                             if (!ok) return;
                             const bool done = h + 1 == G::kSteps;
-                            if (done && j + 1 == tiles) commit(&o_full[w]), ++ou[w];
+                            if (done && j + 1 == tiles) done_with(&o_full[w]), ++ou[w];
                             if (j + 1 < tiles && (done || !G::kWide)) scores(w, w, G::kWide ? 0 : h, k, G::kWide ? 0 : h);
                         };
 #pragma unroll
@@ -774,9 +790,9 @@ prefill_attention_kernel(const __grid_constant__ CUtensorMap tq, const __grid_co
                             else step(x & 1, x >> 1, x & 1 ? n : n0);
                         }
                         if (!ok) break;
-                        commit(&kv_empty[v.stage]);
-                        if (j + 1 < n) commit(&kv_empty[k.stage]);
-                        if (j + 2 == n) commit(&q_empty);
+                        done_with(&kv_empty[v.stage]);
+                        if (j + 1 < n) done_with(&kv_empty[k.stage]);
+                        if (j + 2 == n) done_with(&q_empty);
                     }
                 } else {
                     // Key items: tiles alternate between the warpgroups. head_dim 256: one
@@ -787,10 +803,10 @@ prefill_attention_kernel(const __grid_constant__ CUtensorMap tq, const __grid_co
                         fence_after();
 #pragma unroll
                         for (int h = 0; h < kScores; ++h) scores(0, NT == 2 ? i : 0, NT == 2 ? h : i, k, h);
-                        commit(&kv_empty[k.stage]);
+                        done_with(&kv_empty[k.stage]);
                     }
                     if (!ok) break;
-                    if (n <= ahead_keys) commit(&q_empty);
+                    if (n <= ahead_keys) done_with(&q_empty);
                     for (int j = 0; j < n; ++j) {
                         const int w = NT == 2 ? j & 1 : 0;
                         const bool more = j + ahead_keys < n;
@@ -806,15 +822,15 @@ prefill_attention_kernel(const __grid_constant__ CUtensorMap tq, const __grid_co
                             if (ok && more && (!G::kWide || h + 1 == G::kSteps)) scores(0, w, G::kWide ? 0 : b, k, G::kWide ? 0 : h);
                         }
                         if (!ok) break;
-                        commit(&kv_empty[v.stage]);
-                        if (more) commit(&kv_empty[k.stage]);
-                        if (j + ahead_keys + 1 == n) commit(&q_empty);
-                        if (j + NT >= n) commit(&o_full[w]), ++ou[w];
+                        done_with(&kv_empty[v.stage]);
+                        if (more) done_with(&kv_empty[k.stage]);
+                        if (j + ahead_keys + 1 == n) done_with(&q_empty);
+                        if (j + NT >= n) done_with(&o_full[w]), ++ou[w];
                     }
                 }
             }
             // Nothing may be in flight when tensor memory is freed.
-            commit(&drain);
+            done_with(&drain);
             const long long t0 = clock64();
             while (!mbar_try_wait(&drain, 0) && clock64() - t0 < kWaitCycles) {}
         }
