@@ -1340,6 +1340,7 @@ Status B200Backend::attention_chunk_dev(int64_t layer, const void *q, DType quer
         a.v_scale = d_inv_ + 3 * stride + at;
     }
     a.err = d_err_;
+    a.device = device_;
     s = attention_reserve();
     if (!s.ok()) return s;
     return check("paged_attention_chunk",
@@ -1387,6 +1388,7 @@ Status B200Backend::prompt_attention_dev(const void *q, const void *k, const voi
     a.v = v;
     a.kv_stride = kv_stride;
     a.err = d_err_;
+    a.device = device_;
     s = attention_reserve();
     if (!s.ok()) return s;
     return check("prompt_attention",

@@ -293,6 +293,7 @@ struct PrefillLaunch {
     const float *k_scale = nullptr;  // fp8 pools: [kv_heads] scales of this layer
     const float *v_scale = nullptr;
     DevError *err;
+    int device;
 };
 
 int num_sms(int device);

@@ -47,6 +47,7 @@
 #include <cuda_runtime.h>
 
 #include <algorithm>
+#include <atomic>
 #include <cfloat>
 #include <cstdint>
 #include <type_traits>
@@ -1357,9 +1358,16 @@ cudaError_t launch_tiles(const PrefillLaunch &a, const PrefillWorkspace &ws, int
     p.headers = reinterpret_cast<Header *>(at);
     const int ctas = std::min(sms, ws.ctas);
     auto kern = prefill_attention_kernel<T, D, SRC>;
-    cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, G::kSmem);
-    if (e != cudaSuccess) return e;
+    // Once per kernel and device.
+    static std::atomic<unsigned long long> prepared{0};
+    cudaError_t e;
+    if (a.device >= 64 || !((prepared.load() >> a.device) & 1)) {
+        if ((e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, G::kSmem)) != cudaSuccess) return e;
+        if (a.device < 64) prepared |= 1ull << a.device;
+    }
     if ((e = launch_pdl(kern, dim3((unsigned)ctas), dim3(kPrefillThreads), G::kSmem, st, tq, tk, tv, p)) != cudaSuccess) return e;
+    // Items of fewer tiles than two snaps are never split.
+    if (a.max_len <= (2 * std::min(kSnapRows, kSnapKeys) - 1) * G::kKeys) return cudaSuccess;
     return launch_pdl(prefill_join_kernel<T, D, G::kRowTiles>, dim3((unsigned)ctas, G::kRowTiles * (D / 32)), dim3(128), 0, st, p, ctas);
 }
 

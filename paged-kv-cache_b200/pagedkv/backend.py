@@ -354,34 +354,40 @@ class B200Backend:
         [head_dim] or None, k and v [T][kv heads][head_dim] with rows of any
         pitch; cos_sin f32 [positions][rotary_dim] (see pagedkv.rope_table);
         q_out None rotates q in place, k_out (rows like k) is optional."""
-        s = ctx_lens.shape[0]
-        stride = block_tables.shape[1] if block_tables.dim() == 2 else 0
-        tag = _torch_tag(k)
-        _same_layout(k, v)
-        rows = [x for x in (q, q_out, k, k_out) if x is not None]
-        for x in rows:
-            _head_rows(x)
-            if x.dtype != k.dtype:
-                raise ValueError("q, k, v and their outputs must share a dtype")
-            if x.shape[0] < num_tokens:
-                raise ValueError("num_tokens exceeds the rows")
-        if k.shape[1] * k.shape[2] != self.shard_entry_elems or k.shape[2] != self._cfg.head_dim:
+        tag = _tag(k)
+        t, hkv, d = _head_rows(k)
+        pitch = k.stride(0)
+        if v.shape != k.shape or v.stride(0) != pitch or v.dtype is not k.dtype or _head_rows(v)[0] != t:
+            raise ValueError("k and v must share shape, strides and dtype")
+        if hkv * d != self.shard_entry_elems or d != self._cfg.head_dim:
             raise ValueError("k and v must hold the kv heads of this backend")
-        if q_out is not None and (q is None or q_out.shape != q.shape):
-            raise ValueError("q_out must have the shape of q")
-        if k_out is not None and k_out.shape != k.shape:
-            raise ValueError("k_out must have the shape of k")
-        if q is not None and q.shape[2] != k.shape[2]:
-            raise ValueError("q and k must share head_dim")
-        if cos_sin.dim() != 2 or not cos_sin.is_contiguous() or cos_sin.dtype.itemsize != 4 or not cos_sin.is_floating_point():
+        hq = q_pitch = qo_pitch = ko_pitch = 0
+        if q is not None:
+            rows, hq, dq = _head_rows(q)
+            if dq != d or rows < num_tokens or q.dtype is not k.dtype:
+                raise ValueError("q must hold num_tokens rows of k's head_dim and dtype")
+            q_pitch = q.stride(0)
+        if q_out is not None:
+            if q is None or q_out.shape != q.shape or q_out.dtype is not q.dtype:
+                raise ValueError("q_out must have the shape and dtype of q")
+            _head_rows(q_out)
+            qo_pitch = q_out.stride(0)
+        if k_out is not None:
+            if k_out.shape != k.shape or k_out.dtype is not k.dtype:
+                raise ValueError("k_out must have the shape and dtype of k")
+            _head_rows(k_out)
+            ko_pitch = k_out.stride(0)
+        if t < num_tokens:
+            raise ValueError("num_tokens exceeds the rows")
+        if (cos_sin.dim() != 2 or cos_sin.dtype.itemsize != 4 or not cos_sin.is_floating_point()
+                or not cos_sin.is_contiguous()):
             raise ValueError("cos_sin must be a dense f32 [positions][rotary_dim] tensor")
+        positions, rotary = cos_sin.shape
         _check(lib.pkv_rope_and_cache_dev(
-            self._h, _ptr(block_tables), stride, _ptr(ctx_lens), _ptr(new_lens), s, num_tokens,
-            _ptr(cu_out), _ptr(slots_out), layer, _ptr(q), 0 if q is None else q.stride(0),
-            0 if q is None else q.shape[1], _ptr(q_out), 0 if q_out is None else q_out.stride(0),
-            _ptr(k), _ptr(v), k.stride(0), _ptr(k_out), 0 if k_out is None else k_out.stride(0),
-            tag, _ptr(cos_sin), cos_sin.shape[0], cos_sin.shape[1], int(interleaved),
-            _stream_ptr(stream)))
+            self._h, _ptr(block_tables), _table_stride(block_tables), _ptr(ctx_lens), _ptr(new_lens),
+            len(ctx_lens), num_tokens, _ptr(cu_out), _ptr(slots_out), layer, _ptr(q), q_pitch, hq,
+            _ptr(q_out), qo_pitch, k.data_ptr(), v.data_ptr(), pitch, _ptr(k_out), ko_pitch, tag,
+            _ptr(cos_sin), positions, rotary, int(interleaved), self._stream(stream)))
 
     def paged_attention_chunk(self, q, cu_seqlens, block_tables, ctx_lens, max_new_len: int,
                               max_context_len: int, out, layer: int,
@@ -394,11 +400,10 @@ class B200Backend:
         _dense_out(q, out)
         if softmax_scale is None:
             softmax_scale = d ** -0.5
-        stride = block_tables.shape[1] if block_tables.dim() == 2 else 0
         _check(lib.pkv_paged_attention_chunk_dev(
-            self._h, layer, _ptr(q), _torch_tag(q), q.stride(0), hq, _ptr(cu_seqlens),
-            ctx_lens.shape[0], t, max_new_len, _ptr(block_tables), stride, _ptr(ctx_lens),
-            max_context_len, float(softmax_scale), _ptr(out), _ptr(lse), _stream_ptr(stream)))
+            self._h, layer, q.data_ptr(), _tag(q), q.stride(0), hq, _ptr(cu_seqlens), len(ctx_lens), t,
+            max_new_len, _ptr(block_tables), _table_stride(block_tables), _ptr(ctx_lens),
+            max_context_len, softmax_scale, out.data_ptr(), _ptr(lse), self._stream(stream)))
 
     def prompt_attention(self, q, k, v, cu_seqlens, max_len: int, out,
                          softmax_scale: float | None = None, lse=None, stream=None) -> None:
@@ -408,15 +413,25 @@ class B200Backend:
         cu_seqlens[s + 1], lse optional f32 [T][num_q_heads]."""
         t, hq, d = _head_rows(q)
         _dense_out(q, out)
-        _same_layout(k, v)
-        if _head_rows(k) != (t, self.shard_entry_elems // self._cfg.head_dim, d) or k.dtype != q.dtype:
+        pitch = k.stride(0)
+        if (_head_rows(k) != (t, self.shard_entry_elems // self._cfg.head_dim, d) or k.dtype is not q.dtype
+                or d != self._cfg.head_dim):
             raise ValueError("k and v must hold q's rows, the kv heads of this backend, q's dtype")
+        if v.shape != k.shape or v.stride(0) != pitch or v.dtype is not k.dtype or _head_rows(v)[0] != t:
+            raise ValueError("k and v must share shape, strides and dtype")
         if softmax_scale is None:
             softmax_scale = d ** -0.5
         _check(lib.pkv_prompt_attention_dev(
-            self._h, _ptr(q), _ptr(k), _ptr(v), _torch_tag(q), q.stride(0), k.stride(0), hq,
-            _ptr(cu_seqlens), cu_seqlens.shape[0] - 1, t, max_len, float(softmax_scale), _ptr(out),
-            _ptr(lse), _stream_ptr(stream)))
+            self._h, q.data_ptr(), k.data_ptr(), v.data_ptr(), _tag(q), q.stride(0), pitch, hq,
+            _ptr(cu_seqlens), len(cu_seqlens) - 1, t, max_len, softmax_scale, out.data_ptr(),
+            _ptr(lse), self._stream(stream)))
+
+    def _stream(self, stream) -> int | None:
+        """cudaStream_t: the current stream of this backend's device by default
+        (whatever the current device is)."""
+        if stream is None:
+            return _current_stream(self.device) or None
+        return stream if isinstance(stream, int) else stream.cuda_stream
 
     def attention_reserve(self) -> None:
         """Allocates the workspace of paged_attention_chunk and prompt_attention
@@ -498,11 +513,40 @@ def _same_layout(k, v) -> None:
 def _head_rows(x) -> tuple[int, int, int]:
     """(rows, heads, head_dim) of a [rows][heads][head_dim] tensor whose rows
     are dense and may lie at any pitch."""
-    if x.dim() != 3 or x.stride(2) != 1 or (x.shape[1] > 1 and x.stride(1) != x.shape[2]):
+    shape, stride = x.shape, x.stride()
+    if len(shape) != 3 or stride[2] != 1 or (stride[1] != shape[2] and shape[1] > 1):
         raise ValueError("rows must be contiguous [heads][head_dim]")
-    return tuple(x.shape)
+    return shape[0], shape[1], shape[2]
+
+
+# Dtype tags, and torch's call for a device's current stream: looked up once,
+# since a step's small calls are bound by the host.
+_TAGS: dict = {}
+_raw_stream = None
+
+
+def _tag(x) -> int:
+    tag = _TAGS.get(x.dtype)
+    if tag is None:
+        tag = _TAGS[x.dtype] = _torch_tag(x)
+    return tag
+
+
+def _current_stream(device: int) -> int:
+    global _raw_stream
+    if _raw_stream is None:
+        import torch
+
+        _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
+            lambda d: torch.cuda.current_stream(d).cuda_stream)
+    return _raw_stream(device)
+
+
+def _table_stride(t) -> int:
+    shape = t.shape
+    return shape[1] if len(shape) == 2 else 0
 
 
 def _dense_out(q, out) -> None:
-    if out.shape != q.shape or out.dtype != q.dtype or not out.is_contiguous():
+    if out.shape != q.shape or out.dtype is not q.dtype or not out.is_contiguous():
         raise ValueError("out must be dense, with the shape and dtype of q")
