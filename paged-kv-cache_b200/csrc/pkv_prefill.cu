@@ -113,9 +113,15 @@ struct Geom {
     static_assert(kOCol + kRowTiles * D <= 512, "tensor memory");
 };
 
-// Costs, in key-tile units of 1/128: a tile costs its keys times the row
-// tiles, an item kItemCost more (queries in, outputs out).
-constexpr int kItemCost = 256;
+// Costs, as measured (a row tile pair and 128 keys: 3,700 cycles): a key costs a
+// row item kRowCost, a key item kKeyCost (one row tile, but its K and V come as
+// slowly; over fp8 they are also converted), and an item kItemCost more (queries
+// in, outputs out: 10,000 cycles).
+template <int ROW_TILES, bool FP8>
+struct Rates {
+    static constexpr int kRowCost = 8, kKeyCost = ROW_TILES == 1 ? 8 : FP8 ? 7 : 5;
+    static constexpr int kItemCost = ROW_TILES == 1 ? 3400 : 2600;
+};
 // Shares do not begin or end closer than this many key tiles to an item's
 // ends: the join costs about as much.
 constexpr int kSnapRows = 3, kSnapKeys = 4;
@@ -173,8 +179,9 @@ __device__ __forceinline__ Seq sequence(const PrefillLaunch &a, int s, bool repo
 
 // The cost of the items of a sequence. Items 0 .. items - 2 are full; item i
 // ends at key ctx + min((i + 1) * per, rows).
-template <int ROW_TILES>
+template <int ROW_TILES, bool FP8>
 struct Costs {
+    using R = Rates<ROW_TILES, FP8>;
     long long ctx, per, rows, last;
     int items;
     bool empty;
@@ -185,12 +192,12 @@ struct Costs {
         empty = q.empty;
         items = q.rows > 0 ? (q.rows - 1) / (ROW_TILES * tile_tokens) + 1 : 0;
         const bool two = ROW_TILES == 2 && rows - (items - 1) * per > tile_tokens;
-        last = empty ? kItemCost : (two ? 2 : 1) * (ctx + rows) + kItemCost;
+        last = R::kItemCost + (empty ? 0 : (two ? R::kRowCost : R::kKeyCost) * (ctx + rows));
     }
     // Cost of items 0 .. i - 1, i < items (all full).
     __device__ __forceinline__ long long before(long long i) const {
-        if (empty) return i * kItemCost;
-        return i * (ROW_TILES * ctx + kItemCost) + ROW_TILES * per * (i * (i + 1) / 2);
+        if (empty) return i * R::kItemCost;
+        return i * (R::kRowCost * ctx + R::kItemCost) + R::kRowCost * per * (i * (i + 1) / 2);
     }
     __device__ __forceinline__ long long head() const { return items ? before(items - 1) + last : 0; }
     __device__ __forceinline__ long long of(long long i) const { return i + 1 < items ? before(i + 1) - before(i) : last; }
@@ -202,8 +209,8 @@ struct Pos {
 
 // The place of cost x within sequence s. Rounded to a key tile; within kSnap
 // tiles of an item's ends, to that end.
-template <int ROW_TILES, int KEYS>
-__device__ __forceinline__ Pos locate(const Costs<ROW_TILES> &c, int s, long long x, int tile_tokens) {
+template <int ROW_TILES, int KEYS, bool FP8>
+__device__ __forceinline__ Pos locate(const Costs<ROW_TILES, FP8> &c, int s, long long x, int tile_tokens) {
     const long long head = c.head();
     const int h = (int)(x / head);
     long long r = x - h * head;
@@ -304,7 +311,7 @@ prefill_attention_kernel(const __grid_constant__ CUtensorMap tq, const __grid_co
         const int b0 = min(a.num_seqs, tid * seg), b1 = min(a.num_seqs, b0 + seg);
         long long local = 0;
         for (int s = b0; s < b1; ++s) {
-            const Costs<NT> c(sequence(a, s, blockIdx.x == 0), p.tile_tokens);
+            const Costs<NT, G::kFp8> c(sequence(a, s, blockIdx.x == 0), p.tile_tokens);
             local += c.head() * a.kv_heads;
         }
         long long incl = local;
@@ -329,10 +336,10 @@ prefill_attention_kernel(const __grid_constant__ CUtensorMap tq, const __grid_co
             if (b < n && x >= first && x < first + local) {
                 long long at = first;
                 for (int s = b0; s < b1; ++s) {
-                    const Costs<NT> c(sequence(a, s, false), p.tile_tokens);
+                    const Costs<NT, G::kFp8> c(sequence(a, s, false), p.tile_tokens);
                     const long long w = c.head() * a.kv_heads;
                     if (x < at + w) {
-                        s_range[e] = locate<NT, KEYS>(c, s, x - at, p.tile_tokens);
+                        s_range[e] = locate<NT, KEYS, G::kFp8>(c, s, x - at, p.tile_tokens);
                         break;
                     }
                     at += w;
