@@ -120,14 +120,14 @@ struct Geom {
 template <int ROW_TILES, bool FP8>
 struct Rates {
     static constexpr int kRowCost = 8, kKeyCost = ROW_TILES == 1 ? 8 : FP8 ? 7 : 5;
-    static constexpr int kItemCost = ROW_TILES == 1 ? 3400 : 2600;
+    static constexpr int kItemCost = ROW_TILES == 1 ? 3400 : FP8 ? 4000 : 2600;
 };
 // Shares do not begin or end closer than this many key tiles to an item's
 // ends: the join costs about as much.
-constexpr int kSnapRows = 3, kSnapKeys = 4;
+constexpr int kSnapRows = 3, kSnapKeys = 2;
 
 struct Header {          // of a partial slot
-    int valid, last;     // last: the piece reaches the item's last key
+    int state, pad0;     // 0: none; 1: a piece; 2: the piece reaches the item's last key
     int row0, tokens;    // packed row of the item's first token; its tokens
     int head, two;       // kv head; two row tiles
     int pad[2];
@@ -211,15 +211,23 @@ struct Pos {
 // tiles of an item's ends, to that end.
 template <int ROW_TILES, int KEYS, bool FP8>
 __device__ __forceinline__ Pos locate(const Costs<ROW_TILES, FP8> &c, int s, long long x, int tile_tokens) {
+    // Quotients and the quadratic by 64-bit floats, then put right: integer
+    // division takes longer than the rest of the search.
     const long long head = c.head();
-    const int h = (int)(x / head);
+    int h = (int)((double)x / (double)head);
+    if (h * head > x) --h;
+    if ((h + 1) * head <= x) ++h;
     long long r = x - h * head;
-    long long lo = 0, hi = c.items - 1;
-    while (lo < hi) {
-        const long long mid = (lo + hi + 1) >> 1;
-        if (c.before(mid) <= r) lo = mid;
-        else hi = mid - 1;
+    long long lo;  // the last item with before(lo) <= r
+    if (c.empty) {
+        lo = r / Costs<ROW_TILES, FP8>::R::kItemCost;
+    } else {
+        const double qa = 0.5 * (double)Rates<ROW_TILES, FP8>::kRowCost * (double)c.per, qb = (double)(c.before(1)) - qa;
+        lo = (long long)((sqrt(qb * qb + 4.0 * qa * (double)r) - qb) / (2.0 * qa));
     }
+    lo = max(0ll, min(lo, (long long)c.items - 1));
+    while (lo > 0 && c.before(lo) > r) --lo;
+    while (lo + 1 < c.items && c.before(lo + 1) <= r) ++lo;
     r -= c.before(lo);
     const long long end = c.ctx + min((lo + 1) * c.per, c.rows);
     const int tiles = c.empty ? 0 : (int)((end + KEYS - 1) / KEYS);
@@ -305,13 +313,16 @@ prefill_attention_kernel(const __grid_constant__ CUtensorMap tq, const __grid_co
 
     // ---- this CTA's share ----
     {
-        if (tid < 2) p.headers[2 * blockIdx.x + tid].valid = 0;
+        if (tid < 2) p.headers[2 * blockIdx.x + tid].state = 0;
         if (tid == 0) s_range[0] = s_range[1] = Pos{a.num_seqs, 0, 0, 0};
         const int seg = (a.num_seqs + kPrefillThreads - 1) / kPrefillThreads;
         const int b0 = min(a.num_seqs, tid * seg), b1 = min(a.num_seqs, b0 + seg);
         long long local = 0;
+        Seq mine{0, 0, 0, false};  // the first of this thread's sequences: most often the only one
         for (int s = b0; s < b1; ++s) {
-            const Costs<NT, G::kFp8> c(sequence(a, s, blockIdx.x == 0), p.tile_tokens);
+            const Seq q = sequence(a, s, blockIdx.x == 0);
+            if (s == b0) mine = q;
+            const Costs<NT, G::kFp8> c(q, p.tile_tokens);
             local += c.head() * a.kv_heads;
         }
         long long incl = local;
@@ -332,11 +343,11 @@ prefill_attention_kernel(const __grid_constant__ CUtensorMap tq, const __grid_co
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
             const long long b = blockIdx.x + e;
-            const long long x = total / n * b + total % n * b / n;
+            const long long x = (long long)((double)total * ((double)b / (double)n));
             if (b < n && x >= first && x < first + local) {
                 long long at = first;
                 for (int s = b0; s < b1; ++s) {
-                    const Costs<NT, G::kFp8> c(sequence(a, s, false), p.tile_tokens);
+                    const Costs<NT, G::kFp8> c(s == b0 ? mine : sequence(a, s, false), p.tile_tokens);
                     const long long w = c.head() * a.kv_heads;
                     if (x < at + w) {
                         s_range[e] = locate<NT, KEYS, G::kFp8>(c, s, x - at, p.tile_tokens);
@@ -675,7 +686,7 @@ prefill_attention_kernel(const __grid_constant__ CUtensorMap tq, const __grid_co
                 }
             }
             if (it.slot >= 0 && tid == 0) {
-                Header h{1, it.t1 == it.tiles, it.row0, it.tokens, it.head, two, {0, 0}};
+                Header h{it.t1 == it.tiles ? 2 : 1, 0, it.row0, it.tokens, it.head, two, {0, 0}};
                 p.headers[it.slot] = h;
             }
             fence_before();
@@ -1119,33 +1130,41 @@ prefill_attention_kernel(const __grid_constant__ CUtensorMap tq, const __grid_co
                 }
             } else {
                 if (kScaleQ && n > 0) {
-                    // A thread to a row; its factor is kept per item (the softmax
-                    // of the last item may still read the other).
+                    // A row's factor is kept per item (the softmax of the last item may
+                    // still read the other).
                     ok = together(wait(&q_raw, qn & 1));
                     if (!ok) break;
-                    for (int r = t128; r < (it.two ? 256 : 128); r += kT) {
-                        unsigned char *q = sq + (r >> 7) * G::kQTile + (r & 127) * 128;
-                        float top = 0.f;
-#pragma unroll 4
-                        for (int c = 0; c < D / 8; ++c) {
-                            const uint4 x = *reinterpret_cast<const uint4 *>(q + (c >> 3) * (128 * 128) + (c & 7) * 16);
-                            const __nv_bfloat162 *e = reinterpret_cast<const __nv_bfloat162 *>(&x);
-                            const __nv_bfloat162 y = __hmax2(__hmax2(__habs2(e[0]), __habs2(e[1])), __hmax2(__habs2(e[2]), __habs2(e[3])));
-                            top = fmaxf(top, fmaxf(__low2float(y), __high2float(y)));
-                        }
-                        int ex = 14;
-                        if (top > 0.f && top < INFINITY) frexpf(top, &ex);
-                        const float up = ldexpf(1.f, 14 - ex);
-                        q_factor[(qn & 1) * 256 + r] = ldexpf(1.f, ex - 14);
-#pragma unroll 4
-                        for (int c = 0; c < D / 8; ++c) {
-                            uint4 *at = reinterpret_cast<uint4 *>(q + (c >> 3) * (128 * 128) + (c & 7) * 16);
-                            const uint4 x = *at;
-                            const __nv_bfloat162 *e = reinterpret_cast<const __nv_bfloat162 *>(&x);
-                            uint32_t y[4];
+                    // 8 lanes to a row, a 16-byte chunk of each slab to a lane.
+                    for (int r0 = t128 >> 3; r0 < (it.two ? 256 : 128); r0 += 2 * (kT / 8)) {
 #pragma unroll
-                            for (int k = 0; k < 4; ++k) y[k] = pack2<__half>(__low2float(e[k]) * up, __high2float(e[k]) * up);
-                            *at = make_uint4(y[0], y[1], y[2], y[3]);
+                        for (int k = 0; k < 2; ++k) {
+                            const int r = r0 + k * (kT / 8);
+                            uint4 *q = reinterpret_cast<uint4 *>(sq + (r >> 7) * G::kQTile + (r & 127) * 128 + (lane & 7) * 16);
+                            uint4 x[G::kSlabs];
+                            __nv_bfloat162 most = __floats2bfloat162_rn(0.f, 0.f);
+#pragma unroll
+                            for (int c = 0; c < G::kSlabs; ++c) {
+                                x[c] = q[c * (128 * 128 / 16)];
+                                const __nv_bfloat162 *e = reinterpret_cast<const __nv_bfloat162 *>(&x[c]);
+                                most = __hmax2(most, __hmax2(__hmax2(__habs2(e[0]), __habs2(e[1])), __hmax2(__habs2(e[2]), __habs2(e[3]))));
+                            }
+                            float top = fmaxf(__low2float(most), __high2float(most));
+#pragma unroll
+                            for (int o = 4; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+                            // top = 2^ex * [1, 2); rows of zeros, tiny or infinite ones: as they are or nearly.
+                            int ex = (int)(__float_as_uint(top) >> 23) - 127;
+                            if (ex > 127) ex = 13;
+                            ex = max(ex, -100);
+                            const float up = __uint_as_float((unsigned)(13 - ex + 127) << 23);
+                            if ((lane & 7) == 0) q_factor[(qn & 1) * 256 + r] = __uint_as_float((unsigned)(ex - 13 + 127) << 23);
+#pragma unroll
+                            for (int c = 0; c < G::kSlabs; ++c) {
+                                const __nv_bfloat162 *e = reinterpret_cast<const __nv_bfloat162 *>(&x[c]);
+                                uint32_t y[4];
+#pragma unroll
+                                for (int i = 0; i < 4; ++i) y[i] = pack2<__half>(__low2float(e[i]) * up, __high2float(e[i]) * up);
+                                q[c * (128 * 128 / 16)] = make_uint4(y[0], y[1], y[2], y[3]);
+                            }
                         }
                     }
                     ++qn;
@@ -1228,26 +1247,26 @@ prefill_attention_kernel(const __grid_constant__ CUtensorMap tq, const __grid_co
 
 // Joins the partials of one split item, from the CTA whose share the item
 // begins in on: out = sum_i 2^(m_i - M) O_i / sum_i 2^(m_i - M) l_i, in the
-// order of the keys. A thread takes a row and 32 of its elements; a warp's
+// order of the keys. A thread takes a row and 16 of its elements; a warp's
 // loads are contiguous.
+constexpr int kJoinElems = 16;
 template <typename T, int D, int ROW_TILES>
 __global__ void __launch_bounds__(128) prefill_join_kernel(const __grid_constant__ Params p, int ctas) {
     __shared__ int s_slot[512];
     __shared__ int s_count;
     pdl_wait();
     const PrefillLaunch &a = p.a;
-    const int b = blockIdx.x, w = blockIdx.y / (D / 32), c = blockIdx.y % (D / 32) * 32;
+    const int b = blockIdx.x, w = blockIdx.y / (D / kJoinElems), c = blockIdx.y % (D / kJoinElems) * kJoinElems;
     const Header h = p.headers[2 * b + 1];
-    if (!h.valid || (w && !h.two)) return;
+    if (!h.state || (w && !h.two)) return;
     const int lane = threadIdx.x & 31;
     if (threadIdx.x < 32) {  // the later pieces: up to the one that ends the item
         int n = 0;
         for (int i0 = b + 1; i0 < ctas; i0 += 32) {
             const int i = i0 + lane;
-            int valid = 0, last = 0;
-            if (i < ctas) valid = p.headers[2 * i].valid, last = valid && p.headers[2 * i].last;
-            unsigned some = __ballot_sync(0xffffffffu, valid);
-            const unsigned end = __ballot_sync(0xffffffffu, last);
+            const int state = i < ctas ? p.headers[2 * i].state : 0;
+            unsigned some = __ballot_sync(0xffffffffu, state);
+            const unsigned end = __ballot_sync(0xffffffffu, state == 2);
             if (end) some &= (2u << (__ffs(end) - 1)) - 1;
             if ((some >> lane) & 1u) s_slot[n + __popc(some & ((1u << lane) - 1))] = 2 * i;
             n += __popc(some);
@@ -1261,12 +1280,12 @@ __global__ void __launch_bounds__(128) prefill_join_kernel(const __grid_constant
     const int count = s_count + 1;
     auto slot = [&](int i) { return (long long)(i == 0 ? 2 * b + 1 : s_slot[i - 1]) * ROW_TILES + w; };
     float M = -INFINITY;
-#pragma unroll 4
+#pragma unroll 8
     for (int i = 0; i < count; ++i) M = fmaxf(M, p.part_ml[slot(i) * 128 + row].x);
-    float L = 0.f, acc[32];
+    float L = 0.f, acc[kJoinElems];
 #pragma unroll
-    for (int e = 0; e < 32; ++e) acc[e] = 0.f;
-#pragma unroll 2
+    for (int e = 0; e < kJoinElems; ++e) acc[e] = 0.f;
+#pragma unroll 4
     for (int i = 0; i < count; ++i) {
         const long long at = slot(i);
         const float2 ml = p.part_ml[at * 128 + row];
@@ -1274,7 +1293,7 @@ __global__ void __launch_bounds__(128) prefill_join_kernel(const __grid_constant
         L = fmaf(ml.y, f, L);
         const float4 *o = p.part_o + (at * (D / 4) + c / 4) * 128 + row;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
+        for (int e = 0; e < kJoinElems / 4; ++e) {
             const float4 x = __ldcs(o + e * 128);
             acc[4 * e] = fmaf(x.x, f, acc[4 * e]);
             acc[4 * e + 1] = fmaf(x.y, f, acc[4 * e + 1]);
@@ -1287,7 +1306,7 @@ __global__ void __launch_bounds__(128) prefill_join_kernel(const __grid_constant
     const long long out_row = (long long)(h.row0 + token) * (a.kv_heads * group) + (long long)h.head * group + (row - tau * group);
     T *out = static_cast<T *>(a.out) + out_row * D + c;
 #pragma unroll
-    for (int e = 0; e < 32; e += 8)
+    for (int e = 0; e < kJoinElems; e += 8)
         *reinterpret_cast<uint4 *>(out + e) =
             make_uint4(pack2<T>(acc[e] * inv, acc[e + 1] * inv), pack2<T>(acc[e + 2] * inv, acc[e + 3] * inv),
                        pack2<T>(acc[e + 4] * inv, acc[e + 5] * inv), pack2<T>(acc[e + 6] * inv, acc[e + 7] * inv));
@@ -1375,7 +1394,7 @@ cudaError_t launch_tiles(const PrefillLaunch &a, const PrefillWorkspace &ws, int
     if ((e = launch_pdl(kern, dim3((unsigned)ctas), dim3(kPrefillThreads), G::kSmem, st, tq, tk, tv, p)) != cudaSuccess) return e;
     // Items of fewer tiles than two snaps are never split.
     if (a.max_len <= (2 * std::min(kSnapRows, kSnapKeys) - 1) * G::kKeys) return cudaSuccess;
-    return launch_pdl(prefill_join_kernel<T, D, G::kRowTiles>, dim3((unsigned)ctas, G::kRowTiles * (D / 32)), dim3(128), 0, st, p, ctas);
+    return launch_pdl(prefill_join_kernel<T, D, G::kRowTiles>, dim3((unsigned)ctas, G::kRowTiles * (D / kJoinElems)), dim3(128), 0, st, p, ctas);
 }
 
 template <typename T, Source SRC>
