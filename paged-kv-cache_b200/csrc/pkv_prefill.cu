@@ -137,6 +137,7 @@ struct Params {
     PrefillLaunch a;
     int tile_tokens;     // tokens per 128-row tile: 128 / group
     int wide;            // out takes 32-byte stores
+    unsigned share;      // 2^32 / ctas
     float4 *part_o;      // [2 * ctas][slot rows / 128][D / 4][128]: a column of rows is contiguous
     float2 *part_ml;     // [2 * ctas][slot rows]: reference point (base 2), sum
     Header *headers;     // [2 * ctas]
@@ -211,19 +212,20 @@ struct Pos {
 // tiles of an item's ends, to that end.
 template <int ROW_TILES, int KEYS, bool FP8>
 __device__ __forceinline__ Pos locate(const Costs<ROW_TILES, FP8> &c, int s, long long x, int tile_tokens) {
-    // Quotients and the quadratic by 64-bit floats, then put right: integer
-    // division takes longer than the rest of the search.
+    // Quotients and the quadratic by 32-bit floats, then put right: 64-bit
+    // division and square root take 3 us here.
     const long long head = c.head();
-    int h = (int)((double)x / (double)head);
-    if (h * head > x) --h;
-    if ((h + 1) * head <= x) ++h;
+    int h = (int)__fdividef((float)x, (float)head);
+    while (h > 0 && h * head > x) --h;
+    while ((h + 1) * head <= x) ++h;
     long long r = x - h * head;
     long long lo;  // the last item with before(lo) <= r
+    const float one = (float)(c.empty ? Rates<ROW_TILES, FP8>::kItemCost : c.before(1));
     if (c.empty) {
-        lo = r / Costs<ROW_TILES, FP8>::R::kItemCost;
+        lo = (long long)__fdividef((float)r, one);
     } else {
-        const double qa = 0.5 * (double)Rates<ROW_TILES, FP8>::kRowCost * (double)c.per, qb = (double)(c.before(1)) - qa;
-        lo = (long long)((sqrt(qb * qb + 4.0 * qa * (double)r) - qb) / (2.0 * qa));
+        const float qa = 0.5f * Rates<ROW_TILES, FP8>::kRowCost * (float)c.per, qb = one - qa;
+        lo = (long long)__fdividef(sqrtf(qb * qb + 4.f * qa * (float)r) - qb, 2.f * qa);
     }
     lo = max(0ll, min(lo, (long long)c.items - 1));
     while (lo > 0 && c.before(lo) > r) --lo;
@@ -233,10 +235,10 @@ __device__ __forceinline__ Pos locate(const Costs<ROW_TILES, FP8> &c, int s, lon
     const int tiles = c.empty ? 0 : (int)((end + KEYS - 1) / KEYS);
     const bool two = ROW_TILES == 2 && (lo + 1 < c.items || c.rows - lo * c.per > tile_tokens);
     const int snap = two ? kSnapRows : kSnapKeys;
-    int t = (int)((double)r / (double)c.of(lo) * tiles + 0.5);
-    if (t < snap && t * 2 <= tiles) t = 0;
-    if (tiles - t < snap) t = tiles;
+    int t = (int)((float)r / (float)c.of(lo) * (float)tiles + 0.5f);
     if (tiles < 2 * snap) t = 2 * t < tiles ? 0 : tiles;
+    else if (t < snap) t = 0;
+    else if (tiles - t < snap) t = tiles;
     Pos p{s, h, (int)lo, t};
     if (t == tiles && (tiles > 0 || r > 0)) {  // the item's end is the next one's beginning
         p.t = 0;
@@ -280,6 +282,7 @@ prefill_attention_kernel(const __grid_constant__ CUtensorMap tq, const __grid_co
     __shared__ unsigned s_flag[kItemRing][kFlagWords + 1];
     __shared__ unsigned char s_mask[kMaskRing];
     __shared__ Pos s_range[2];
+    __shared__ Seq s_first;  // the share's first sequence
     __shared__ uint32_t s_tmem;
     __shared__ volatile int s_failed;
 
@@ -314,7 +317,7 @@ prefill_attention_kernel(const __grid_constant__ CUtensorMap tq, const __grid_co
     // ---- this CTA's share ----
     {
         if (tid < 2) p.headers[2 * blockIdx.x + tid].state = 0;
-        if (tid == 0) s_range[0] = s_range[1] = Pos{a.num_seqs, 0, 0, 0};
+        if (tid == 0) s_range[0] = s_range[1] = Pos{a.num_seqs, 0, 0, 0};  // no work
         const int seg = (a.num_seqs + kPrefillThreads - 1) / kPrefillThreads;
         const int b0 = min(a.num_seqs, tid * seg), b1 = min(a.num_seqs, b0 + seg);
         long long local = 0;
@@ -340,16 +343,20 @@ prefill_attention_kernel(const __grid_constant__ CUtensorMap tq, const __grid_co
             total += s_scan[w];
         }
         const long long first = add + incl - local, n = gridDim.x;
-#pragma unroll
+#pragma unroll 1  // run once, from a cold instruction cache: the shorter the better
         for (int e = 0; e < 2; ++e) {
             const long long b = blockIdx.x + e;
-            const long long x = (long long)((double)total * ((double)b / (double)n));
+            // total * b / n, by b times n's reciprocal in 32 fraction bits.
+            const unsigned long long part = (unsigned long long)b * p.share;
+            const long long x = (long long)((__umul64hi(total, part) << 32) | ((unsigned long long)total * part >> 32));
             if (b < n && x >= first && x < first + local) {
                 long long at = first;
                 for (int s = b0; s < b1; ++s) {
-                    const Costs<NT, G::kFp8> c(s == b0 ? mine : sequence(a, s, false), p.tile_tokens);
+                    const Seq q = s == b0 ? mine : sequence(a, s, false);
+                    const Costs<NT, G::kFp8> c(q, p.tile_tokens);
                     const long long w = c.head() * a.kv_heads;
                     if (x < at + w) {
+                        if (e == 0) s_first = q;
                         s_range[e] = locate<NT, KEYS, G::kFp8>(c, s, x - at, p.tile_tokens);
                         break;
                     }
@@ -357,7 +364,6 @@ prefill_attention_kernel(const __grid_constant__ CUtensorMap tq, const __grid_co
                 }
             }
         }
-        if (blockIdx.x == 0 && tid == 0) s_range[0] = Pos{0, 0, 0, 0};
     }
     if (tid == 0) {
         for (int i = 0; i < kItemRing; ++i) s_flag[i][kFlagWords] = 0;
@@ -961,6 +967,7 @@ prefill_attention_kernel(const __grid_constant__ CUtensorMap tq, const __grid_co
         // ================= items, and Q by TMA =================
         Pos at = s_range[0];
         const Pos end = s_range[1];
+        bool fresh = true;
         unsigned qn = 0;
         bool ok = true;
         auto publish = [&](const Item &it) -> bool {
@@ -981,7 +988,12 @@ prefill_attention_kernel(const __grid_constant__ CUtensorMap tq, const __grid_co
             // The next sequence with rows, from at.s on: 32 at a time.
             const int s = at.s + lane;
             Seq q{0, 0, 0, false};
-            if (s < a.num_seqs) q = sequence(a, s, false);
+            if (fresh) {
+                if (lane == 0) q = s_first;
+                fresh = false;
+            } else if (s < a.num_seqs) {
+                q = sequence(a, s, false);
+            }
             const unsigned some = __ballot_sync(0xffffffffu, q.rows > 0);
             if (!some) {
                 at = Pos{at.s + 32, 0, 0, 0};
@@ -1375,14 +1387,14 @@ cudaError_t launch_tiles(const PrefillLaunch &a, const PrefillWorkspace &ws, int
         ok = map_pages(&tk, t, a.k, entry, a.pool_rows, D / 64) && map_pages(&tv, t, a.v, entry, a.pool_rows, D / 64);
     }
     if (!ok) return cudaErrorInvalidValue;
-    Params p{a, tile_tokens, aligned(a.out, 32), nullptr, nullptr, nullptr};
+    const int ctas = std::min(sms, ws.ctas);
+    Params p{a, tile_tokens, aligned(a.out, 32), (unsigned)((1ull << 32) / ctas), nullptr, nullptr, nullptr};
     unsigned char *at = static_cast<unsigned char *>(ws.base);
     p.part_o = reinterpret_cast<float4 *>(at);
     at += (size_t)2 * ws.ctas * G::kSlotRows * D * sizeof(float);
     p.part_ml = reinterpret_cast<float2 *>(at);
     at += (size_t)2 * ws.ctas * G::kSlotRows * sizeof(float2);
     p.headers = reinterpret_cast<Header *>(at);
-    const int ctas = std::min(sms, ws.ctas);
     auto kern = prefill_attention_kernel<T, D, SRC>;
     // Once per kernel and device.
     static std::atomic<unsigned long long> prepared{0};
