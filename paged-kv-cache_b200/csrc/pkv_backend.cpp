@@ -1264,6 +1264,17 @@ Status B200Backend::check_prefill(const char *what, const void *q, int64_t num_q
     return Status::Ok();
 }
 
+// The prefill workspace, made on first use, but not under a stream capture.
+Status B200Backend::prefill_workspace(cudaStream_t st) {
+    if (d_prefill_ws_) return Status::Ok();
+    cudaStreamCaptureStatus capturing = cudaStreamCaptureStatusNone;
+    if (cudaStreamIsCapturing(st, &capturing) == cudaSuccess && capturing != cudaStreamCaptureStatusNone)
+        return error(PKV_ERR_DEVICE, 0, 0,
+                     "the prefill workspace is not allocated: call pkv_attention_reserve (or run one call) "
+                     "before capturing");
+    return attention_reserve();
+}
+
 Status B200Backend::attention_reserve() {
     const uint64_t hd = cfg_.head_dim;
     if (hd != 64 && hd != 128 && hd != 256)
@@ -1341,7 +1352,7 @@ Status B200Backend::attention_chunk_dev(int64_t layer, const void *q, DType quer
     }
     a.err = d_err_;
     a.device = device_;
-    s = attention_reserve();
+    s = prefill_workspace(st);
     if (!s.ok()) return s;
     return check("paged_attention_chunk",
                  launch_prefill_attention(a, query, dtype_, {d_prefill_ws_, sms_}, sms_, st));
@@ -1389,7 +1400,7 @@ Status B200Backend::prompt_attention_dev(const void *q, const void *k, const voi
     a.kv_stride = kv_stride;
     a.err = d_err_;
     a.device = device_;
-    s = attention_reserve();
+    s = prefill_workspace(st);
     if (!s.ok()) return s;
     return check("prompt_attention",
                  launch_prefill_attention(a, dtype, dtype, {d_prefill_ws_, sms_}, sms_, st));

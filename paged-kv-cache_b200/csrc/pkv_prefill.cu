@@ -483,9 +483,11 @@ prefill_attention_kernel(const __grid_constant__ CUtensorMap tq, const __grid_co
                     // (Rows of no token hold whatever Q's shared memory held: never.)
                     const bool grew = live && !(mt <= m + kLazy);
                     if (__any_sync(0xffffffffu, grew)) {
-                        float mn = max_nan(m, mt);
+                        // Only the rows that need it move: a row's result does not hang on
+                        // the rows beside it.
+                        float mn = grew ? max_nan(m, mt) : m;
                         if (mn == INFINITY) mn = NAN;
-                        const float corr = m == -INFINITY ? 0.f : ex2(m - mn);
+                        const float corr = !grew ? 1.f : m == -INFINITY ? 0.f : ex2(m - mn);
                         l *= corr;
                         m = mn;
                         if (i > 0) {
