@@ -76,8 +76,11 @@ static_assert(2 * (kSoftmaxRegs + kOtherRegs) * 128 <= 128 * kPrefillThreads, "r
 // relative precision, and most tiles skip the rescale of O.
 constexpr float kLazy = 8.0f;
 // One pair of weights in this many is computed on the FMA units, the others by
-// the special-function unit, whose rate (16 a clock) bounds the softmax.
-constexpr int kPolyEvery = 4;
+// the special-function unit. More would relieve the unit (16 results a clock)
+// but the warps are bound by issue: with every 2nd, 4th, 8th and no pair 2,048
+// rows over 32 k keys took 967, 943, 919 and 930 us, and 1,650 rows over fp8,
+// where the conversions take issue slots too, 220, 212, 202 and 191 us.
+constexpr int kPolyEvery = 8;
 
 enum Source { kPaged = 0, kPagedFp8 = 1, kRows = 2 };
 
@@ -137,7 +140,7 @@ struct Params {
     PrefillLaunch a;
     int tile_tokens;     // tokens per 128-row tile: 128 / group
     int wide;            // out takes 32-byte stores
-    unsigned share;      // 2^32 / ctas
+    double share;        // 1 / ctas
     float4 *part_o;      // [2 * ctas][slot rows / 128][D / 4][128]: a column of rows is contiguous
     float2 *part_ml;     // [2 * ctas][slot rows]: reference point (base 2), sum
     Header *headers;     // [2 * ctas]
@@ -180,28 +183,32 @@ __device__ __forceinline__ Seq sequence(const PrefillLaunch &a, int s, bool repo
 
 // The cost of the items of a sequence. Items 0 .. items - 2 are full; item i
 // ends at key ctx + min((i + 1) * per, rows).
+// Held in f64: whole numbers far below 2^53, in fewer instructions than 64-bit
+// integers take (this code runs once a launch, from a cold instruction cache).
 template <int ROW_TILES, bool FP8>
 struct Costs {
     using R = Rates<ROW_TILES, FP8>;
-    long long ctx, per, rows, last;
-    int items;
+    double ctx, per, last;
+    int rows, items;
     bool empty;
     __device__ __forceinline__ Costs(const Seq &q, int tile_tokens) {
+        const int full = ROW_TILES * tile_tokens;
         ctx = q.ctx;
-        per = (long long)ROW_TILES * tile_tokens;
+        per = full;
         rows = q.rows;
         empty = q.empty;
-        items = q.rows > 0 ? (q.rows - 1) / (ROW_TILES * tile_tokens) + 1 : 0;
-        const bool two = ROW_TILES == 2 && rows - (items - 1) * per > tile_tokens;
-        last = R::kItemCost + (empty ? 0 : (two ? R::kRowCost : R::kKeyCost) * (ctx + rows));
+        items = rows > 0 ? (rows - 1) / full + 1 : 0;
+        const bool two = ROW_TILES == 2 && rows - (items - 1) * full > tile_tokens;
+        last = R::kItemCost + (empty ? 0. : (two ? R::kRowCost : R::kKeyCost) * (ctx + rows));
     }
     // Cost of items 0 .. i - 1, i < items (all full).
-    __device__ __forceinline__ long long before(long long i) const {
-        if (empty) return i * R::kItemCost;
-        return i * (R::kRowCost * ctx + R::kItemCost) + R::kRowCost * per * (i * (i + 1) / 2);
+    __device__ __forceinline__ double before(int i) const {
+        const double n = i;
+        if (empty) return n * R::kItemCost;
+        return n * (R::kRowCost * ctx + R::kItemCost) + (0.5 * R::kRowCost * per) * (n * (n + 1.));
     }
-    __device__ __forceinline__ long long head() const { return items ? before(items - 1) + last : 0; }
-    __device__ __forceinline__ long long of(long long i) const { return i + 1 < items ? before(i + 1) - before(i) : last; }
+    __device__ __forceinline__ double head() const { return items ? before(items - 1) + last : 0.; }
+    __device__ __forceinline__ double of(int i) const { return i + 1 < items ? before(i + 1) - before(i) : last; }
 };
 
 struct Pos {
@@ -211,36 +218,32 @@ struct Pos {
 // The place of cost x within sequence s. Rounded to a key tile; within kSnap
 // tiles of an item's ends, to that end.
 template <int ROW_TILES, int KEYS, bool FP8>
-__device__ __forceinline__ Pos locate(const Costs<ROW_TILES, FP8> &c, int s, long long x, int tile_tokens) {
-    // Quotients and the quadratic by 32-bit floats, then put right: 64-bit
-    // division and square root take 3 us here.
-    const long long head = c.head();
+__device__ __forceinline__ Pos locate(const Costs<ROW_TILES, FP8> &c, int s, double x, int tile_tokens) {
+    // Quotients and the quadratic by 32-bit floats, then put right.
+    const double head = c.head();
     int h = (int)__fdividef((float)x, (float)head);
     while (h > 0 && h * head > x) --h;
     while ((h + 1) * head <= x) ++h;
-    long long r = x - h * head;
-    long long lo;  // the last item with before(lo) <= r
-    const float one = (float)(c.empty ? Rates<ROW_TILES, FP8>::kItemCost : c.before(1));
-    if (c.empty) {
-        lo = (long long)__fdividef((float)r, one);
-    } else {
-        const float qa = 0.5f * Rates<ROW_TILES, FP8>::kRowCost * (float)c.per, qb = one - qa;
-        lo = (long long)__fdividef(sqrtf(qb * qb + 4.f * qa * (float)r) - qb, 2.f * qa);
-    }
-    lo = max(0ll, min(lo, (long long)c.items - 1));
+    double r = x - h * head;
+    // The last item lo with before(lo) <= r.
+    const float one = (float)(c.empty ? (double)Rates<ROW_TILES, FP8>::kItemCost : c.before(1));
+    const float qa = c.empty ? 0.f : 0.5f * Rates<ROW_TILES, FP8>::kRowCost * (float)c.per, qb = one - qa;
+    // (sqrt(qb^2 + 4 qa r) - qb) / (2 qa), in the form that holds for qa = 0 too.
+    int lo = (int)__fdividef(2.f * (float)r, qb + sqrtf(qb * qb + 4.f * qa * (float)r));
+    lo = max(0, min(lo, c.items - 1));
     while (lo > 0 && c.before(lo) > r) --lo;
     while (lo + 1 < c.items && c.before(lo + 1) <= r) ++lo;
     r -= c.before(lo);
-    const long long end = c.ctx + min((lo + 1) * c.per, c.rows);
-    const int tiles = c.empty ? 0 : (int)((end + KEYS - 1) / KEYS);
-    const bool two = ROW_TILES == 2 && (lo + 1 < c.items || c.rows - lo * c.per > tile_tokens);
+    const int end = (int)c.ctx + (int)min((lo + 1) * c.per, (double)c.rows);
+    const int tiles = c.empty ? 0 : (end - 1) / KEYS + 1;
+    const bool two = ROW_TILES == 2 && (lo + 1 < c.items || c.rows - lo * ROW_TILES * tile_tokens > tile_tokens);
     const int snap = two ? kSnapRows : kSnapKeys;
-    int t = (int)((float)r / (float)c.of(lo) * (float)tiles + 0.5f);
+    int t = (int)(__fdividef((float)r, (float)c.of(lo)) * (float)tiles + 0.5f);
     if (tiles < 2 * snap) t = 2 * t < tiles ? 0 : tiles;
     else if (t < snap) t = 0;
     else if (tiles - t < snap) t = tiles;
-    Pos p{s, h, (int)lo, t};
-    if (t == tiles && (tiles > 0 || r > 0)) {  // the item's end is the next one's beginning
+    Pos p{s, h, lo, t};
+    if (t == tiles && (tiles > 0 || r > 0.)) {  // the item's end is the next one's beginning
         p.t = 0;
         ++p.i;
     }
@@ -292,7 +295,7 @@ prefill_attention_kernel(const __grid_constant__ CUtensorMap tq, const __grid_co
     unsigned char *sq = smem, *skv = smem + NT * G::kQTile, *sraw = skv + ST * G::kTile;
     float2 *stat = reinterpret_cast<float2 *>(sraw + G::kRawStages * G::kRawTile);
     float *q_factor = reinterpret_cast<float *>(stat + 2 * 128);
-    long long *s_scan = reinterpret_cast<long long *>(stat);  // while the share is found
+    double *s_scan = reinterpret_cast<double *>(stat);  // while the share is found
 
     if (smem_u32(smem) & 1023u) {  // the swizzle's atoms would not line up
         if (tid == 0) record_error(a.err, kDeviceCode, blockIdx.x);
@@ -320,7 +323,7 @@ prefill_attention_kernel(const __grid_constant__ CUtensorMap tq, const __grid_co
         if (tid == 0) s_range[0] = s_range[1] = Pos{a.num_seqs, 0, 0, 0};  // no work
         const int seg = (a.num_seqs + kPrefillThreads - 1) / kPrefillThreads;
         const int b0 = min(a.num_seqs, tid * seg), b1 = min(a.num_seqs, b0 + seg);
-        long long local = 0;
+        double local = 0.;
         Seq mine{0, 0, 0, false};  // the first of this thread's sequences: most often the only one
         for (int s = b0; s < b1; ++s) {
             const Seq q = sequence(a, s, blockIdx.x == 0);
@@ -328,33 +331,31 @@ prefill_attention_kernel(const __grid_constant__ CUtensorMap tq, const __grid_co
             const Costs<NT, G::kFp8> c(q, p.tile_tokens);
             local += c.head() * a.kv_heads;
         }
-        long long incl = local;
+        double incl = local;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
-            const long long y = __shfl_up_sync(0xffffffffu, incl, o);
+            const double y = __shfl_up_sync(0xffffffffu, incl, o);
             if (lane >= o) incl += y;
         }
         if (lane == 31) s_scan[warp] = incl;
         __syncthreads();
-        long long add = 0, total = 0;
+        double add = 0., total = 0.;
 #pragma unroll
         for (int w = 0; w < kPrefillThreads / 32; ++w) {
             if (w < warp) add += s_scan[w];
             total += s_scan[w];
         }
-        const long long first = add + incl - local, n = gridDim.x;
+        const double first = add + incl - local;
 #pragma unroll 1  // run once, from a cold instruction cache: the shorter the better
         for (int e = 0; e < 2; ++e) {
-            const long long b = blockIdx.x + e;
-            // total * b / n, by b times n's reciprocal in 32 fraction bits.
-            const unsigned long long part = (unsigned long long)b * p.share;
-            const long long x = (long long)((__umul64hi(total, part) << 32) | ((unsigned long long)total * part >> 32));
-            if (b < n && x >= first && x < first + local) {
-                long long at = first;
+            const int b = blockIdx.x + e;
+            const double x = floor(total * (b * p.share));
+            if (b < (int)gridDim.x && x >= first && x < first + local) {
+                double at = first;
                 for (int s = b0; s < b1; ++s) {
                     const Seq q = s == b0 ? mine : sequence(a, s, false);
                     const Costs<NT, G::kFp8> c(q, p.tile_tokens);
-                    const long long w = c.head() * a.kv_heads;
+                    const double w = c.head() * a.kv_heads;
                     if (x < at + w) {
                         if (e == 0) s_first = q;
                         s_range[e] = locate<NT, KEYS, G::kFp8>(c, s, x - at, p.tile_tokens);
@@ -520,7 +521,7 @@ prefill_attention_kernel(const __grid_constant__ CUtensorMap tq, const __grid_co
                         for (int e = 0; e < 16; ++e) {
                             float x, y;
                             const uint64_t xy = fma2(pair(s[2 * e], s[2 * e + 1]), sc2, mr2);
-                            if (e % kPolyEvery == kPolyEvery - 1) {
+                            if (!G::kFp8 && e % kPolyEvery == kPolyEvery - 1) {
                                 ex2_poly(xy, x, y);
                             } else {
                                 unpair(xy, x, y);
@@ -1346,7 +1347,7 @@ bool map_2d(CUtensorMap *m, CUtensorMapDataType t, int es, const void *base, lon
     const cuuint64_t strides[1] = {(cuuint64_t)(stride * es)};
     const cuuint32_t box[2] = {(cuuint32_t)box_cols, (cuuint32_t)box_rows}, ones[2] = {1, 1};
     return encoder()(m, t, 2, const_cast<void *>(base), dims, strides, box, ones, CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle,
-                     CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+                     CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
 // A pool plane as [rows / 8][slabs of 64][8 rows][64]: a box is 16 rows of a
@@ -1356,7 +1357,7 @@ bool map_pages(CUtensorMap *m, CUtensorMapDataType t, const void *base, long lon
     const cuuint64_t strides[3] = {(cuuint64_t)(entry * 2), 128, (cuuint64_t)(entry * 16)};
     const cuuint32_t box[4] = {64, 8, (cuuint32_t)slabs, 2}, ones[4] = {1, 1, 1, 1};
     return encoder()(m, t, 4, const_cast<void *>(base), dims, strides, box, ones, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                     CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                     CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
                      CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
@@ -1373,7 +1374,7 @@ cudaError_t launch_tiles(const PrefillLaunch &a, const PrefillWorkspace &ws, int
         const cuuint64_t strides[2] = {(cuuint64_t)D * 2, (cuuint64_t)a.q_stride * 2};
         const cuuint32_t box[3] = {64, (cuuint32_t)a.group, (cuuint32_t)tile_tokens}, ones[3] = {1, 1, 1};
         if (encoder()(&tq, t, 3, const_cast<void *>(a.q), dims, strides, box, ones, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                      CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                      CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
                       CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
             return cudaErrorInvalidValue;
     }
@@ -1390,7 +1391,7 @@ cudaError_t launch_tiles(const PrefillLaunch &a, const PrefillWorkspace &ws, int
     }
     if (!ok) return cudaErrorInvalidValue;
     const int ctas = std::min(sms, ws.ctas);
-    Params p{a, tile_tokens, aligned(a.out, 32), (unsigned)((1ull << 32) / ctas), nullptr, nullptr, nullptr};
+    Params p{a, tile_tokens, aligned(a.out, 32), 1.0 / ctas, nullptr, nullptr, nullptr};
     unsigned char *at = static_cast<unsigned char *>(ws.base);
     p.part_o = reinterpret_cast<float4 *>(at);
     at += (size_t)2 * ws.ctas * G::kSlotRows * D * sizeof(float);
