@@ -25,8 +25,8 @@
  * work on the handle's own blocking CUDA stream, which is ordered with the
  * legacy default stream; device entry points use the stream they are given.
  * Per-handle device state is shared by the calls that use it: the device
- * error word (all entry points), the split workspace of the attention entry
- * points and the sequence order of pkv_paged_attention_plan_dev. Calls on
+ * error word (all entry points), the split workspaces of the attention entry
+ * points (the decode calls' and the prefill calls') and the sequence order of pkv_paged_attention_plan_dev. Calls on
  * one handle that run concurrently on different streams share them too, so
  * give one handle's device calls one stream (or order the streams) when the
  * error word or attention's partial results must stay apart, and do not
@@ -401,7 +401,11 @@ int pkv_rope_and_cache_dev(pkv_backend *b, const int32_t *block_tables, int64_t 
  * recorded and not touched, nor are rows of no sequence. Keys in blocks
  * outside the pool are recorded (InvalidBlock) and skipped; a row left with no
  * key gives zeros and -inf. Positions that a row does not attend may hold
- * anything, NaN and infinities included.
+ * anything, NaN and infinities included. A row's result does not depend on
+ * the rows beside it, but on how its keys are split over CTAs, which follows
+ * from all lengths of the batch (in the last bits).
+ * With max_new_len 1 and at most 16 query heads per kv head (block_size 16) the
+ * call runs the decode kernel.
  *
  * Uses the handle's prefill workspace (a fixed size, see
  * pkv_attention_reserve). */

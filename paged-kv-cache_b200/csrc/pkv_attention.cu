@@ -266,13 +266,41 @@ __device__ __forceinline__ int checked_ctx(const AttnLaunch &a, int seq, bool re
     return ctx;
 }
 
+// The ragged form (a.cu given): sequence s has the packed rows cu[s] .. cu[s + 1],
+// at most one (its token at position ctx[s], ctx counting the tokens before it).
+// False when there is no row to compute; a sequence whose lengths are refused
+// has its rows written as empty by the caller's first split.
+struct RaggedRow {
+    int lo, hi, ctx;
+    bool refused;
+};
+__device__ __forceinline__ bool ragged_row(const AttnLaunch &a, int seq, bool report, RaggedRow *r) {
+    r->lo = __ldg(a.cu + seq);
+    r->hi = __ldg(a.cu + seq + 1);
+    const int before = __ldg(a.ctx + seq);
+    r->refused = false;
+    if (r->lo < 0 || r->hi < r->lo || r->hi > a.num_tokens) {
+        if (report) record_error(a.err, kShapeMismatch, seq);
+        return false;
+    }
+    if (r->lo == r->hi) return false;
+    r->ctx = before + 1;
+    if (r->hi - r->lo > 1 || before < 0 || before >= a.max_ctx) {
+        if (report) record_error(a.err, kShapeMismatch, seq);
+        r->refused = true;
+        return false;
+    }
+    return true;
+}
+
 // T: query and output type. FP8: the pool holds E4M3 codes with per-(layer,
 // kv head) scales; the tiles are converted to f16 in registers and the math
 // runs in f16 (queries too, scaled by a power of two into f16 range), with
 // the K scale folded into the softmax scale and the V scale into the output.
 // MQ: several query tokens per sequence (a.q_len > 1), causal among
-// themselves; without it the kernel is the one-token decode form.
-template <typename T, int D, int NT, bool FP8, bool MQ>
+// themselves; without it the kernel is the one-token decode form. RAGGED: rows
+// given by a.cu (one-token form).
+template <typename T, int D, int NT, bool FP8, bool MQ, bool RAGGED>
 __global__ void __launch_bounds__(kAttnThreads, attn_min_ctas<D, FP8>(NT))
 paged_attention_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtensorMap tv,
                        const AttnLaunch a) {
@@ -297,7 +325,24 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap tk, const __grid_cons
         seq = (int)__ldg(a.order + blockIdx.z);
         if (seq >= a.num_seqs) return;  // not a sequence (a plan made while the lengths changed)
     }
-    const int ctx = checked_ctx(a, seq, threadIdx.x == 0 && split == 0 && kvh == 0);
+    const bool lead = threadIdx.x == 0 && split == 0 && kvh == 0;
+    int row0 = seq, ctx;  // the sequence's row of q and out
+    if constexpr (RAGGED) {
+        RaggedRow r;
+        if (!ragged_row(a, seq, lead, &r)) {
+            if (r.refused && split == 0)
+                for (long long i = (long long)r.lo * a.group + threadIdx.x / 32; i < (long long)r.hi * a.group; i += kAttnWarps) {
+                    const long long sq = i / a.group * a.num_q_heads + (long long)kvh * a.group + i % a.group;
+                    for (int d = lane; d < D; d += 32) static_cast<T *>(a.out)[sq * D + d] = from_float<T>(0.f);
+                    if (lane == 0 && a.lse) a.lse[sq] = -INFINITY;
+                }
+            return;
+        }
+        row0 = r.lo;
+        ctx = r.ctx;
+    } else {
+        ctx = checked_ctx(a, seq, lead);
+    }
     const int nblk = (ctx + kTok - 1) / kTok;
     const int b0 = split * a.blocks_per_split;
     const int b1 = min(nblk, b0 + a.blocks_per_split);
@@ -311,7 +356,7 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap tk, const __grid_cons
     // Query tile: row r < cols is query token r / group (of the sequence's
     // q_len) and head kvh * group + r % group; other rows zero.
     const int cols = MQ ? a.q_len * a.group : a.group;
-    const T *q = static_cast<const T *>(a.q) + (long long)seq * (MQ ? a.q_len : 1) * a.q_seq_stride +
+    const T *q = static_cast<const T *>(a.q) + (long long)row0 * (MQ ? a.q_len : 1) * a.q_seq_stride +
                  (long long)kvh * a.group * D;
     auto q_row = [&](int r) {
         if constexpr (MQ) {
@@ -757,19 +802,22 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap tk, const __grid_cons
 #pragma unroll
         for (int w = 0; w < kAttnWarps; ++w) M = fmaxf(M, mm[w * 16 + row]);
         float L = 0.f, acc = 0.f;
-        if (M != -INFINITY) {
+        if (M != -INFINITY || RAGGED) {
 #pragma unroll
             for (int w = 0; w < kAttnWarps; ++w) {
+                if (RAGGED && ll[w * 16 + row] == 0.f) continue;
                 const float f = exp2f(mm[w * 16 + row] - M);
                 L += ll[w * 16 + row] * f;
                 acc += om[(w * 16 + row) * D + d] * f;
             }
         }
-        const float val = (L > 0.f && !failed) ? acc / L * v_scale : 0.f;
-        const float lse2 = (L > 0.f && !failed) ? M + log2f(L) : -INFINITY;
+        // The ragged form keeps a NaN (of the query, or of a key it attends).
+        const bool some = (RAGGED ? L != 0.f : L > 0.f) && !failed;
+        const float val = some ? acc / L * v_scale : 0.f;
+        const float lse2 = some ? M + log2f(L) : -INFINITY;
         const int qi = MQ ? row / a.group : 0;  // query token of the row
         const long long qh = (long long)kvh * a.group + (row - qi * a.group);
-        const long long sq = ((long long)seq * (MQ ? a.q_len : 1) + qi) * a.num_q_heads + qh;
+        const long long sq = ((long long)row0 * (MQ ? a.q_len : 1) + qi) * a.num_q_heads + qh;
         if (a.num_splits == 1) {
             static_cast<T *>(a.out)[sq * D + d] = from_float<T>(val);
             if (d == 0 && a.lse) a.lse[sq] = lse2 * 0.69314718055994531f;
@@ -783,7 +831,7 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap tk, const __grid_cons
 // Merges the splits of one sequence, all its query tokens and heads: per
 // (token, head) row the weights 2^(lse_i - max) / sum go to shared memory,
 // then every thread combines float4 runs of the partial outputs.
-template <typename T, int D>
+template <typename T, int D, bool RAGGED>
 __global__ void __launch_bounds__(256)
 paged_attention_combine_kernel(const AttnLaunch a) {
     extern __shared__ float s_w[];  // [q_len * num_q_heads][num_splits]
@@ -792,26 +840,36 @@ paged_attention_combine_kernel(const AttnLaunch a) {
     // until that grid has completed and its partials are visible.
     asm volatile("griddepcontrol.wait;" ::: "memory");
     const int seq = blockIdx.x;
-    const int ctx = checked_ctx(a, seq, false);
+    int row0 = seq, ctx;
+    if constexpr (RAGGED) {
+        RaggedRow r;
+        if (!ragged_row(a, seq, false, &r)) return;
+        row0 = r.lo;
+        ctx = r.ctx;
+    } else {
+        ctx = checked_ctx(a, seq, false);
+    }
     const int nblk = (ctx + kTok - 1) / kTok;
     const int used = max(1, (nblk + a.blocks_per_split - 1) / a.blocks_per_split);
     const int rows = a.q_len * a.num_q_heads;  // the sequence's output rows, contiguous
     for (int h = threadIdx.x; h < rows; h += blockDim.x) {
-        const long long sq = (long long)seq * rows + h;
+        const long long sq = (long long)row0 * rows + h;
         const float *lse = a.part_lse + sq * a.num_splits;
         float M = -INFINITY;
         for (int i = 0; i < used; ++i) M = fmaxf(M, lse[i]);
         float den = 0.f;
-        if (M != -INFINITY)
-            for (int i = 0; i < used; ++i) den += exp2f(lse[i] - M);
+        if (M != -INFINITY || RAGGED)
+            for (int i = 0; i < used; ++i)
+                if (!RAGGED || lse[i] != -INFINITY) den += exp2f(lse[i] - M);
+        const bool some = RAGGED ? den != 0.f : den > 0.f;
         for (int i = 0; i < used; ++i)
-            s_w[h * a.num_splits + i] = den > 0.f ? exp2f(lse[i] - M) / den : 0.f;
-        if (a.lse) a.lse[sq] = den > 0.f ? (M + log2f(den)) * 0.69314718055994531f : -INFINITY;
+            s_w[h * a.num_splits + i] = some && (!RAGGED || lse[i] != -INFINITY) ? exp2f(lse[i] - M) / den : 0.f;
+        if (a.lse) a.lse[sq] = some ? (M + log2f(den)) * 0.69314718055994531f : -INFINITY;
     }
     __syncthreads();
     for (int it = threadIdx.x; it < rows * (D / 4); it += blockDim.x) {
         const int h = it / (D / 4), d4 = it - h * (D / 4);
-        const long long sq = (long long)seq * rows + h;
+        const long long sq = (long long)row0 * rows + h;
         const float4 *po = reinterpret_cast<const float4 *>(a.part_o + sq * a.num_splits * D) + d4;
         float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
         for (int i = 0; i < used; ++i) {
@@ -829,10 +887,10 @@ paged_attention_combine_kernel(const AttnLaunch a) {
     }
 }
 
-template <typename T, int D, int NT, bool FP8, bool MQ>
+template <typename T, int D, int NT, bool FP8, bool MQ, bool RAGGED = false>
 cudaError_t launch_main(const AttnLaunch &a, const CUtensorMap *maps, cudaStream_t st) {
     using G = AttnGeom<D, FP8, attn_stages<D, FP8>(NT)>;
-    auto kern = paged_attention_kernel<T, D, NT, FP8, MQ>;
+    auto kern = paged_attention_kernel<T, D, NT, FP8, MQ, RAGGED>;
     cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, G::kSmem);
     if (e != cudaSuccess) return e;
     dim3 grid((unsigned)a.num_splits, (unsigned)a.kv_heads, (unsigned)a.num_seqs);
@@ -843,7 +901,9 @@ template <typename T, int D, bool FP8>
 cudaError_t launch_td(const AttnLaunch &a, const CUtensorMap *maps, cudaStream_t st) {
     if (a.q_len < 1 || a.q_len * a.group > 16) return cudaErrorInvalidValue;
     const bool nt1 = a.q_len * a.group <= 8;
-    cudaError_t e = a.q_len == 1 ? (nt1 ? launch_main<T, D, 1, FP8, false>(a, maps, st)
+    cudaError_t e = a.cu         ? (nt1 ? launch_main<T, D, 1, FP8, false, true>(a, maps, st)
+                                        : launch_main<T, D, 2, FP8, false, true>(a, maps, st))
+                    : a.q_len == 1 ? (nt1 ? launch_main<T, D, 1, FP8, false>(a, maps, st)
                                         : launch_main<T, D, 2, FP8, false>(a, maps, st))
                                  : (nt1 ? launch_main<T, D, 1, FP8, true>(a, maps, st)
                                         : launch_main<T, D, 2, FP8, true>(a, maps, st));
@@ -851,9 +911,9 @@ cudaError_t launch_td(const AttnLaunch &a, const CUtensorMap *maps, cudaStream_t
     if (a.num_splits > 1) {
         const size_t smem = (size_t)a.q_len * a.num_q_heads * a.num_splits * sizeof(float);
         if (smem > 227 * 1024) return cudaErrorInvalidValue;
+        auto combine = a.cu ? paged_attention_combine_kernel<T, D, true> : paged_attention_combine_kernel<T, D, false>;
         if (smem > 48 * 1024 &&
-            (e = cudaFuncSetAttribute(paged_attention_combine_kernel<T, D>,
-                                      cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem)) != cudaSuccess)
+            (e = cudaFuncSetAttribute(combine, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem)) != cudaSuccess)
             return e;
         cudaLaunchConfig_t cfg{};
         cfg.gridDim = dim3((unsigned)a.num_seqs);
@@ -865,7 +925,7 @@ cudaError_t launch_td(const AttnLaunch &a, const CUtensorMap *maps, cudaStream_t
         attr[0].val.programmaticStreamSerializationAllowed = 1;
         cfg.attrs = attr;
         cfg.numAttrs = 1;
-        e = cudaLaunchKernelEx(&cfg, paged_attention_combine_kernel<T, D>, a);
+        e = cudaLaunchKernelEx(&cfg, combine, a);
     }
     return e;
 }

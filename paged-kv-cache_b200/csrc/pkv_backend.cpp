@@ -995,6 +995,16 @@ Status B200Backend::resolve_and_cache_dev(const int32_t *tables, int64_t table_s
     return check("resolve_and_cache", launch_resolve_cache(a, sms_, st));
 }
 
+// The decode kernel's tensor maps of the planes, made on first use.
+Status B200Backend::attention_maps(long long rows) {
+    if (tmaps_ready_) return Status::Ok();
+    const cudaError_t e = make_attention_tmaps(k_plane_, v_plane_, dtype_, (long long)shard_entry_, rows,
+                                               (int)cfg_.head_dim, tmaps_);
+    if (e != cudaSuccess) return device_error("building the attention tensor maps", e);
+    tmaps_ready_ = true;
+    return Status::Ok();
+}
+
 // Decode attention over one layer (no counterpart in the reference: the
 // trait leaves paged_attention for later, crates/paged-kv-core/src/backend.rs:18-22).
 Status B200Backend::paged_attention_dev(int64_t layer, const void *q, DType query, int64_t q_seq_stride,
@@ -1049,12 +1059,8 @@ Status B200Backend::paged_attention_dev(int64_t layer, const void *q, DType quer
     if (rows >= (1ll << 31)) return error(PKV_ERR_DEVICE, 0, 0, "pool too tall for paged attention");
     DeviceGuard g(device_);
     cudaError_t e;
-    if (!tmaps_ready_) {
-        if ((e = make_attention_tmaps(k_plane_, v_plane_, dtype_, (long long)shard_entry_, rows,
-                                      (int)hd, tmaps_)) != cudaSuccess)
-            return device_error("building the attention tensor maps", e);
-        tmaps_ready_ = true;
-    }
+    const Status maps = attention_maps(rows);
+    if (!maps.ok()) return maps;
     AttnLaunch a{};
     a.q = q;
     a.q_seq_stride = q_seq_stride;
@@ -1321,6 +1327,56 @@ Status B200Backend::attention_chunk_dev(int64_t layer, const void *q, DType quer
     if (num_seqs == 0 || num_tokens == 0) return Status::Ok();
     if (!tables || !ctx) return error(PKV_ERR_DEVICE, 0, 0, "null device pointer");
     DeviceGuard g(device_);
+    const float *k_scale = nullptr, *v_scale = nullptr;
+    if (dtype_ == DType::FP8_E4M3) {
+        const long long stride = std::max<long long>((long long)(cfg_.num_layers * cfg_.num_kv_heads), 1);
+        const long long at = layer * (long long)cfg_.num_kv_heads + (long long)(elem_offset() / cfg_.head_dim);
+        k_scale = d_inv_ + 2 * stride + at;
+        v_scale = d_inv_ + 3 * stride + at;
+    }
+    s = prefill_workspace(st);
+    if (!s.ok()) return s;
+    max_new = std::min(max_new, num_tokens);
+    const int64_t group = num_q_heads / kv;
+    // No sequence has more than one row: the decode kernel's ragged form. It is
+    // bound by the K/V stream where the tile kernel, whose 128-row products such
+    // rows leave nearly empty, is bound by the chain of its steps (16 sequences of
+    // up to 15,679 keys, 8 kv heads of 64, f16: 55 us against 73). Its splits go
+    // to the prefill workspace; a call that would need more takes the tile kernel.
+    if (max_new <= 1 && group <= 16 && cfg_.block_size == 16) {
+        AttnLaunch d{};
+        d.num_splits = attention_splits((long long)num_seqs * kv, (int)max_len, sms_, &d.blocks_per_split,
+                                        dtype_ == DType::FP8_E4M3);
+        const size_t parts = (size_t)num_tokens * num_q_heads * d.num_splits;
+        if (d.num_splits == 1 || (parts * (cfg_.head_dim + 1) * sizeof(float) <= prefill_workspace_bytes((int)cfg_.head_dim, sms_) &&
+                                  (size_t)num_q_heads * d.num_splits * sizeof(float) <= 227 * 1024)) {
+            if ((s = attention_maps(rows)).ok() == false) return s;
+            d.q = q;
+            d.q_seq_stride = q_stride;
+            d.out = out;
+            d.lse = lse;
+            d.tables = tables;
+            d.table_stride = table_stride;
+            d.ctx = ctx;
+            d.cu = cu;
+            d.num_tokens = (int)num_tokens;
+            d.num_seqs = (int)num_seqs;
+            d.kv_heads = (int)kv;
+            d.group = (int)group;
+            d.num_q_heads = (int)num_q_heads;
+            d.layer_row0 = (int)(layer * (int64_t)slots_per_layer());
+            d.num_blocks = (int)cfg_.num_blocks;
+            d.max_ctx = (int)max_len;
+            d.scale_log2 = softmax_scale * 1.4426950408889634f;
+            d.k_scale = k_scale;
+            d.v_scale = v_scale;
+            d.err = d_err_;
+            d.part_o = static_cast<float *>(d_prefill_ws_);
+            d.part_lse = d.part_o + parts * cfg_.head_dim;
+            return check("paged_attention_chunk",
+                         launch_paged_attention(d, tmaps_, dtype_, query, (int)cfg_.head_dim, st));
+        }
+    }
     PrefillLaunch a{};
     a.q = q;
     a.q_stride = q_stride;
@@ -1330,10 +1386,10 @@ Status B200Backend::attention_chunk_dev(int64_t layer, const void *q, DType quer
     a.ctx = ctx;
     a.num_seqs = (int)num_seqs;
     a.num_tokens = (int)num_tokens;
-    a.max_new = (int)std::min(max_new, num_tokens);
+    a.max_new = (int)max_new;
     a.max_len = (int)max_len;
     a.kv_heads = (int)kv;
-    a.group = (int)(num_q_heads / kv);
+    a.group = (int)group;
     a.head_dim = (int)cfg_.head_dim;
     a.scale_log2 = softmax_scale * 1.4426950408889634f;
     a.k = k_plane_;
@@ -1344,16 +1400,10 @@ Status B200Backend::attention_chunk_dev(int64_t layer, const void *q, DType quer
     a.block_size = (int)cfg_.block_size;
     a.layer_row0 = layer * (long long)slots_per_layer();
     a.pool_rows = rows;
-    if (dtype_ == DType::FP8_E4M3) {
-        const long long stride = std::max<long long>((long long)(cfg_.num_layers * cfg_.num_kv_heads), 1);
-        const long long at = layer * (long long)cfg_.num_kv_heads + (long long)(elem_offset() / cfg_.head_dim);
-        a.k_scale = d_inv_ + 2 * stride + at;
-        a.v_scale = d_inv_ + 3 * stride + at;
-    }
+    a.k_scale = k_scale;
+    a.v_scale = v_scale;
     a.err = d_err_;
     a.device = device_;
-    s = prefill_workspace(st);
-    if (!s.ok()) return s;
     return check("paged_attention_chunk",
                  launch_prefill_attention(a, query, dtype_, {d_prefill_ws_, sms_}, sms_, st));
 }

@@ -181,6 +181,7 @@ class B200Backend {
     Status upload_inv_scales();
     Status whole_heads(const char *what, int64_t *kv_heads) const;
     Status prefill_workspace(cudaStream_t st);
+    Status attention_maps(long long rows);
     Status check_prefill(const char *what, const void *q, int64_t num_q_heads, int64_t kv_heads,
                          int64_t *q_stride, const int32_t *cu, int64_t num_seqs,
                          int64_t num_tokens, int64_t max_new, int64_t max_len,

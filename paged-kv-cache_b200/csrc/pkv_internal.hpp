@@ -218,6 +218,11 @@ struct AttnLaunch {
     // Optional order of the sequences (pkv_paged_attention_plan_dev): grid
     // slot z runs sequence order[z]. Any permutation gives the same results.
     const unsigned *order = nullptr;
+    // Ragged rows (the chunk entry point where no sequence has more than one):
+    // sequence s has rows cu[s] .. cu[s + 1] of the num_tokens rows of q and out,
+    // ctx counts the tokens before them and max_ctx bounds ctx + 1.
+    const int *cu = nullptr;
+    int num_tokens = 0;
     DevError *err;
 };
 
