@@ -385,7 +385,7 @@ class B200Backend:
         positions, rotary = cos_sin.shape
         _check(lib.pkv_rope_and_cache_dev(
             self._h, _ptr(block_tables), _table_stride(block_tables), _ptr(ctx_lens), _ptr(new_lens),
-            len(ctx_lens), num_tokens, _ptr(cu_out), _ptr(slots_out), layer, _ptr(q), q_pitch, hq,
+            ctx_lens.shape[0], num_tokens, _ptr(cu_out), _ptr(slots_out), layer, _ptr(q), q_pitch, hq,
             _ptr(q_out), qo_pitch, k.data_ptr(), v.data_ptr(), pitch, _ptr(k_out), ko_pitch, tag,
             _ptr(cos_sin), positions, rotary, int(interleaved), self._stream(stream)))
 
@@ -401,7 +401,7 @@ class B200Backend:
         if softmax_scale is None:
             softmax_scale = d ** -0.5
         _check(lib.pkv_paged_attention_chunk_dev(
-            self._h, layer, q.data_ptr(), _tag(q), q.stride(0), hq, _ptr(cu_seqlens), len(ctx_lens), t,
+            self._h, layer, q.data_ptr(), _tag(q), q.stride(0), hq, _ptr(cu_seqlens), ctx_lens.shape[0], t,
             max_new_len, _ptr(block_tables), _table_stride(block_tables), _ptr(ctx_lens),
             max_context_len, softmax_scale, out.data_ptr(), _ptr(lse), self._stream(stream)))
 
@@ -423,7 +423,7 @@ class B200Backend:
             softmax_scale = d ** -0.5
         _check(lib.pkv_prompt_attention_dev(
             self._h, q.data_ptr(), k.data_ptr(), v.data_ptr(), _tag(q), q.stride(0), pitch, hq,
-            _ptr(cu_seqlens), len(cu_seqlens) - 1, t, max_len, softmax_scale, out.data_ptr(),
+            _ptr(cu_seqlens), cu_seqlens.shape[0] - 1, t, max_len, softmax_scale, out.data_ptr(),
             _ptr(lse), self._stream(stream)))
 
     def _stream(self, stream) -> int | None:
