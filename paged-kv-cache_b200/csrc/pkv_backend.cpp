@@ -1338,12 +1338,12 @@ Status B200Backend::attention_chunk_dev(int64_t layer, const void *q, DType quer
     if (!s.ok()) return s;
     max_new = std::min(max_new, num_tokens);
     const int64_t group = num_q_heads / kv;
-    // No sequence has more than one row: the decode kernel's ragged form. It is
+    // A sequence has at most one row: the decode kernel's ragged form. It is
     // bound by the K/V stream where the tile kernel, whose 128-row products such
     // rows leave nearly empty, is bound by the chain of its steps (16 sequences of
     // up to 15,679 keys, 8 kv heads of 64, f16: 55 us against 73). Its splits go
     // to the prefill workspace; a call that would need more takes the tile kernel.
-    if (max_new <= 1 && group <= 16 && cfg_.block_size == 16) {
+    if (max_new == 1 && group <= 16 && cfg_.block_size == 16) {
         AttnLaunch d{};
         d.num_splits = attention_splits((long long)num_seqs * kv, (int)max_len, sms_, &d.blocks_per_split,
                                         dtype_ == DType::FP8_E4M3);

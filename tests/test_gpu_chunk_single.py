@@ -92,6 +92,41 @@ def test_rows_and_keys_that_are_not_finite(cuda, ctx0):
     assert torch.isnan(out[2]).all() and torch.isnan(lse[2]).all() and torch.isfinite(out[0]).all()
 
 
+def test_no_rows_allowed(cuda):
+    """max_new_len 0: a sequence with a row is refused, zeros and a record."""
+    import torch
+
+    b = make_pool(cuda, "bf16", 2, 64)
+    tables = tables_for(np.random.default_rng(7), 128, [9, 9])
+    q = random_rows(cuda, (2, 6, 64), "bf16", seed=3)
+    out, lse = run_chunk(cuda, b, q, tables, [8, 8], [0, 1], max_new=0)
+    err = b.device_error()
+    assert err is not None and isinstance(err[0], ShapeMismatch) and err[1] == 1
+    assert (out[0] == 0).all() and torch.isneginf(lse[0]).all() and torch.isnan(out[1]).all()
+    out, lse = run_chunk(cuda, b, q, tables, [8, 8], [0, 0], max_new=0)
+    assert b.device_error() is None and torch.isnan(out).all()
+
+
+@pytest.mark.parametrize("max_new", [1, 2])
+@pytest.mark.parametrize("d", [64, 128])
+def test_nan_codes_behind_the_sequence(cuda, d, max_new):
+    """An fp8 pool whose slots behind each sequence hold NaN codes, by both kernels."""
+    import torch
+
+    ctx = [40, 700, 2703]
+    b = make_pool(cuda, "fp8_e4m3", 2, d, num_blocks=600, layers=1)
+    tables = tables_for(np.random.default_rng(7), 600, np.add(ctx, 1))
+    for p in b.planes():
+        codes = p.view(torch.uint8)
+        for s, c in enumerate(ctx):
+            codes[0, tables[s, c // 16], c % 16 + 1:] = 0x7F
+    q = random_rows(cuda, (3, 8, d), "bf16", seed=3)
+    out, lse = run_chunk(cuda, b, q, tables, ctx, [1] * 3, layer=0, max_new=max_new)
+    assert b.device_error() is None
+    assert torch.isfinite(out).all()
+    check_chunk(b, q, out, lse, tables, ctx, [1] * 3, 0, "bf16")
+
+
 def test_bad_blocks(cuda):
     import torch
 
