@@ -10,6 +10,7 @@ arrays; the device entry points take CUDA tensors (torch) or raw addresses.
 from __future__ import annotations
 
 import ctypes as C
+import functools
 from typing import Iterable, Sequence
 
 import numpy as np
@@ -383,9 +384,18 @@ class B200Backend:
                 or not cos_sin.is_contiguous()):
             raise ValueError("cos_sin must be a dense f32 [positions][rotary_dim] tensor")
         positions, rotary = cos_sin.shape
+        seqs = ctx_lens.shape[0]
+        int32, int64, _ = _types()
+        table_stride = _table_stride(block_tables, seqs)
+        _dense(ctx_lens, int32, seqs, "ctx_lens")
+        _dense(new_lens, int32, seqs, "new_lens")
+        _dense(cu_out, int32, seqs + 1, "cu_out")
+        if slots_out is not None:
+            _dense(slots_out, int64, num_tokens, "slots_out")
+        self._held(k, v, cos_sin, block_tables, ctx_lens, new_lens, cu_out, q, q_out, k_out, slots_out)
         _check(lib.pkv_rope_and_cache_dev(
-            self._h, _ptr(block_tables), _table_stride(block_tables), _ptr(ctx_lens), _ptr(new_lens),
-            ctx_lens.shape[0], num_tokens, _ptr(cu_out), _ptr(slots_out), layer, _ptr(q), q_pitch, hq,
+            self._h, _ptr(block_tables), table_stride, _ptr(ctx_lens), _ptr(new_lens),
+            seqs, num_tokens, _ptr(cu_out), _ptr(slots_out), layer, _ptr(q), q_pitch, hq,
             _ptr(q_out), qo_pitch, k.data_ptr(), v.data_ptr(), pitch, _ptr(k_out), ko_pitch, tag,
             _ptr(cos_sin), positions, rotary, int(interleaved), self._stream(stream)))
 
@@ -398,11 +408,21 @@ class B200Backend:
         tokens cached before them, lse optional f32 [T][num_q_heads]."""
         t, hq, d = _head_rows(q)
         _dense_out(q, out)
+        if d != self._cfg.head_dim:
+            raise ValueError("q must hold heads of this backend's head_dim")
         if softmax_scale is None:
             softmax_scale = d ** -0.5
+        seqs = ctx_lens.shape[0]
+        int32, _, float32 = _types()
+        table_stride = _table_stride(block_tables, seqs)
+        _dense(ctx_lens, int32, seqs, "ctx_lens")
+        _dense(cu_seqlens, int32, seqs + 1, "cu_seqlens")
+        if lse is not None:
+            _dense(lse, float32, t * hq, "lse")
+        self._held(q, out, cu_seqlens, block_tables, ctx_lens, lse)
         _check(lib.pkv_paged_attention_chunk_dev(
-            self._h, layer, q.data_ptr(), _tag(q), q.stride(0), hq, _ptr(cu_seqlens), ctx_lens.shape[0], t,
-            max_new_len, _ptr(block_tables), _table_stride(block_tables), _ptr(ctx_lens),
+            self._h, layer, q.data_ptr(), _tag(q), q.stride(0), hq, _ptr(cu_seqlens), seqs, t,
+            max_new_len, _ptr(block_tables), table_stride, _ptr(ctx_lens),
             max_context_len, softmax_scale, out.data_ptr(), _ptr(lse), self._stream(stream)))
 
     def prompt_attention(self, q, k, v, cu_seqlens, max_len: int, out,
@@ -421,10 +441,23 @@ class B200Backend:
             raise ValueError("k and v must share shape, strides and dtype")
         if softmax_scale is None:
             softmax_scale = d ** -0.5
+        seqs = cu_seqlens.shape[0] - 1
+        int32, _, float32 = _types()
+        _dense(cu_seqlens, int32, 1, "cu_seqlens")
+        if lse is not None:
+            _dense(lse, float32, t * hq, "lse")
+        self._held(q, k, v, out, cu_seqlens, lse)
         _check(lib.pkv_prompt_attention_dev(
             self._h, q.data_ptr(), k.data_ptr(), v.data_ptr(), _tag(q), q.stride(0), pitch, hq,
-            _ptr(cu_seqlens), cu_seqlens.shape[0] - 1, t, max_len, softmax_scale, out.data_ptr(),
+            _ptr(cu_seqlens), seqs, t, max_len, softmax_scale, out.data_ptr(),
             _ptr(lse), self._stream(stream)))
+
+    def _held(self, *tensors) -> None:
+        """Refuses a tensor (None aside) that is not in this backend's GPU."""
+        device = self.device
+        for t in tensors:
+            if t is not None and t.get_device() != device:
+                raise ValueError("tensors must be on the backend's device")
 
     def _stream(self, stream) -> int | None:
         """cudaStream_t: the current stream of this backend's device by default
@@ -542,9 +575,23 @@ def _current_stream(device: int) -> int:
     return _raw_stream(device)
 
 
-def _table_stride(t) -> int:
+@functools.cache
+def _types():
+    import torch
+
+    return torch.int32, torch.int64, torch.float32
+
+
+def _dense(t, dtype, count: int, what: str) -> None:
+    if t.dtype is not dtype or t.numel() < count or not t.is_contiguous():
+        raise ValueError(f"{what} must be a dense {dtype} tensor of at least {count} elements")
+
+
+def _table_stride(t, seqs: int) -> int:
     shape = t.shape
-    return shape[1] if len(shape) == 2 else 0
+    stride = shape[1] if len(shape) == 2 else 0
+    _dense(t, _types()[0], seqs * stride, "block_tables")
+    return stride
 
 
 def _dense_out(q, out) -> None:

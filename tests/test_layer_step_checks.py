@@ -54,6 +54,50 @@ def test_prompt_attention_refuses_keys(k, v):
         hollow().prompt_attention(rows(4, 4), k, v, i, 4, rows(4, 4))
 
 
+def ints(*shape, dtype=torch.int32):
+    return torch.zeros(shape, dtype=dtype)
+
+
+@pytest.mark.parametrize("what,bad", [
+    ("tables", ints(2, 3, dtype=torch.int64)), ("tables", ints(1, 3)), ("tables", ints(2, 6)[:, ::2]),
+    ("tables", ints(2, 6)[:, :3]), ("ctx", ints(2, dtype=torch.int64)), ("ctx", ints(4)[::2]), ("new", ints(1)),
+    ("new", ints(2, dtype=torch.int64)), ("cu", ints(2)), ("cu", ints(3, dtype=torch.int64)), ("slots", ints(4)),
+    ("slots", ints(3, dtype=torch.int64)), ("lse", torch.zeros(4, 3)), ("lse", torch.zeros(4, 4, dtype=torch.float64)),
+    ("lse", torch.zeros(4, 8)[:, ::2])])
+def test_lengths_tables_and_side_outputs_are_refused(what, bad):
+    """Types, sizes and strides that the kernels would read or write wrongly.
+    (With none of them wrong the tensors' device is refused: they are the CPU's.)"""
+    a = dict(tables=ints(2, 3), ctx=ints(2), new=ints(2), cu=ints(3), slots=ints(4, dtype=torch.int64),
+             lse=torch.zeros(4, 4))
+    b = hollow()
+    b.device = 0
+
+    def rope(a):
+        b.rope_and_cache(a["tables"], a["ctx"], a["new"], 4, a["cu"], rows(4, 4), rows(4, 2), rows(4, 2),
+                         torch.zeros((9, 64)), 0, slots_out=a["slots"])
+
+    def chunk(a):
+        b.paged_attention_chunk(rows(4, 4), a["cu"], a["tables"], a["ctx"], 4, 4, rows(4, 4), 0, lse=a["lse"])
+
+    def prompt(a):
+        b.prompt_attention(rows(4, 4), rows(4, 2), rows(4, 2), a["cu"], 4, rows(4, 4), lse=a["lse"])
+
+    takes = {rope: ("tables", "ctx", "new", "cu", "slots"), chunk: ("tables", "ctx", "cu", "lse"), prompt: ("cu", "lse")}
+    for call, names in takes.items():
+        with pytest.raises(ValueError, match="device"):
+            call(a)
+        if what in names and not (call is prompt and bad.dtype is torch.int32):  # its cu gives the count
+            with pytest.raises(ValueError, match="dense"):
+                call(dict(a, **{what: bad}))
+
+
+def test_chunk_refuses_another_head_dim():
+    """Rows of another head size at a pitch that would cover this backend's."""
+    wide = rows(4, 8, 64)[:, :2]
+    with pytest.raises(ValueError, match="head_dim"):
+        hollow(d=128).paged_attention_chunk(wide, ints(2), ints(1, 1), ints(1), 4, 4, rows(4, 2), 0)
+
+
 def test_rope_table():
     t = rope_table(100001, 64, base=1e6)
     assert t.dtype == np.float32 and t.shape == (100001, 64)
