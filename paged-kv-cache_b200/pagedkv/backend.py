@@ -355,49 +355,51 @@ class B200Backend:
         [head_dim] or None, k and v [T][kv heads][head_dim] with rows of any
         pitch; cos_sin f32 [positions][rotary_dim] (see pagedkv.rope_table);
         q_out None rotates q in place, k_out (rows like k) is optional."""
-        tag = _tag(k)
-        t, hkv, d = _head_rows(k)
-        pitch = k.stride(0)
-        if v.shape != k.shape or v.stride(0) != pitch or v.dtype is not k.dtype or _head_rows(v)[0] != t:
+        tag, dtype = _tag(k), k.dtype
+        int32, int64, float32 = _types()
+        laid = t, hkv, d, pitch = _head_rows(k)
+        if _head_rows(v) != laid or v.dtype is not dtype:
             raise ValueError("k and v must share shape, strides and dtype")
         if hkv * d != self.shard_entry_elems or d != self._cfg.head_dim:
             raise ValueError("k and v must hold the kv heads of this backend")
-        hq = q_pitch = qo_pitch = ko_pitch = 0
-        if q is not None:
-            rows, hq, dq = _head_rows(q)
-            if dq != d or rows < num_tokens or q.dtype is not k.dtype:
-                raise ValueError("q must hold num_tokens rows of k's head_dim and dtype")
-            q_pitch = q.stride(0)
-        if q_out is not None:
-            if q is None or q_out.shape != q.shape or q_out.dtype is not q.dtype:
-                raise ValueError("q_out must have the shape and dtype of q")
-            _head_rows(q_out)
-            qo_pitch = q_out.stride(0)
-        if k_out is not None:
-            if k_out.shape != k.shape or k_out.dtype is not k.dtype:
-                raise ValueError("k_out must have the shape and dtype of k")
-            _head_rows(k_out)
-            ko_pitch = k_out.stride(0)
         if t < num_tokens:
             raise ValueError("num_tokens exceeds the rows")
-        if (cos_sin.dim() != 2 or cos_sin.dtype.itemsize != 4 or not cos_sin.is_floating_point()
-                or not cos_sin.is_contiguous()):
+        hq = q_pitch = qo_pitch = ko_pitch = 0
+        q_at = qo_at = ko_at = slots_at = None
+        if q is not None:
+            rows, hq, dq, q_pitch = _head_rows(q)
+            if dq != d or rows < num_tokens or q.dtype is not dtype:
+                raise ValueError("q must hold num_tokens rows of k's head_dim and dtype")
+            q_at = q.data_ptr()
+        if q_out is not None:
+            if q is None:
+                raise ValueError("q_out without q")
+            *like, qo_pitch = _head_rows(q_out)
+            if like != [rows, hq, d] or q_out.dtype is not dtype:
+                raise ValueError("q_out must have the shape and dtype of q")
+            qo_at = q_out.data_ptr()
+        if k_out is not None:
+            *like, ko_pitch = _head_rows(k_out)
+            if like != [t, hkv, d] or k_out.dtype is not dtype:
+                raise ValueError("k_out must have the shape and dtype of k")
+            ko_at = k_out.data_ptr()
+        if cos_sin.dim() != 2 or cos_sin.dtype is not float32 or not cos_sin.is_contiguous():
             raise ValueError("cos_sin must be a dense f32 [positions][rotary_dim] tensor")
         positions, rotary = cos_sin.shape
         seqs = ctx_lens.shape[0]
-        int32, int64, _ = _types()
-        table_stride = _table_stride(block_tables, seqs)
+        table_stride = _table_stride(block_tables, seqs, int32)
         _dense(ctx_lens, int32, seqs, "ctx_lens")
         _dense(new_lens, int32, seqs, "new_lens")
         _dense(cu_out, int32, seqs + 1, "cu_out")
         if slots_out is not None:
             _dense(slots_out, int64, num_tokens, "slots_out")
+            slots_at = slots_out.data_ptr()
         self._held(k, v, cos_sin, block_tables, ctx_lens, new_lens, cu_out, q, q_out, k_out, slots_out)
         _check(lib.pkv_rope_and_cache_dev(
-            self._h, _ptr(block_tables), table_stride, _ptr(ctx_lens), _ptr(new_lens),
-            seqs, num_tokens, _ptr(cu_out), _ptr(slots_out), layer, _ptr(q), q_pitch, hq,
-            _ptr(q_out), qo_pitch, k.data_ptr(), v.data_ptr(), pitch, _ptr(k_out), ko_pitch, tag,
-            _ptr(cos_sin), positions, rotary, int(interleaved), self._stream(stream)))
+            self._h, block_tables.data_ptr(), table_stride, ctx_lens.data_ptr(), new_lens.data_ptr(), seqs,
+            num_tokens, cu_out.data_ptr(), slots_at, layer, q_at, q_pitch, hq, qo_at, qo_pitch, k.data_ptr(),
+            v.data_ptr(), pitch, ko_at, ko_pitch, tag, cos_sin.data_ptr(), positions, rotary, int(interleaved),
+            self._stream(stream)))
 
     def paged_attention_chunk(self, q, cu_seqlens, block_tables, ctx_lens, max_new_len: int,
                               max_context_len: int, out, layer: int,
@@ -406,7 +408,7 @@ class B200Backend:
         (pkv_paged_attention_chunk_dev): q and out [T][num_q_heads][head_dim],
         sequence s at rows cu_seqlens[s] .. cu_seqlens[s + 1], ctx_lens the
         tokens cached before them, lse optional f32 [T][num_q_heads]."""
-        t, hq, d = _head_rows(q)
+        t, hq, d, q_pitch = _head_rows(q)
         _dense_out(q, out)
         if d != self._cfg.head_dim:
             raise ValueError("q must hold heads of this backend's head_dim")
@@ -414,15 +416,15 @@ class B200Backend:
             softmax_scale = d ** -0.5
         seqs = ctx_lens.shape[0]
         int32, _, float32 = _types()
-        table_stride = _table_stride(block_tables, seqs)
+        table_stride = _table_stride(block_tables, seqs, int32)
         _dense(ctx_lens, int32, seqs, "ctx_lens")
         _dense(cu_seqlens, int32, seqs + 1, "cu_seqlens")
         if lse is not None:
             _dense(lse, float32, t * hq, "lse")
         self._held(q, out, cu_seqlens, block_tables, ctx_lens, lse)
         _check(lib.pkv_paged_attention_chunk_dev(
-            self._h, layer, q.data_ptr(), _tag(q), q.stride(0), hq, _ptr(cu_seqlens), seqs, t,
-            max_new_len, _ptr(block_tables), table_stride, _ptr(ctx_lens),
+            self._h, layer, q.data_ptr(), _tag(q), q_pitch, hq, cu_seqlens.data_ptr(), seqs, t,
+            max_new_len, block_tables.data_ptr(), table_stride, ctx_lens.data_ptr(),
             max_context_len, softmax_scale, out.data_ptr(), _ptr(lse), self._stream(stream)))
 
     def prompt_attention(self, q, k, v, cu_seqlens, max_len: int, out,
@@ -431,13 +433,13 @@ class B200Backend:
         (pkv_prompt_attention_dev): q and out [T][num_q_heads][head_dim], k and
         v [T][kv heads][head_dim], sequence s at rows cu_seqlens[s] ..
         cu_seqlens[s + 1], lse optional f32 [T][num_q_heads]."""
-        t, hq, d = _head_rows(q)
+        t, hq, d, q_pitch = _head_rows(q)
         _dense_out(q, out)
-        pitch = k.stride(0)
-        if (_head_rows(k) != (t, self.shard_entry_elems // self._cfg.head_dim, d) or k.dtype is not q.dtype
+        laid = _head_rows(k)
+        if (laid[:3] != (t, self.shard_entry_elems // self._cfg.head_dim, d) or k.dtype is not q.dtype
                 or d != self._cfg.head_dim):
             raise ValueError("k and v must hold q's rows, the kv heads of this backend, q's dtype")
-        if v.shape != k.shape or v.stride(0) != pitch or v.dtype is not k.dtype or _head_rows(v)[0] != t:
+        if _head_rows(v) != laid or v.dtype is not k.dtype:
             raise ValueError("k and v must share shape, strides and dtype")
         if softmax_scale is None:
             softmax_scale = d ** -0.5
@@ -448,8 +450,8 @@ class B200Backend:
             _dense(lse, float32, t * hq, "lse")
         self._held(q, k, v, out, cu_seqlens, lse)
         _check(lib.pkv_prompt_attention_dev(
-            self._h, q.data_ptr(), k.data_ptr(), v.data_ptr(), _tag(q), q.stride(0), pitch, hq,
-            _ptr(cu_seqlens), seqs, t, max_len, softmax_scale, out.data_ptr(),
+            self._h, q.data_ptr(), k.data_ptr(), v.data_ptr(), _tag(q), q_pitch, laid[3], hq,
+            cu_seqlens.data_ptr(), seqs, t, max_len, softmax_scale, out.data_ptr(),
             _ptr(lse), self._stream(stream)))
 
     def _held(self, *tensors) -> None:
@@ -543,13 +545,20 @@ def _same_layout(k, v) -> None:
         raise ValueError("entries must be contiguous")
 
 
-def _head_rows(x) -> tuple[int, int, int]:
-    """(rows, heads, head_dim) of a [rows][heads][head_dim] tensor whose rows
-    are dense and may lie at any pitch."""
-    shape, stride = x.shape, x.stride()
-    if len(shape) != 3 or stride[2] != 1 or (stride[1] != shape[2] and shape[1] > 1):
+def _head_rows(x) -> tuple[int, int, int, int]:
+    """(rows, heads, head_dim, row pitch) of a [rows][heads][head_dim] tensor
+    whose rows are dense and may lie at any pitch that keeps them apart (0, the
+    dense one, where there are not two)."""
+    if x.dim() != 3:
+        raise ValueError("rows must be [rows][heads][head_dim]")
+    (rows, heads, dim), (pitch, head_pitch, unit) = x.shape, x.stride()
+    if unit != 1 or (head_pitch != dim and heads > 1):
         raise ValueError("rows must be contiguous [heads][head_dim]")
-    return shape[0], shape[1], shape[2]
+    if rows < 2:
+        return rows, heads, dim, 0
+    if pitch < heads * dim:
+        raise ValueError("rows must not overlap")
+    return rows, heads, dim, pitch
 
 
 # Dtype tags, and torch's call for a device's current stream: looked up once,
@@ -587,10 +596,10 @@ def _dense(t, dtype, count: int, what: str) -> None:
         raise ValueError(f"{what} must be a dense {dtype} tensor of at least {count} elements")
 
 
-def _table_stride(t, seqs: int) -> int:
+def _table_stride(t, seqs: int, int32) -> int:
     shape = t.shape
     stride = shape[1] if len(shape) == 2 else 0
-    _dense(t, _types()[0], seqs * stride, "block_tables")
+    _dense(t, int32, seqs * stride, "block_tables")
     return stride
 
 

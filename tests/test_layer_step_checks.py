@@ -98,6 +98,22 @@ def test_chunk_refuses_another_head_dim():
         hollow(d=128).paged_attention_chunk(wide, ints(2), ints(1, 1), ints(1), 4, 4, rows(4, 2), 0)
 
 
+def test_rows_that_lie_over_one_another_are_refused():
+    """Expanded rows (pitch 0), or rows at less than their own length."""
+    one, i = rows(1, 4), ints(2)
+    b = hollow(heads=4)
+    for r in (one.expand(4, 4, 64), torch.zeros(600, dtype=torch.bfloat16).as_strided((4, 4, 64), (64, 64, 1))):
+        with pytest.raises(ValueError, match="overlap"):
+            b.paged_attention_chunk(r, i, ints(1, 1), ints(1), 4, 4, rows(4, 4), 0)
+        with pytest.raises(ValueError, match="overlap"):
+            b.prompt_attention(rows(4, 4), r, r, i, 4, rows(4, 4))
+        for name in ("q", "k", "q_out", "k_out"):
+            a = dict(dict(q=rows(4, 4), k=rows(4, 4), q_out=rows(4, 4), k_out=rows(4, 4)), **{name: r})
+            with pytest.raises(ValueError, match="overlap"):
+                b.rope_and_cache(ints(1, 1), ints(1), ints(1), 4, i, a["q"], a["k"], r if name == "k" else rows(4, 4),
+                                 torch.zeros((9, 64)), 0, q_out=a["q_out"], k_out=a["k_out"])
+
+
 def test_rope_table():
     t = rope_table(100001, 64, base=1e6)
     assert t.dtype == np.float32 and t.shape == (100001, 64)
