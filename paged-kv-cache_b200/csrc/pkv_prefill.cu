@@ -29,8 +29,23 @@
 // kernel joins an item's partials in order. Everything is derived from the
 // lengths on the device; nothing depends on which CTA finishes first.
 // Roles (16 warps): 8 warps softmax and epilogue, one issues the products, one
-// brings K and V by TMA, one plans items and brings Q, four fill the V tiles
+// brings K and one V by TMA, one plans items and brings Q, four fill the V tiles
 // that a mask crosses (and, over an fp8 pool, convert every tile).
+//
+// Bounds, as measured (kernel and join in a graph; products against 1,630
+// TFLOP/s, a matrix product's rate in a burst):
+// - long rows: a step's chain of products and softmax. 2,048 rows over 32 k keys,
+//   28/4 heads of 128: 866 us, 0.66 of it; a prompt of 8,192: 431 us, 0.68. A
+//   pair of row tiles takes 3,700 cycles a tile of 128 keys, 2,048 of them
+//   products. Under a steady load the power limit lowers the clock to 1.66 GHz
+//   first (926 and 497 us).
+// - prompts of 8,192 rows in ten sequences: 150 us, 0.36: a CTA's start (4 us to
+//   its share, 7 us to its first scores, from a cold instruction cache), the
+//   queries in and outputs out between items, and the join (5 us).
+// - over fp8 (1,657 rows, 32/8 heads of 128): 184 us a call, 0.42: the conversion of K
+//   and V in four warps takes issue slots from the softmax.
+// - head_dim 256 (3,800 rows, 8/4): 50 us, 0.28: one warpgroup's softmax and
+//   its products alternate (1,900 cycles a step of 64 keys, 1,280 of products).
 //
 // Masked keys may hold anything. A masked score is replaced before it is used.
 // A masked value still meets a weight of 0 in the product, and 0 * NaN is NaN,
@@ -104,10 +119,11 @@ struct Geom {
     static constexpr int kGranules = kKeys / 16;
     static constexpr int kSteps = kKeys / 64;                   // 64-key steps of a tile
     // head_dim 128: the scores of a tile's two steps by one product of N = 128
-    // (N = 64 reads Q from shared memory twice as often as it can: its products
-    // took 2,900 cycles a tile in place of 2,100), although the next scores then
-    // wait for both steps' weights. 64: the softmax is longer than the products
-    // in any case, and two buffers keep it from waiting.
+    // (N = 64 reads Q from shared memory as often for half the keys: 48 cycles in
+    // place of 32 a product, 2,476 in place of 2,048 for a tile's products of two
+    // row tiles), although the next scores then wait for both steps' weights:
+    // 941 us in place of 962 on 2,048 rows over 32 k keys. 64: the softmax is
+    // longer than the products in any case, and two buffers keep it from waiting.
     static constexpr bool kWide = D == 128;
     static constexpr int kOCol = kRowTiles * 128;               // after two S buffers of 64 columns a row tile
     static constexpr int kStatBytes = 2 * 128 * 8 + (SRC == kPagedFp8 ? 2 * 256 * 4 : 0);  // and the query rows' factors
@@ -657,8 +673,8 @@ prefill_attention_kernel(const __grid_constant__ CUtensorMap tq, const __grid_co
                 }
                 // A lane has a row of its own: a store would meet 32 lines. Four lanes
                 // exchange 32-byte pieces of their four rows, so that each has one
-                // piece of every row and a store covers whole lines (measured: an
-                // item's stores 5,300 -> 2,000 cycles).
+                // piece of every row and a store covers whole lines. (An item's
+                // outputs take 1,000 to 2,000 of its epilogue's 5,000 cycles.)
                 const bool hi = lane & 2, lo = lane & 1;
                 uint32_t y[2][16];
 #pragma unroll
@@ -1263,7 +1279,10 @@ prefill_attention_kernel(const __grid_constant__ CUtensorMap tq, const __grid_co
 // Joins the partials of one split item, from the CTA whose share the item
 // begins in on: out = sum_i 2^(m_i - M) O_i / sum_i 2^(m_i - M) l_i, in the
 // order of the keys. A thread takes a row and 16 of its elements; a warp's
-// loads are contiguous.
+// loads are contiguous. Bound by latency: a launch, the search for the item's
+// pieces, two dependent loads: about 5 us behind the tile kernel whether few or
+// many items are split. (A block of 1,024 threads for a whole row tile, 8 times
+// fewer blocks: the same within 2 us on every shape tried.)
 constexpr int kJoinElems = 16;
 template <typename T, int D, int ROW_TILES>
 __global__ void __launch_bounds__(128) prefill_join_kernel(const __grid_constant__ Params p, int ctas) {
