@@ -44,8 +44,10 @@
 //   queries in and outputs out between items, and the join (5 us).
 // - over fp8 (1,657 rows, 32/8 heads of 128): 184 us a call, 0.42: the conversion of K
 //   and V in four warps takes issue slots from the softmax.
-// - head_dim 256 (3,800 rows, 8/4): 50 us, 0.28: one warpgroup's softmax and
-//   its products alternate (1,900 cycles a step of 64 keys, 1,280 of products).
+// - head_dim 256: a prompt of 8,192, 8/4 heads, 261 us, 0.64: 1,280 cycles of
+//   products a step of 64 keys, of about 1,900. (Two warpgroups with half of a
+//   row's keys each took the same time, on long rows and short.) 3,800 rows in
+//   three prompts: 50 us, 0.28: start, items' ends and the join.
 //
 // Masked keys may hold anything. A masked score is replaced before it is used.
 // A masked value still meets a weight of 0 in the product, and 0 * NaN is NaN,
