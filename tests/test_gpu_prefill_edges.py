@@ -160,6 +160,41 @@ def test_two_handles_at_once(cuda):
         assert all(torch.equal(o, wants[i]) for o in outs[i])
 
 
+def test_two_graphs_share_the_workspace(cuda):
+    """Captured calls of one handle (split items, single rows, a prompt), their
+    graphs replayed in turn on one stream: each as if alone."""
+    import torch
+
+    b = make_pool(cuda, "bf16", 2, 64, num_blocks=700, layers=1)
+    tables = tables_for(np.random.default_rng(7), 700, [5000, 2000])
+    t = ints(cuda, tables)
+    q = random_rows(cuda, (400, 6, 64), "bf16", seed=3)
+    k, v = (random_rows(cuda, (400, 2, 64), "bf16", seed=s) for s in (4, 5))
+    few, one, cu = ints(cuda, [0, 30, 47]), ints(cuda, [0, 1, 2]), ints(cuda, [0, 390, 400])
+    ctx = ints(cuda, [4900, 1900])
+    calls = [lambda o: b.paged_attention_chunk(q, few, t, ctx, 30, 5000, o, 0),
+             lambda o: b.paged_attention_chunk(q, one, t, ctx, 1, 5000, o, 0),
+             lambda o: b.prompt_attention(q, k, v, cu, 390, o)]
+    wants, outs, graphs = [], [], []
+    for call in calls:
+        wants.append(torch.zeros_like(q))
+        call(wants[-1])
+    torch.cuda.synchronize()
+    for call in calls:
+        outs.append(torch.zeros_like(q))
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1]):
+            call(outs[-1])
+    for order in ((0, 1, 2), (2, 0, 1), (1, 1, 0, 0, 2)):
+        for o in outs:
+            o.zero_()
+        for i in order:
+            graphs[i].replay()
+        torch.cuda.synchronize()
+        assert b.device_error() is None
+        assert all(torch.equal(o, w) for o, w in zip(outs, wants))
+
+
 @pytest.mark.parametrize("seed", range(8))
 def test_random_batches(cuda, seed):
     rng = np.random.default_rng(seed)
