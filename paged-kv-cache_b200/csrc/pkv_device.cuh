@@ -36,11 +36,12 @@ __device__ __forceinline__ unsigned long long elem_hash(long long gidx, int plan
     return mix64(((unsigned long long)gidx * 2 + plane) * 0x9E3779B97F4A7C15ull + bits);
 }
 
-__device__ __forceinline__ int warp_inclusive_scan(int x) {
+// Modulo 2^32: the sums that do not fit are found apart (scan_lengths).
+__device__ __forceinline__ unsigned warp_inclusive_scan(unsigned x) {
     const int lane = threadIdx.x & 31;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-        const int y = __shfl_up_sync(0xffffffffu, x, o);
+        const unsigned y = __shfl_up_sync(0xffffffffu, x, o);
         if (lane >= o) x += y;
     }
     return x;
@@ -48,7 +49,10 @@ __device__ __forceinline__ int warp_inclusive_scan(int x) {
 
 // Exclusive prefix of new_lens into s_cu[0..num_seqs] (one contiguous
 // segment per thread, then warp shuffles); sets *s_bad when a length or a
-// context is negative. Every thread of the CTA must call it.
+// context is negative or the sum does not fit 31 bits (s_cu is then no
+// prefix). The scan is modulo 2^32. A step of the prefix adds less than 2^31,
+// so the first prefix that passes 31 bits still shows it in bit 31: each is
+// checked as it is written. Every thread of the CTA must call it.
 __device__ __forceinline__ void scan_lengths(const int *__restrict__ ctx,
                                              const int *__restrict__ nnew, int num_seqs,
                                              int *s_cu, int *s_warp, int *s_bad) {
@@ -58,27 +62,28 @@ __device__ __forceinline__ void scan_lengths(const int *__restrict__ ctx,
     const int seg = (num_seqs + kThreads - 1) / kThreads;
     const int b0 = min(num_seqs, tid * seg);
     const int b1 = min(num_seqs, b0 + seg);
-    int local = 0;
+    unsigned local = 0;
     for (int q = b0; q < b1; ++q) {
         const int n = __ldg(nnew + q);
         if (n < 0 || __ldg(ctx + q) < 0) *s_bad = 1;
         local += max(n, 0);
     }
-    const int incl = warp_inclusive_scan(local);
-    if ((tid & 31) == 31) s_warp[tid >> 5] = incl;
+    const unsigned incl = warp_inclusive_scan(local);
+    if ((tid & 31) == 31) s_warp[tid >> 5] = (int)incl;
     __syncthreads();
     if (tid < 32) {
-        const int w = tid < kThreads / 32 ? s_warp[tid] : 0;
-        const int wi = warp_inclusive_scan(w);
-        if (tid < kThreads / 32) s_warp[tid] = wi - w;
+        const unsigned w = tid < kThreads / 32 ? (unsigned)s_warp[tid] : 0u;
+        const unsigned wi = warp_inclusive_scan(w);
+        if (tid < kThreads / 32) s_warp[tid] = (int)(wi - w);
     }
     __syncthreads();
-    int run = s_warp[tid >> 5] + incl - local;
+    unsigned run = (unsigned)s_warp[tid >> 5] + incl - local;
     for (int q = b0; q < b1; ++q) {
-        s_cu[q] = run;
+        s_cu[q] = (int)run;
         run += max(__ldg(nnew + q), 0);
+        if ((int)run < 0) *s_bad = 1;
     }
-    if (b1 == num_seqs && b0 < b1) s_cu[num_seqs] = run;
+    if (b1 == num_seqs && b0 < b1) s_cu[num_seqs] = (int)run;
     if (num_seqs == 0 && tid == 0) s_cu[0] = 0;
     __syncthreads();
 }

@@ -139,11 +139,11 @@ __device__ __forceinline__ Place place_of_token(const RopeCacheLaunch &a, const 
 
 // The prefix of new_lens in s_cu, published to cu_seqlens by the first CTA.
 // The number of rows that hold tokens, or -1 when the lengths are refused: a
-// negative one, or more tokens than rows.
+// negative one, a sum beyond 31 bits, or more tokens than rows.
 __device__ __forceinline__ long long scan_tokens(const RopeCacheLaunch &a, int *s_cu, int *s_warp, int *s_bad) {
     scan_lengths(a.ctx_lens, a.new_lens, (int)a.num_seqs, s_cu, s_warp, s_bad);
     const long long total = s_cu[a.num_seqs];
-    const bool refused = *s_bad || total < 0 || total > a.num_tokens;
+    const bool refused = *s_bad || total > a.num_tokens;
     if (blockIdx.x == 0) {
         for (int q = threadIdx.x; q <= a.num_seqs; q += kThreads) a.cu_seqlens[q] = s_cu[q];
         if (threadIdx.x == 0 && refused) record_error(a.err, kShapeMismatch, *s_bad ? -1 : total);
