@@ -391,7 +391,7 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap tk, const __grid_cons
         if (qmax < INFINITY) frexpf(qmax, &ex);
         const int e = max(0, ex - 14);
         const float down = ldexpf(1.f, -e);
-        c *= __ldg(a.k_scale + a.scale_row + kvh) * ldexpf(1.f, e);
+        c = fmaxf(c * (__ldg(a.k_scale + a.scale_row + kvh) * ldexpf(1.f, e)), kLeastFp8Scale);
         v_scale = __ldg(a.v_scale + a.scale_row + kvh);
         for (int i = threadIdx.x; i < 16 * (D / 8); i += kAttnThreads) {
             const int r = i / (D / 8), cc = i - r * (D / 8);

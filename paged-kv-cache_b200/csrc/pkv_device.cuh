@@ -6,6 +6,7 @@
 #include <cuda_runtime.h>
 
 #include <algorithm>
+#include <cfloat>
 #include <cstdint>
 #include <initializer_list>
 
@@ -87,6 +88,13 @@ __device__ __forceinline__ void scan_lengths(const int *__restrict__ ctx,
     if (num_seqs == 0 && tid == 0) s_cu[0] = 0;
     __syncthreads();
 }
+
+// The least softmax scale (base 2) of scores over E4M3 codes. It is a product
+// (softmax scale, K scale, the power of two that the queries were divided by)
+// which may underflow, and 0 times the -inf of a masked score would be NaN.
+// |q . k| over codes and f16 queries stays below 2^33, so from here down every
+// key weighs the same.
+constexpr float kLeastFp8Scale = FLT_MIN;
 
 // Programmatic dependent launch. A grid launched with programmatic stream
 // serialization may be set up while the previous grid in its stream still

@@ -451,7 +451,10 @@ prefill_attention_kernel(const __grid_constant__ CUtensorMap tq, const __grid_co
             int others = two && w ? max(0, min(it.t1, (it.key0 + min(p.tile_tokens, it.tokens) + KEYS - 1) / KEYS) - it.t0) : n;
             if (keys) mine = (n - w + 1) / 2, others = (n - (w ^ 1) + 1) / 2;
             float scale = a.scale_log2, v_scale = 1.f;
-            if constexpr (SRC == kPagedFp8) scale *= __ldg(a.k_scale + it.head), v_scale = __ldg(a.v_scale + it.head);
+            if constexpr (SRC == kPagedFp8) {
+                scale *= __ldg(a.k_scale + it.head), v_scale = __ldg(a.v_scale + it.head);
+                if constexpr (!kScaleQ) scale = fmaxf(scale, kLeastFp8Scale);
+            }
             float m = -INFINITY, l = 0.f;
             const bool warp_live = __any_sync(0xffffffffu, live);
             const int careful = first_careful(it);
@@ -465,7 +468,8 @@ prefill_attention_kernel(const __grid_constant__ CUtensorMap tq, const __grid_co
                     s_ph ^= 1u << (i & 1);
                     fence_after();
                 }
-                if (kScaleQ && i == 0) scale *= q_factor[(qn & 1) * 256 + (two ? w * 128 : 0) + row];
+                if (kScaleQ && i == 0)
+                    scale = fmaxf(scale * q_factor[(qn & 1) * 256 + (two ? w * 128 : 0) + row], kLeastFp8Scale);
                 if (warp_live) {
                     const int first_key = t * KEYS + (i % G::kSteps) * 64;
                     const unsigned blocks =
