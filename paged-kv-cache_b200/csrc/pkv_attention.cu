@@ -299,7 +299,10 @@ __device__ __forceinline__ bool ragged_row(const AttnLaunch &a, int seq, bool re
 // the K scale folded into the softmax scale and the V scale into the output.
 // MQ: several query tokens per sequence (a.q_len > 1), causal among
 // themselves; without it the kernel is the one-token decode form. RAGGED: rows
-// given by a.cu (one-token form).
+// given by a.cu (one-token form); bf16 queries over fp8 are scaled by a power
+// of two of each row's own, up or down, as the tile kernel scales them, so that
+// the two forms take the same queries and a head's range is not its
+// neighbours'. (In the other forms a group shares one, which only scales down.)
 template <typename T, int D, int NT, bool FP8, bool MQ, bool RAGGED>
 __global__ void __launch_bounds__(kAttnThreads, attn_min_ctas<D, FP8>(NT))
 paged_attention_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtensorMap tv,
@@ -307,10 +310,12 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap tk, const __grid_cons
     using G = AttnGeom<D, FP8, attn_stages<D, FP8>(NT)>;
     using C = std::conditional_t<FP8, __half, T>;  // tensor-core operand type
     constexpr int kStages = G::kStages;
+    constexpr bool kOwnQuery = FP8 && RAGGED, kRowPower = kOwnQuery && !std::is_same_v<T, __half>;
     extern __shared__ unsigned char smem_raw[];
     __shared__ __align__(8) uint64_t bars[kAttnWarps][kStages];
     __shared__ int s_failed;
     __shared__ int s_qmax;  // fp8: max |q| of the group, as f32 bits
+    __shared__ float s_qdown[16];  // kRowPower: what each row's queries were divided by
     unsigned char *smem = reinterpret_cast<unsigned char *>(
         (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     unsigned char *qs = smem + kAttnWarps * G::kRingBytes;
@@ -368,7 +373,37 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap tk, const __grid_cons
     };
     float c = a.scale_log2;
     float v_scale = 1.f;
-    if constexpr (FP8) {
+    if constexpr (kOwnQuery) {
+        c *= __ldg(a.k_scale + a.scale_row + kvh);
+        if constexpr (!kRowPower) c = fmaxf(c, kLeastFp8Scale);
+        v_scale = __ldg(a.v_scale + a.scale_row + kvh);
+        // A row at a time to a warp, 16 bytes a lane; all of its loads first.
+        constexpr int kRows = 16 / kAttnWarps;
+        uint4 v[kRows];
+#pragma unroll
+        for (int i = 0; i < kRows; ++i) {
+            const int r = warp + i * kAttnWarps;
+            v[i] = make_uint4(0, 0, 0, 0);
+            if (r < cols && lane < D / 8) v[i] = __ldg(reinterpret_cast<const uint4 *>(q_row(r)) + lane);
+        }
+#pragma unroll
+        for (int i = 0; i < kRows; ++i) {
+            const int r = warp + i * kAttnWarps;
+            if constexpr (kRowPower) {
+                const T *e = reinterpret_cast<const T *>(&v[i]);
+                float x[8], top = 0.f;
+#pragma unroll
+                for (int k = 0; k < 8; ++k) top = fmaxf(top, fabsf(x[k] = to_float(e[k])));
+#pragma unroll
+                for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+                const QueryPower pw = query_power(top);
+                if (lane == 0) s_qdown[r] = pw.down;
+                v[i] = make_uint4(pack2<__half>(x[0] * pw.up, x[1] * pw.up), pack2<__half>(x[2] * pw.up, x[3] * pw.up),
+                                  pack2<__half>(x[4] * pw.up, x[5] * pw.up), pack2<__half>(x[6] * pw.up, x[7] * pw.up));
+            }
+            if (lane < D / 8) *reinterpret_cast<uint4 *>(qs + r * G::kQPitch + lane * 16) = v[i];
+        }
+    } else if constexpr (FP8) {
         // f16 holds every E4M3 code exactly; the queries are brought into
         // its range by 2^-e (e > 0 only when some |q| >= 2^14), and 2^e
         // joins the K scale in the softmax scale.
@@ -450,6 +485,20 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap tk, const __grid_cons
             }
         }
     }
+
+    // Softmax scale of this lane's columns ([nt][hc]: head 8nt + 2j + hc).
+    float c_row[NT][2];
+    if constexpr (kRowPower) {
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int hc = 0; hc < 2; ++hc)
+                c_row[nt][hc] = fmaxf(c * s_qdown[nt * 8 + (lane & 3) * 2 + hc], kLeastFp8Scale);
+    }
+    auto scale_of = [&](int nt, int hc) {
+        if constexpr (kRowPower) return c_row[nt][hc];
+        else return c;
+    };
 
     unsigned char *ring = smem + warp * G::kRingBytes;
     const uint32_t ring_u32 = smem_u32(ring);
@@ -681,7 +730,7 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap tk, const __grid_cons
             for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
                 for (int hc = 0; hc < 2; ++hc)  // always on the first block (m = -inf)
-                    grew |= fmaf(fmaxf(sc[nt][hc], sc[nt][2 + hc]), c, -mc[nt][hc]) > 8.0f;
+                    grew |= fmaf(fmaxf(sc[nt][hc], sc[nt][2 + hc]), scale_of(nt, hc), -mc[nt][hc]) > 8.0f;
             if (__any_sync(0xffffffffu, grew)) {
                 // Move every head's reference point to its maximum: rescale
                 // its sum and output by 2^(m_old - m_new).
@@ -695,7 +744,7 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap tk, const __grid_cons
                         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
                         // Finite: one token's blocks all hold a key of the
                         // head; several tokens' mc starts at -FLT_MAX.
-                        const float m_new = fmaxf(mc[nt][hc], mx * c);
+                        const float m_new = fmaxf(mc[nt][hc], mx * scale_of(nt, hc));
                         const float corr = ex2(mc[nt][hc] - m_new);
                         l_run[nt][hc] *= corr;
 #pragma unroll
@@ -714,7 +763,7 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap tk, const __grid_cons
             for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    sc[nt][e] = ex2(fmaf(sc[nt][e], c, -mc[nt][e & 1]));
+                    sc[nt][e] = ex2(fmaf(sc[nt][e], scale_of(nt, e & 1), -mc[nt][e & 1]));
                     l_run[nt][e & 1] += sc[nt][e];
                 }
                 pb[nt][0] = movmatrix_trans(pack2<C>(sc[nt][0], sc[nt][1]));

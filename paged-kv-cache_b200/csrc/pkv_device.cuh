@@ -89,6 +89,21 @@ __device__ __forceinline__ void scan_lengths(const int *__restrict__ ctx,
     __syncthreads();
 }
 
+// bf16 queries over E4M3 codes are held in f16, each row times `up`, the power
+// of two that brings its largest element `top` to [2^13, 2^14) (elements down
+// to 2^-28 of it keep their 8 bits); `down`, its inverse, joins the row's
+// softmax scale. Rows of zeros, below 2^-100 or with an infinity: as they are
+// or nearly.
+struct QueryPower {
+    float up, down;
+};
+__device__ __forceinline__ QueryPower query_power(float top) {
+    int ex = (int)(__float_as_uint(top) >> 23) - 127;  // top = 2^ex * [1, 2)
+    if (ex > 127) ex = 13;
+    ex = max(ex, -100);
+    return {__uint_as_float((unsigned)(13 - ex + 127) << 23), __uint_as_float((unsigned)(ex - 13 + 127) << 23)};
+}
+
 // The least softmax scale (base 2) of scores over E4M3 codes. It is a product
 // (softmax scale, K scale, the power of two that the queries were divided by)
 // which may underflow, and 0 times the -inf of a masked score would be NaN.

@@ -1188,18 +1188,14 @@ prefill_attention_kernel(const __grid_constant__ CUtensorMap tq, const __grid_co
                             float top = fmaxf(__low2float(most), __high2float(most));
 #pragma unroll
                             for (int o = 4; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-                            // top = 2^ex * [1, 2); rows of zeros, tiny or infinite ones: as they are or nearly.
-                            int ex = (int)(__float_as_uint(top) >> 23) - 127;
-                            if (ex > 127) ex = 13;
-                            ex = max(ex, -100);
-                            const float up = __uint_as_float((unsigned)(13 - ex + 127) << 23);
-                            if ((lane & 7) == 0) q_factor[(qn & 1) * 256 + r] = __uint_as_float((unsigned)(ex - 13 + 127) << 23);
+                            const QueryPower pw = query_power(top);
+                            if ((lane & 7) == 0) q_factor[(qn & 1) * 256 + r] = pw.down;
 #pragma unroll
                             for (int c = 0; c < G::kSlabs; ++c) {
                                 const __nv_bfloat162 *e = reinterpret_cast<const __nv_bfloat162 *>(&x[c]);
                                 uint32_t y[4];
 #pragma unroll
-                                for (int i = 0; i < 4; ++i) y[i] = pack2<__half>(__low2float(e[i]) * up, __high2float(e[i]) * up);
+                                for (int i = 0; i < 4; ++i) y[i] = pack2<__half>(__low2float(e[i]) * pw.up, __high2float(e[i]) * pw.up);
                                 q[c * (128 * 128 / 16)] = make_uint4(y[0], y[1], y[2], y[3]);
                             }
                         }
