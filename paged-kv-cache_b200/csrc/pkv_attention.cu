@@ -586,15 +586,13 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap tk, const __grid_cons
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
         for (int mt = 0; mt < D / 16; ++mt) o[nt][mt][0] = o[nt][mt][1] = o[nt][mt][2] = o[nt][mt][3] = 0.f;
-    // With several query tokens the reference points start at -FLT_MAX
-    // rather than -inf, so that a head whose scores are all masked in a block
-    // (a query token before the block's first key) keeps finite arithmetic:
-    // its weights are 2^-inf = 0. With one token every block holds a key of
-    // every head.
+    // The reference points start at -FLT_MAX rather than -inf, so that a head
+    // whose scores in a block are all -inf (masked ones: a query token before
+    // the block's first key; keys at infinity) keeps finite arithmetic: its
+    // weights are 2^-inf = 0.
     float mc[NT][2], l_run[NT][2];
-    constexpr float kM0 = MQ ? -FLT_MAX : -INFINITY;
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt) mc[nt][0] = mc[nt][1] = kM0, l_run[nt][0] = l_run[nt][1] = 0.f;
+    for (int nt = 0; nt < NT; ++nt) mc[nt][0] = mc[nt][1] = -FLT_MAX, l_run[nt][0] = l_run[nt][1] = 0.f;
     // Query token index of this lane's two columns per n-tile, 4 bits each
     // (q_len * group <= 16); padding columns take the last token's limit.
     uint32_t qcols = 0;
@@ -729,7 +727,7 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap tk, const __grid_cons
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-                for (int hc = 0; hc < 2; ++hc)  // always on the first block (m = -inf)
+                for (int hc = 0; hc < 2; ++hc)  // on the first block, and until a score is finite
                     grew |= fmaf(fmaxf(sc[nt][hc], sc[nt][2 + hc]), scale_of(nt, hc), -mc[nt][hc]) > 8.0f;
             if (__any_sync(0xffffffffu, grew)) {
                 // Move every head's reference point to its maximum: rescale
@@ -742,8 +740,6 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap tk, const __grid_cons
                         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
                         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
                         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
-                        // Finite: one token's blocks all hold a key of the
-                        // head; several tokens' mc starts at -FLT_MAX.
                         const float m_new = fmaxf(mc[nt][hc], mx * scale_of(nt, hc));
                         const float corr = ex2(mc[nt][hc] - m_new);
                         l_run[nt][hc] *= corr;

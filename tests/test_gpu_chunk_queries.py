@@ -6,7 +6,7 @@ tests/layer_step.py."""
 import numpy as np
 import pytest
 
-from tests.layer_step import make_pool, tables_for
+from tests.layer_step import ints, make_pool, tables_for
 from tests.test_gpu_prefill_attention import check_chunk, random_rows, run_chunk
 
 pytestmark = pytest.mark.gpu
@@ -63,3 +63,40 @@ def test_fp8_with_scales_whose_product_underflows(cuda, k_scale, scale, zero, qd
     out, lse = run_chunk(cuda, b, q, tables, CTX, ONES, scale=scale, max_new=max_new)
     assert b.device_error() is None
     check_chunk(b, q, out, lse, tables, CTX, ONES, 1, qdtype, scale=scale)
+
+
+@pytest.mark.parametrize("max_new", [1, 2])
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+def test_keys_at_minus_infinity_weigh_nothing(cuda, dtype, max_new):
+    """Whole pages whose scores are -inf, before and between finite ones."""
+    ctx, new = [200, 2700, 70], [1] * 3
+    b = make_pool(cuda, dtype, 1, 64, num_blocks=220, layers=1)
+    tables = tables_for(np.random.default_rng(7), 220, np.add(ctx, 1))
+    k, _ = b.planes()
+    for s, pages in enumerate(([0, 1, 2, 3, 4, 9], list(range(64)) + [100], [0, 1, 2, 3])):
+        k[0, tables[s, pages], :, 5] = -float("inf")
+    q = random_rows(cuda, (3, 4, 64), dtype, seed=3)
+    q[..., 5] = q[..., 5].abs() + 0.5
+    out, lse = run_chunk(cuda, b, q, tables, ctx, new, layer=0, max_new=max_new)
+    assert b.device_error() is None
+    check_chunk(b, q, out, lse, tables, ctx, new, 0, dtype)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+def test_keys_at_minus_infinity_in_decode(cuda, dtype):
+    """The same through decode attention, with one split and several."""
+    import torch
+
+    b = make_pool(cuda, dtype, 1, 64, num_blocks=220, layers=1)
+    k, _ = b.planes()
+    for count in (2, 200):
+        ctx = [200, 70] * (count // 2)
+        tables = np.repeat(tables_for(np.random.default_rng(7), 220, [201]), count, 0)  # shared pages
+        k[0, tables[0, [0, 1, 2, 9]], :, 5] = -float("inf")
+        q = random_rows(cuda, (count, 4, 64), dtype, seed=3)
+        q[..., 5] = q[..., 5].abs() + 0.5
+        out, lse = torch.full_like(q, float("nan")), torch.full((count, 4), float("nan"), device=cuda)
+        b.paged_attention(q, ints(cuda, tables), ints(cuda, np.add(ctx, 1)), 201, out, 0, lse=lse)
+        torch.cuda.synchronize()
+        assert b.device_error() is None
+        check_chunk(b, q, out, lse, tables, ctx, [1] * count, 0, dtype)
