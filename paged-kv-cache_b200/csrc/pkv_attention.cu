@@ -731,7 +731,9 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap tk, const __grid_cons
                     grew |= fmaf(fmaxf(sc[nt][hc], sc[nt][2 + hc]), scale_of(nt, hc), -mc[nt][hc]) > 8.0f;
             if (__any_sync(0xffffffffu, grew)) {
                 // Move every head's reference point to its maximum: rescale
-                // its sum and output by 2^(m_old - m_new).
+                // its sum and output by 2^(m_old - m_new). The ragged form
+                // moves only the heads that ask for it, so that a head's
+                // weights are not rounded differently for the heads beside it.
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -740,6 +742,7 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap tk, const __grid_cons
                         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
                         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
                         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
+                        if (RAGGED && !(fmaf(mx, scale_of(nt, hc), -mc[nt][hc]) > 8.0f)) mx = -INFINITY;
                         const float m_new = fmaxf(mc[nt][hc], mx * scale_of(nt, hc));
                         const float corr = ex2(mc[nt][hc] - m_new);
                         l_run[nt][hc] *= corr;

@@ -100,3 +100,29 @@ def test_keys_at_minus_infinity_in_decode(cuda, dtype):
         torch.cuda.synchronize()
         assert b.device_error() is None
         check_chunk(b, q, out, lse, tables, ctx, [1] * count, 0, dtype)
+
+
+@pytest.mark.parametrize("max_new", [1, 2])
+@pytest.mark.parametrize("pool,qdtype", [("bf16", "bf16"), ("f16", "f16"), ("fp8_e4m3", "bf16"), ("fp8_e4m3", "f16")])
+@pytest.mark.parametrize("d,group", [(64, 4), (128, 7), (128, 16)])
+@pytest.mark.parametrize("factor", [40.0, 0.0, float("nan")])
+def test_a_head_does_not_hang_on_the_heads_beside_it(cuda, factor, d, group, pool, qdtype, max_new):
+    """One head's queries change, and with them how often its maximum grows along
+    the keys: the other heads keep every bit. Few sequences (keys split over
+    CTAs) and many (every CTA walks a whole sequence)."""
+    import torch
+
+    b = make_pool(cuda, pool, 4, d, num_blocks=220, layers=1)
+    hq = 4 * group
+    changed = list(range(1, hq, group))
+    rest = [h for h in range(hq) if h not in changed]
+    for ctx in (CTX, list(range(20, 340, 4))):
+        n = len(ctx)
+        tables = np.repeat(tables_for(np.random.default_rng(7), 220, [2701]), n, 0)  # shared pages
+        q = random_rows(cuda, (n, hq, d), qdtype, seed=3)
+        want, want_lse = run_chunk(cuda, b, q, tables, ctx, [1] * n, layer=0, max_new=max_new)
+        assert torch.isfinite(want).all()
+        q[:, changed] *= factor
+        out, lse = run_chunk(cuda, b, q, tables, ctx, [1] * n, layer=0, max_new=max_new)
+        assert torch.equal(out[:, rest], want[:, rest]) and torch.equal(lse[:, rest], want_lse[:, rest])
+        assert torch.isnan(out[:, changed]).all() == (factor != factor)
