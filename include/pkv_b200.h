@@ -302,8 +302,10 @@ int pkv_paged_attention_dev(pkv_backend *b, int64_t layer, const void *q, int64_
  * it is PKV_BF16 or PKV_F16, and attention reads the dequantised cache,
  * code * scale with the per-(layer, kv head) scales of pkv_set_kv_scales.
  * The codes enter the tensor cores as f16 (exact for every E4M3 value), and
- * so do the queries, scaled by a power of two into f16 range; the scores,
- * softmax and output accumulate in f32. Otherwise as pkv_paged_attention_dev.
+ * so do the queries, scaled up or down into f16 range by a power of two, one
+ * for a sequence's queries of a kv head: a bf16 element is off by at most 2^-23
+ * of the largest of them. The scores, softmax and output accumulate in f32.
+ * Otherwise as pkv_paged_attention_dev.
  * No counterpart in the reference (no attention, no fp8 format). */
 int pkv_paged_attention_typed_dev(pkv_backend *b, int64_t layer, const void *q, int query_dtype,
                                   int64_t q_seq_stride, int64_t num_seqs, int64_t num_q_heads,
@@ -390,7 +392,8 @@ int pkv_rope_and_cache_dev(pkv_backend *b, const int32_t *block_tables, int64_t 
  * cached BEFORE the chunk (as for pkv_rope_and_cache_dev), and attends keys 0
  * .. that position. Any mix of lengths, 0 and 1 (decoded tokens) among them.
  * q is [num_tokens][num_q_heads][head_dim] in query_dtype (as
- * pkv_paged_attention_typed_dev), row pitch q_token_stride elements (<= 0:
+ * pkv_paged_attention_typed_dev, but over an fp8 pool each row of bf16 queries
+ * has a power of two of its own), row pitch q_token_stride elements (<= 0:
  * dense; else a multiple of 8); out is dense; lse (optional, f32
  * [num_tokens][num_q_heads]) receives log(sum exp(scale * q.k)). head_dim 64,
  * 128 or 256, block_size a multiple of 16, at most 128 query heads per kv head.

@@ -302,7 +302,7 @@ __device__ __forceinline__ bool ragged_row(const AttnLaunch &a, int seq, bool re
 // given by a.cu (one-token form); bf16 queries over fp8 are scaled by a power
 // of two of each row's own, up or down, as the tile kernel scales them, so that
 // the two forms take the same queries and a head's range is not its
-// neighbours'. (In the other forms a group shares one, which only scales down.)
+// neighbours'. (In the other forms a group shares one.)
 template <typename T, int D, int NT, bool FP8, bool MQ, bool RAGGED>
 __global__ void __launch_bounds__(kAttnThreads, attn_min_ctas<D, FP8>(NT))
 paged_attention_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtensorMap tv,
@@ -405,8 +405,10 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap tk, const __grid_cons
         }
     } else if constexpr (FP8) {
         // f16 holds every E4M3 code exactly; the queries are brought into
-        // its range by 2^-e (e > 0 only when some |q| >= 2^14), and 2^e
-        // joins the K scale in the softmax scale.
+        // its range by 2^-e, and 2^e joins the K scale in the softmax scale.
+        // e is 0 unless the largest |q| is 2^14 or more, or below 2^-2:
+        // elements below f16's 2^-14 are off by up to 2^-25 then, which is at
+        // most 2^-23 of the largest.
         if (threadIdx.x == 0) s_qmax = 0;
         __syncthreads();
         float mx = 0.f;
@@ -423,10 +425,10 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap tk, const __grid_cons
         __syncthreads();
         const float qmax = __int_as_float(s_qmax);
         int ex = 0;
-        if (qmax < INFINITY) frexpf(qmax, &ex);
-        const int e = max(0, ex - 14);
+        if (qmax < INFINITY) frexpf(qmax, &ex);  // qmax in [2^(ex - 1), 2^ex)
+        const int e = ex > 14 || ex < -1 ? max(ex - 14, -100) : 0;
         const float down = ldexpf(1.f, -e);
-        c = fmaxf(c * (__ldg(a.k_scale + a.scale_row + kvh) * ldexpf(1.f, e)), kLeastFp8Scale);
+        c = fmaxf(c * ldexpf(1.f, e) * __ldg(a.k_scale + a.scale_row + kvh), kLeastFp8Scale);
         v_scale = __ldg(a.v_scale + a.scale_row + kvh);
         for (int i = threadIdx.x; i < 16 * (D / 8); i += kAttnThreads) {
             const int r = i / (D / 8), cc = i - r * (D / 8);
