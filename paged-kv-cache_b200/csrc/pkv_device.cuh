@@ -116,15 +116,17 @@ constexpr float kLeastFp8Scale = FLT_MIN;
 // runs; griddepcontrol.wait then holds it until that grid has completed and
 // its writes are visible (a no-op for a grid launched the ordinary way), so
 // stream order is kept and only the launch and set-up overlap. Called first,
-// by every thread, before any global memory access. The kernels that use it
-// release their dependents only by exiting: a release at entry let the next
-// step's CTAs take SM slots while this step's still streamed, and the decode
-// step got slower (bf16: 5.91 -> 5.98 us, against 5.64 us with the release at
-// exit).
+// by every thread, before any global memory access. Most of the kernels that
+// use it release their dependents only by exiting: a release at entry let the
+// next step's CTAs take SM slots while this step's still streamed, and the
+// decode step got slower (bf16: 5.91 -> 5.98 us, against 5.64 us with the
+// release at exit). The attentions that a combine or a join follows release
+// it early: it waits for their results in any case, and a tile kernel's CTA
+// fills its SM, so that nothing takes a slot beside it.
 __device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 
 // Launches kern<<<grid, block, smem, st>>>(args...) with programmatic stream
-// serialization (the kernel starts with pdl_enter()).
+// serialization (the kernel starts with pdl_wait()).
 template <typename... KArgs, typename... Args>
 inline cudaError_t launch_pdl(void (*kern)(KArgs...), dim3 grid, dim3 block, size_t smem,
                               cudaStream_t st, Args... args) {
