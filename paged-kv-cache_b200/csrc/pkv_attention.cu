@@ -42,6 +42,7 @@
 #include <cstring>
 #include <type_traits>
 
+#include "pkv_async.cuh"
 #include "pkv_device.cuh"
 #include "pkv_internal.hpp"
 
@@ -70,7 +71,6 @@ constexpr int kIdsPerLane =
                                                         : PKV_ATTN_SPLIT_BLOCKS_FP8) + 127) / 128;
 constexpr int kTok = 16;                 // tokens per pool block
 constexpr int kDeviceCode = 9;           // PKV_ERR_DEVICE
-constexpr long long kAttnWaitCycles = 4000000000ll;  // about 2 s at 2 GHz
 
 // Tile geometry. A tile is one pool block of one kv head: 16 rows of D
 // elements, brought in as boxes of 16 rows x up to 128 bytes, swizzled in
@@ -115,48 +115,6 @@ __host__ __device__ constexpr int attn_stages(int nt) {
 template <int D, bool FP8>
 __host__ __device__ constexpr int attn_min_ctas(int nt) {
     return D > 128 ? 2 : FP8 ? (nt == 1 ? 4 : 3) : 3;
-}
-
-__device__ __forceinline__ uint32_t smem_u32(const void *p) {
-    return static_cast<uint32_t>(__cvta_generic_to_shared(p));
-}
-
-__device__ __forceinline__ void mbar_init(uint64_t *bar) {
-    asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(smem_u32(bar)) : "memory");
-}
-
-__device__ __forceinline__ void mbar_expect_tx(uint64_t *bar, uint32_t bytes) {
-    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(smem_u32(bar)), "r"(bytes)
-                 : "memory");
-}
-
-__device__ __forceinline__ bool mbar_try_wait(uint64_t *bar, uint32_t parity) {
-    uint32_t done;
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
-        "selp.u32 %0, 1, 0, p;\n\t}"
-        : "=r"(done)
-        : "r"(smem_u32(bar)), "r"(parity)
-        : "memory");
-    return done != 0;
-}
-
-__device__ __forceinline__ bool mbar_wait_bounded(uint64_t *bar, uint32_t parity) {
-    const long long t0 = clock64();
-    while (!mbar_try_wait(bar, parity))
-        if (clock64() - t0 > kAttnWaitCycles) return false;
-    return true;
-}
-
-// One box of a 2-D tensor map (x = element column, y = row) into shared memory.
-__device__ __forceinline__ void tma_load_2d(void *dst, const CUtensorMap *map, int x, int y,
-                                            uint64_t *bar) {
-    asm volatile(
-        "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
-        " [%0], [%1, {%2, %3}], [%4];" ::"r"(smem_u32(dst)),
-        "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(smem_u32(bar))
-        : "memory");
 }
 
 // ldmatrix of four 8x8 b16 matrices from a shared-memory address.
@@ -572,8 +530,8 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap tk, const __grid_cons
             const int y = a.layer_row0 + blk * kTok;
 #pragma unroll
             for (int hf = 0; hf < G::kBoxes; ++hf) {
-                tma_load_2d(buf + hf * G::kBoxBytes, &tk, kvh * D + hf * G::kBoxElems, y, bar);
-                tma_load_2d(buf + G::kTileBytes + hf * G::kBoxBytes, &tv, kvh * D + hf * G::kBoxElems, y, bar);
+                tma_load_2d(smem_u32(buf + hf * G::kBoxBytes), &tk, kvh * D + hf * G::kBoxElems, y, bar);
+                tma_load_2d(smem_u32(buf + G::kTileBytes + hf * G::kBoxBytes), &tv, kvh * D + hf * G::kBoxElems, y, bar);
             }
         }
     };

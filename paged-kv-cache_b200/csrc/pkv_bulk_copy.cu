@@ -11,7 +11,7 @@
 //
 // Same work and results as copy_blocks_kernel (pkv_kernels.cu); pairs with an
 // id outside the pool are skipped and recorded, self-copies are skipped. Every
-// wait on an mbarrier is bounded: past the budget the kernel records an error,
+// wait on an mbarrier is bounded: past the limit the kernel records an error,
 // drains its own stores and returns.
 
 #include <cuda_runtime.h>
@@ -19,6 +19,7 @@
 #include <algorithm>
 #include <cstdint>
 
+#include "pkv_async.cuh"
 #include "pkv_internal.hpp"
 
 namespace pkv {
@@ -38,44 +39,9 @@ constexpr long long kChunkMax = PKV_BULK_CHUNK_MAX;  // bytes per bulk copy, at 
 constexpr int kCtasPerSm = PKV_BULK_CTAS_PER_SM;
 constexpr int kInvalidBlock = 2;
 constexpr int kDevice = 9;
-constexpr long long kWaitBudgetCycles = 4000000000ll;  // about 2 s at 2 GHz
-
-__device__ __forceinline__ uint32_t smem_u32(const void *p) {
-    return static_cast<uint32_t>(__cvta_generic_to_shared(p));
-}
 
 __device__ __forceinline__ void record(DevError *e, int code, long long index) {
     if (atomicCAS(&e->code, 0, code) == 0) e->index = index;
-}
-
-__device__ __forceinline__ void mbar_init(uint64_t *bar) {
-    asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(smem_u32(bar)) : "memory");
-}
-
-__device__ __forceinline__ void mbar_expect_tx(uint64_t *bar, uint32_t bytes) {
-    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(smem_u32(bar)),
-                 "r"(bytes)
-                 : "memory");
-}
-
-__device__ __forceinline__ bool mbar_try_wait(uint64_t *bar, uint32_t parity) {
-    uint32_t done;
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
-        "selp.u32 %0, 1, 0, p;\n\t}"
-        : "=r"(done)
-        : "r"(smem_u32(bar)), "r"(parity)
-        : "memory");
-    return done != 0;
-}
-
-// Waits for the barrier's phase to complete, for at most kWaitBudgetCycles.
-__device__ __forceinline__ bool mbar_wait_bounded(uint64_t *bar, uint32_t parity) {
-    const long long t0 = clock64();
-    while (!mbar_try_wait(bar, parity))
-        if (clock64() - t0 > kWaitBudgetCycles) return false;
-    return true;
 }
 
 __device__ __forceinline__ void bulk_load(void *smem_dst, const void *gmem_src, uint32_t bytes,

@@ -25,6 +25,15 @@ __device__ __forceinline__ void record_error(DevError *e, int code, long long in
     if (atomicCAS(&e->code, 0, code) == 0) e->index = index;
 }
 
+// E4M3 codes of two f32 values, `lo` in the low byte: round to nearest even,
+// saturating at +-448 (see pkv_set_kv_scales). The PTX conversion writes its
+// first source operand to the upper byte.
+__device__ __forceinline__ uint32_t e4m3x2(float lo, float hi) {
+    unsigned short r;
+    asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(hi), "f"(lo));
+    return r;
+}
+
 // splitmix64 finaliser (Steele, Lea & Flood, 2014): the per-element hash of
 // the plane digests, mix64(((index * 2 + plane) * golden) + f32 bits).
 __device__ __forceinline__ unsigned long long mix64(unsigned long long z) {

@@ -27,14 +27,6 @@
 namespace pkv {
 namespace {
 
-// E4M3 codes of two f32 values, `lo` in the low byte. The PTX conversion
-// writes its first source operand to the upper byte.
-__device__ __forceinline__ uint32_t e4m3x2(float lo, float hi) {
-    unsigned short r;
-    asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(hi), "f"(lo));
-    return r;
-}
-
 __device__ __forceinline__ uint32_t e4m3(float x) { return e4m3x2(x, 0.0f) & 0xffu; }
 
 // f32 bits of an E4M3 code (exact): sign, exponent bias 7 -> 127, 3 mantissa

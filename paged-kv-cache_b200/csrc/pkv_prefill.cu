@@ -79,7 +79,6 @@ namespace {
 using namespace tc;
 
 constexpr int kDeviceCode = 9;                            // PKV_ERR_DEVICE
-constexpr long long kWaitCycles = 4000000000ll;           // about 2 s
 constexpr int kPrefillThreads = 512;
 constexpr int kItemRing = 4;
 constexpr int kMaskRing = 32;                             // key tiles whose block masks are kept

@@ -53,14 +53,6 @@ __device__ __forceinline__ __nv_bfloat16 narrow<__nv_bfloat16>(float x) { return
 template <>
 __device__ __forceinline__ __half narrow<__half>(float x) { return __float2half_rn(x); }
 
-// E4M3 codes of two values, `lo` in the low byte: round to nearest even,
-// saturating at +-448 (the pool's quantisation, see pkv_set_kv_scales).
-__device__ __forceinline__ uint32_t codes2(float lo, float hi) {
-    unsigned short r;
-    asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(hi), "f"(lo));
-    return r;
-}
-
 // Eight consecutive elements as f32.
 template <typename T>
 __device__ __forceinline__ void load8(const T *p, float (&x)[8]) {
@@ -93,10 +85,10 @@ __device__ __forceinline__ void store8(T *p, const float (&x)[8]) {
 
 __device__ __forceinline__ void store8_codes(uint8_t *p, const float (&x)[8], float inv) {
     uint2 w;
-    w.x = codes2(__fmul_rn(x[0], inv), __fmul_rn(x[1], inv)) |
-          (codes2(__fmul_rn(x[2], inv), __fmul_rn(x[3], inv)) << 16);
-    w.y = codes2(__fmul_rn(x[4], inv), __fmul_rn(x[5], inv)) |
-          (codes2(__fmul_rn(x[6], inv), __fmul_rn(x[7], inv)) << 16);
+    w.x = e4m3x2(__fmul_rn(x[0], inv), __fmul_rn(x[1], inv)) |
+          (e4m3x2(__fmul_rn(x[2], inv), __fmul_rn(x[3], inv)) << 16);
+    w.y = e4m3x2(__fmul_rn(x[4], inv), __fmul_rn(x[5], inv)) |
+          (e4m3x2(__fmul_rn(x[6], inv), __fmul_rn(x[7], inv)) << 16);
     __stcs(reinterpret_cast<uint2 *>(p), w);
 }
 
@@ -302,8 +294,8 @@ __global__ void __launch_bounds__(kThreads) rope_cache_any_kernel(const RopeCach
             P *dst = static_cast<P *>(is_k ? a.k_layer : a.v_layer) + (at.slot * a.kv_heads + hh) * a.head_dim;
             if constexpr (FP8) {
                 const float inv = __ldg((is_k ? a.k_inv : a.v_inv) + hh);
-                dst[f0] = (uint8_t)(codes2(__fmul_rn(x, inv), 0.f) & 0xffu);
-                if (pair) dst[f1] = (uint8_t)(codes2(__fmul_rn(y, inv), 0.f) & 0xffu);
+                dst[f0] = (uint8_t)(e4m3x2(__fmul_rn(x, inv), 0.f) & 0xffu);
+                if (pair) dst[f1] = (uint8_t)(e4m3x2(__fmul_rn(y, inv), 0.f) & 0xffu);
             } else {
                 dst[f0] = narrow<T>(x);
                 if (pair) dst[f1] = narrow<T>(y);

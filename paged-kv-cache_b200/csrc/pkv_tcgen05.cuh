@@ -1,6 +1,6 @@
 // pkv_tcgen05.cuh -- the sm_100a instructions that the prefill attention
-// kernel is made of: mbarriers, TMA tile copies, tensor memory, and
-// tcgen05.mma with its descriptors.
+// kernel is made of, beside those of pkv_async.cuh: TMA tile copies, tensor
+// memory, and tcgen05.mma with its descriptors.
 #pragma once
 
 #include <cuda.h>
@@ -10,12 +10,10 @@
 
 #include <cstdint>
 
+#include "pkv_async.cuh"
+
 namespace pkv {
 namespace tc {
-
-__device__ __forceinline__ uint32_t smem_u32(const void *p) {
-    return static_cast<uint32_t>(__cvta_generic_to_shared(p));
-}
 
 // True in one lane of a converged warp. The single-thread roles run under it
 // rather than under lane == 0: the operands of tcgen05.mma and of TMA sit in
@@ -28,29 +26,7 @@ __device__ __forceinline__ bool elect_one() {
     return p != 0;
 }
 
-// ---- mbarriers ---------------------------------------------------------------
-
-__device__ __forceinline__ void mbar_init(uint64_t *bar, uint32_t count) {
-    asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(smem_u32(bar)), "r"(count) : "memory");
-}
-__device__ __forceinline__ void mbar_arrive(uint64_t *bar) {
-    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
-}
-__device__ __forceinline__ void mbar_expect_tx(uint64_t *bar, uint32_t bytes) {
-    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(smem_u32(bar)), "r"(bytes)
-                 : "memory");
-}
-__device__ __forceinline__ bool mbar_try_wait(uint64_t *bar, uint32_t parity) {
-    uint32_t done;
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
-        "selp.u32 %0, 1, 0, p;\n\t}"
-        : "=r"(done)
-        : "r"(smem_u32(bar)), "r"(parity)
-        : "memory");
-    return done != 0;
-}
+// ---- proxies ------------------------------------------------------------------
 
 // Shared-memory writes by ordinary stores, before the async proxy (TMA, the
 // tensor core) touches the same bytes.
@@ -61,13 +37,6 @@ __device__ __forceinline__ void fence_barrier_init() {
 
 // ---- TMA tile loads ------------------------------------------------------------
 
-__device__ __forceinline__ void tma_load_2d(uint32_t dst, const CUtensorMap *map, int x, int y, uint64_t *bar) {
-    asm volatile(
-        "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
-        " [%0], [%1, {%2, %3}], [%4];" ::"r"(dst),
-        "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(smem_u32(bar))
-        : "memory");
-}
 __device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap *map, int x, int y, int z, uint64_t *bar) {
     asm volatile(
         "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
