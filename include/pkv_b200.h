@@ -347,7 +347,8 @@ int pkv_paged_attention_plan_dev(pkv_backend *b, const int32_t *context_lens, in
  * rope_and_cache, then attention of the same tokens: over their own rows for
  * whole prompts (prompt_attention), over the cache for later chunks and for
  * decoded tokens (paged_attention_chunk), which read the cu_seqlens that
- * rope_and_cache wrote. No counterparts in the reference. */
+ * rope_and_cache wrote. Pointers must be aligned to their elements
+ * (PKV_ERR_DEVICE otherwise). No counterparts in the reference. */
 
 /* Appends the new tokens' keys and values to layer `layer` of the pool, the
  * queries and keys rotated by their positions on the way (one launch).
@@ -368,7 +369,8 @@ int pkv_paged_attention_plan_dev(pkv_backend *b, const int32_t *context_lens, in
  * the rotated keys as rows (it may be k), each rounded once to src_dtype; the
  * cache takes them rounded once from f32 (quantised as pkv_set_kv_scales says
  * for an fp8 pool). src_dtype is f32, bf16 or f16 and equals the pool type, or
- * the pool is fp8. Other overlaps of outputs with inputs are not allowed.
+ * the pool is fp8. Rows rotated in place keep their pitch. Other overlaps of
+ * outputs with inputs are not allowed.
  * Writes cu_seqlens[0..num_seqs] and, if given, slot_mapping. The sum of
  * new_lens may be less than num_tokens (a padded batch): rows past it are left
  * as they were. More, or a negative length, is recorded as ShapeMismatch and

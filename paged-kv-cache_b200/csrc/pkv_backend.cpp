@@ -1131,6 +1131,13 @@ Status B200Backend::paged_attention_plan_dev(const int32_t *ctx, int64_t num_seq
     return Status::Ok();
 }
 
+// Whether every pointer (null ones aside) lies at a multiple of `bytes`, a power of two.
+static bool all_aligned(std::initializer_list<const void *> ptrs, uintptr_t bytes) {
+    uintptr_t bits = 0;
+    for (const void *p : ptrs) bits |= reinterpret_cast<uintptr_t>(p);
+    return (bits & (bytes - 1)) == 0;
+}
+
 // The kv heads held here, for calls that work on whole heads.
 Status B200Backend::whole_heads(const char *what, int64_t *kv_heads) const {
     const uint64_t hd = cfg_.head_dim;
@@ -1198,6 +1205,13 @@ Status B200Backend::rope_and_cache_dev(const int32_t *tables, int64_t table_stri
         if (*r.stride <= 0) *r.stride = r.least;
         if (r.used && *r.stride < r.least) return error(PKV_ERR_SHAPE_MISMATCH, r.least, *r.stride, r.what);
     }
+    if (!all_aligned({tables, ctx, new_lens, cu, cos_sin}, 4) || !all_aligned({slots_out}, 8) ||
+        !all_aligned({q, q_out, k, v, k_out}, (uintptr_t)dtype_size(src)))
+        return error(PKV_ERR_DEVICE, 0, 0, "rope_and_cache pointers must be aligned to their elements");
+    if (num_tokens > 1 && ((num_q_heads > 0 && q_out == q && q_out_stride != q_stride) ||
+                           (k_out && k_out == k && k_out_stride != kv_stride)))
+        return error(PKV_ERR_SHAPE_MISMATCH, q_out == q ? q_stride : kv_stride,
+                     q_out == q ? q_out_stride : k_out_stride, "rows rotated in place must keep their pitch");
     DeviceGuard g(device_);
     const size_t layer_bytes = (size_t)layer * slots_per_layer() * entry_bytes();
     RopeCacheLaunch a{};
@@ -1242,7 +1256,7 @@ Status B200Backend::rope_and_cache_dev(const int32_t *tables, int64_t table_stri
 Status B200Backend::check_prefill(const char *what, const void *q, int64_t num_q_heads, int64_t kv_heads,
                                   int64_t *q_stride, const int32_t *cu, int64_t num_seqs,
                                   int64_t num_tokens, int64_t max_new, int64_t max_len,
-                                  float softmax_scale, const void *out) const {
+                                  float softmax_scale, const void *out, const float *lse) const {
     const int64_t hd = (int64_t)cfg_.head_dim;
     if (hd != 64 && hd != 128 && hd != 256)
         return error(PKV_ERR_DEVICE, 0, 0, std::string(what) + " supports head_dim 64, 128 or 256");
@@ -1265,8 +1279,8 @@ Status B200Backend::check_prefill(const char *what, const void *q, int64_t num_q
         return error(PKV_ERR_DEVICE, 0, 0, "softmax scale must be finite and positive");
     if (num_seqs == 0 || num_tokens == 0) return Status::Ok();
     if (!q || !out || !cu) return error(PKV_ERR_DEVICE, 0, 0, "null device pointer");
-    if (reinterpret_cast<uintptr_t>(q) % 16 || reinterpret_cast<uintptr_t>(out) % 16)
-        return error(PKV_ERR_DEVICE, 0, 0, "query and output must be 16-byte aligned");
+    if (!all_aligned({q, out}, 16)) return error(PKV_ERR_DEVICE, 0, 0, "query and output must be 16-byte aligned");
+    if (!all_aligned({cu, lse}, 4)) return error(PKV_ERR_DEVICE, 0, 0, "cu_seqlens and lse must be 4-byte aligned");
     return Status::Ok();
 }
 
@@ -1317,7 +1331,7 @@ Status B200Backend::attention_chunk_dev(int64_t layer, const void *q, DType quer
     Status s = whole_heads("chunk attention", &kv);
     if (!s.ok()) return s;
     s = check_prefill("chunk attention", q, num_q_heads, kv, &q_stride, cu, num_seqs, num_tokens,
-                      max_new, max_len, softmax_scale, out);
+                      max_new, max_len, softmax_scale, out, lse);
     if (!s.ok()) return s;
     if (table_stride < 0 || max_len > table_stride * (int64_t)cfg_.block_size)
         return error(PKV_ERR_SHAPE_MISMATCH, table_stride * (int64_t)cfg_.block_size, max_len,
@@ -1326,6 +1340,8 @@ Status B200Backend::attention_chunk_dev(int64_t layer, const void *q, DType quer
     if (rows >= (1ll << 31)) return error(PKV_ERR_DEVICE, 0, 0, "pool too tall for paged attention");
     if (num_seqs == 0 || num_tokens == 0) return Status::Ok();
     if (!tables || !ctx) return error(PKV_ERR_DEVICE, 0, 0, "null device pointer");
+    if (!all_aligned({tables, ctx}, 4))
+        return error(PKV_ERR_DEVICE, 0, 0, "block tables and lengths must be 4-byte aligned");
     DeviceGuard g(device_);
     const float *k_scale = nullptr, *v_scale = nullptr;
     if (dtype_ == DType::FP8_E4M3) {
@@ -1419,7 +1435,7 @@ Status B200Backend::prompt_attention_dev(const void *q, const void *k, const voi
     Status s = whole_heads("prompt attention", &kv);
     if (!s.ok()) return s;
     s = check_prefill("prompt attention", q, num_q_heads, kv, &q_stride, cu, num_seqs, num_tokens,
-                      max_len, max_len, softmax_scale, out);
+                      max_len, max_len, softmax_scale, out, lse);
     if (!s.ok()) return s;
     const int64_t entry = (int64_t)shard_entry_;
     if (kv_stride <= 0) kv_stride = entry;
@@ -1428,8 +1444,7 @@ Status B200Backend::prompt_attention_dev(const void *q, const void *k, const voi
                      "key and value row pitch must cover the heads and be a multiple of 8 elements");
     if (num_seqs == 0 || num_tokens == 0) return Status::Ok();
     if (!k || !v) return error(PKV_ERR_DEVICE, 0, 0, "null device pointer");
-    if (reinterpret_cast<uintptr_t>(k) % 16 || reinterpret_cast<uintptr_t>(v) % 16)
-        return error(PKV_ERR_DEVICE, 0, 0, "keys and values must be 16-byte aligned");
+    if (!all_aligned({k, v}, 16)) return error(PKV_ERR_DEVICE, 0, 0, "keys and values must be 16-byte aligned");
     DeviceGuard g(device_);
     PrefillLaunch a{};
     a.q = q;

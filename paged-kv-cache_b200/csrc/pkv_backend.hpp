@@ -185,7 +185,7 @@ class B200Backend {
     Status check_prefill(const char *what, const void *q, int64_t num_q_heads, int64_t kv_heads,
                          int64_t *q_stride, const int32_t *cu, int64_t num_seqs,
                          int64_t num_tokens, int64_t max_new, int64_t max_len,
-                         float softmax_scale, const void *out) const;
+                         float softmax_scale, const void *out, const float *lse) const;
     Status check(const char *what, cudaError_t e) const;
 
     pkv_config cfg_{};
