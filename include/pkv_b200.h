@@ -409,8 +409,10 @@ int pkv_rope_and_cache_dev(pkv_backend *b, const int32_t *block_tables, int64_t 
  * anything, NaN and infinities included. A row's result does not depend on
  * the rows beside it, but on how its keys are split over CTAs, which follows
  * from all lengths of the batch (in the last bits).
- * With max_new_len 1 and at most 16 query heads per kv head (block_size 16) the
- * call runs the decode kernel.
+ * Scores, softmax and outputs accumulate in f32; the weights are rounded to
+ * the query type (over an fp8 pool to f16) for the product with V. With
+ * max_new_len 1 and at most 16 query heads per kv head (block_size 16) the call
+ * runs the decode kernel.
  *
  * Uses the handle's prefill workspace (a fixed size, see
  * pkv_attention_reserve). */

@@ -32,22 +32,34 @@
 // brings K and one V by TMA, one plans items and brings Q, four fill the V tiles
 // that a mask crosses (and, over an fp8 pool, convert every tile).
 //
-// Bounds, as measured (kernel and join in a graph; products against 1,630
-// TFLOP/s, a matrix product's rate in a burst):
+// Bounds, as measured (kernel and join, 20 calls in a graph, inputs in L2;
+// products against 1,630 TFLOP/s, a matrix product's rate in a burst):
 // - long rows: a step's chain of products and softmax. 2,048 rows over 32 k keys,
-//   28/4 heads of 128: 866 us, 0.66 of it; a prompt of 8,192: 431 us, 0.68. A
-//   pair of row tiles takes 3,700 cycles a tile of 128 keys, 2,048 of them
-//   products. Under a steady load the power limit lowers the clock to 1.66 GHz
-//   first (926 and 497 us).
-// - prompts of 8,192 rows in ten sequences: 150 us, 0.36: a CTA's start (4 us to
+//   28/4 heads of 128: 829 to 866 us, 0.66 to 0.69 of it; a prompt of 8,192: 432
+//   us, 0.68. A pair of row tiles takes 3,700 cycles a tile of 128 keys, 2,048 of
+//   them products, and no unit is full: a warpgroup's maximum, exponentials and
+//   stores of one 64-key step end before it reads the next one's scores. Under a
+//   steady load the power limit lowers the clock to 1.68 GHz (922 and 498 us).
+// - heads of 64: the same chain, whose products are half and exponentials are as
+//   many: 7 of 8 by the special-function unit, 16 a clock and SM. 2,048 rows over
+//   8 k keys, 32/8 heads: 197 us, 0.45 of that unit's rate; a prompt of 8,192: 421
+//   us, 0.48.
+// - prompts of 8,192 rows in ten sequences: 144 us, 0.37: a CTA's start (4 us to
 //   its share, 7 us to its first scores, from a cold instruction cache), the
 //   queries in and outputs out between items, and the join (5 us).
-// - over fp8 (1,657 rows, 32/8 heads of 128): 184 us a call, 0.42: the conversion of K
-//   and V in four warps takes issue slots from the softmax.
-// - head_dim 256: a prompt of 8,192, 8/4 heads, 261 us, 0.64: 1,280 cycles of
+// - over fp8 (1,657 rows, 32/8 heads of 128): 182 us, 0.43 (195 beside other
+//   allocations): the conversion of K and V in four warps takes issue slots from
+//   the softmax.
+// - head_dim 256: a prompt of 8,192, 8/4 heads, 259 us, 0.65: 1,280 cycles of
 //   products a step of 64 keys, of about 1,900. (Two warpgroups with half of a
 //   row's keys each took the same time, on long rows and short.) 3,800 rows in
-//   three prompts: 50 us, 0.28: start, items' ends and the join.
+//   three prompts: 48 us, 0.29: start, items' ends and the join.
+//
+// Roundings to fewer than 32 bits: scores, statistics and outputs are f32. The
+// weights are rounded to the type of the products (the queries' type; f16 over
+// fp8), which is what the tensor core takes for O += P V; their sum takes them
+// unrounded. An output moves by at most half a step of that type times the mean
+// |v|; f16 holds a weight below 2^-14 of the largest to 2^-25 of the largest.
 //
 // Masked keys may hold anything. A masked score is replaced before it is used.
 // A masked value still meets a weight of 0 in the product, and 0 * NaN is NaN,
@@ -92,10 +104,11 @@ static_assert(2 * (kSoftmaxRegs + kOtherRegs) * 128 <= 128 * kPrefillThreads, "r
 // relative precision, and most tiles skip the rescale of O.
 constexpr float kLazy = 8.0f;
 // One pair of weights in this many is computed on the FMA units, the others by
-// the special-function unit. More would relieve the unit (16 results a clock)
-// but the warps are bound by issue: with every 2nd, 4th, 8th and no pair 2,048
-// rows over 32 k keys took 967, 943, 919 and 930 us, and 1,650 rows over fp8,
-// where the conversions take issue slots too, 220, 212, 202 and 191 us.
+// the special-function unit (16 results a clock). More would relieve the unit
+// but lengthen a step's chain, since a pair takes more instructions there: with
+// every 2nd, 4th and no pair 2,048 rows over 32 k keys took 1.05, 1.03 and 1.01
+// times as long as with every 8th, and 1,650 rows over fp8, where four warps
+// convert beside them, 1.09, 1.05 and 0.95 times (so none there).
 constexpr int kPolyEvery = 8;
 
 enum Source { kPaged = 0, kPagedFp8 = 1, kRows = 2 };
@@ -123,7 +136,7 @@ struct Geom {
     // (N = 64 reads Q from shared memory as often for half the keys: 48 cycles in
     // place of 32 a product, 2,476 in place of 2,048 for a tile's products of two
     // row tiles), although the next scores then wait for both steps' weights:
-    // 941 us in place of 962 on 2,048 rows over 32 k keys. 64: the softmax is
+    // 0.98 of the time on 2,048 rows over 32 k keys. 64: the softmax is
     // longer than the products in any case, and two buffers keep it from waiting.
     static constexpr bool kWide = D == 128;
     static constexpr int kOCol = kRowTiles * 128;               // after two S buffers of 64 columns a row tile
@@ -133,7 +146,8 @@ struct Geom {
     static_assert(kOCol + kRowTiles * D <= 512, "tensor memory");
 };
 
-// Costs, as measured (a row tile pair and 128 keys: 3,700 cycles): a key costs a
+// Costs, as measured at heads of 128 and 256 (a row tile pair and 128 keys of
+// 128: 3,700 cycles); heads of 64 share 128's, not measured apart. A key costs a
 // row item kRowCost, a key item kKeyCost (one row tile, but its K and V come as
 // slowly; over fp8 they are also converted), and an item kItemCost more (queries
 // in, outputs out: 10,000 cycles).

@@ -22,7 +22,8 @@
 // pool, 1.27 GB, 212 us, 0.92 of a device copy's rate; 4,096 tokens of 28/4
 // heads, 81 MB, 15.3 us, 0.81 (the ramp of a launch); 48 single tokens 3.7 us,
 // all of it a launch, the prefix scan and one chain of loads (lengths, table,
-// angles and rows, stores).
+// angles and rows, stores). f32 rows and pool, 4,096 tokens of 28/4 heads, 161
+// MB: 35.7 us, 0.69.
 
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -237,7 +238,10 @@ __global__ void __launch_bounds__(kThreads, 4) rope_cache_kernel(const RopeCache
 }
 
 // Any head size, rotary dimension and alignment: a thread takes one pair (or
-// one pass-through element) of one head.
+// one pass-through element) of one head. Bound by instructions: each pair pays
+// a 64-bit division and the search for its sequence, which the vector form pays
+// once a token, and accesses are of one element. 4,096 tokens of 28/4 heads of
+// 80, 20 of them rotated, bf16: 142 us, 0.05 of a device copy's rate.
 template <typename T, bool FP8>
 __global__ void __launch_bounds__(kThreads) rope_cache_any_kernel(const RopeCacheLaunch a) {
     using P = std::conditional_t<FP8, uint8_t, T>;
